@@ -494,6 +494,95 @@ int  k3g_combine(K3gCtx *ctx, const float *contrib, const int32_t *idx, const fl
 int  k3g_moe_noalloc(const K3gLayer *L, const float *x, int T, float *out, int32_t *idx,
                      float *wt, int *err, void *stream);
 
+/* ----------------------------------------- tokens in expert order and back -- */
+/* The order of k3g_dispatch, and what a caller with experts of its own needs around them:
+ * token rows brought into expert order, expert rows brought back with the router's weights,
+ * and the gradients of both. No reference counterpart (the engine walks its experts one by
+ * one); they take no context and allocate nothing: device pointers, asynchronous on `stream`
+ * (NULL = the null stream), launched on the stream's device, where every pointer must be
+ * readable. Rows are fp32 (K3_WF32) or bf16 (K3_WBF16), tagged by dt, contiguous, of any width
+ * n from 1 to 2^24, at any address their elements may have; sums are fp32 in a fixed order and
+ * rounded once, to nearest even. 1 <= topk <= 64, T topk <= 2^26 pairs; T = 0 is a call without
+ * rows. Outputs must not overlap inputs. Each returns 0, or -1 with a message for arguments it
+ * does not take (nothing is launched then).
+ *
+ * pos [T * topk] says where a pair (t, j) lies among the sorted rows; a value outside
+ * [0, T * topk), -1 as k3g_sort_tokens writes it, leaves the pair out, whatever its weight or
+ * gradient: no row is read or written for it. The kept pairs' places must differ. */
+
+/* Bytes of device memory k3g_sort_tokens works in: 0 for up to 4096 pairs (and for sizes it
+ * does not take). Calls that may overlap need one each. */
+size_t k3g_sort_bytes(int T, int topk, int n_experts);
+/* The pairs t * topk + j grouped by idx [T][topk] (1 to 1024 experts), ascending within an
+ * expert, as k3g_dispatch groups them: off [n_experts + 1] receives each expert's first place
+ * and the kept pairs' count, perm [T * topk] the pair of each place (entries from
+ * off[n_experts] on are left as they were), pos [T * topk] the place of each pair, -1 for a
+ * dropped one (idx < 0). An expert number >= n_experts drops its pair too and sets *err
+ * (device, may be NULL) to 1 if it was 0. work: k3g_sort_bytes, 4-byte aligned. */
+int  k3g_sort_tokens(const int32_t *idx, int T, int topk, int n_experts, int32_t *perm,
+                     int32_t *off, int32_t *pos, int *err, void *work, size_t work_bytes,
+                     void *stream);
+/* sorted[pos[t][j]] = x[t] for every kept pair; other rows of sorted are left as they were. */
+int  k3g_permute(const void *x, int dt, int T, int topk, int n, const int32_t *pos,
+                 void *sorted, void *stream);
+/* Its gradient: dx[t] = sum over kept j, in order, of dsorted[pos[t][j]] (0 when none is). */
+int  k3g_permute_grad(const void *dsorted, int dt, int T, int topk, int n,
+                      const int32_t *pos, void *dx, void *stream);
+/* out[t] = sum over kept j, in order, of wt[t][j] * sorted[pos[t][j]] (products and sums
+ * rounded separately, as k3g_combine's), then + add[t] when add is given ([T][n], dt; its
+ * gradient is dout). wt is fp32. */
+int  k3g_unpermute(const void *sorted, int dt, int T, int topk, int n, const int32_t *pos,
+                   const float *wt, const void *add, void *out, void *stream);
+/* Its gradients, from dout [T][n]: dsorted[pos[t][j]] = wt[t][j] * dout[t] (other rows left as
+ * they were) and dwt [T][topk] = sum_i sorted[pos[t][j]][i] * dout[t][i], 0 for a dropped pair.
+ * dsorted or dwt may be NULL when it is not wanted (frozen experts, a frozen router); sorted
+ * is read for dwt only, wt for dsorted only. */
+int  k3g_unpermute_grad(const void *dout, const void *sorted, int dt, int T, int topk, int n,
+                        const int32_t *pos, const float *wt, void *dsorted, float *dwt,
+                        void *stream);
+
+/* ------------------------------------------------------- MXFP4 both ways -- */
+/* Values quantised to MXFP4 as the checkpoint stores it and read back, and products with both
+ * sides in MXFP4 on the FP4 matrix cores. As above: device pointers, no context, no allocation,
+ * fp32 or bf16 values, the stream's device. cols is a multiple of 32 from 32 to 2^20, rows 0 to
+ * 2^26; value pointers and packed are aligned to 16 bytes. No reference counterpart. */
+
+/* x [rows][cols] -> packed [rows][cols / 2] (low nibble = even column) and E8M0 scales
+ * [rows][cols / 32], by the OCP MX 1.0 rule: with m the largest magnitude of 32 values and
+ * E = max(floor(log2 m) - 2, -127), the scale byte is E + 127 and a code is x / 2^E in E2M1, to
+ * nearest even, clamped to +-6. A block that holds an infinity or a NaN becomes scale 255 (NaN
+ * in the format) and zero codes. k3g_tile_mxfp4 takes the result to the tiled layout; it and
+ * k3_mxfp4_dequant read scale 255 as the engine does, as zeros. */
+int  k3g_quant_mxfp4(const void *x, int dt, int rows, int cols, void *packed, void *scales,
+                     void *stream);
+/* out [rows][cols] = the values packed and scales stand for, exact but where they leave dt's
+ * normal range (nearest even there); a block of scale 255 is NaN. */
+int  k3g_dequant_mxfp4(const void *packed, const void *scales, int rows, int cols, void *out,
+                       int dt, void *stream);
+
+/* Bytes of device memory the products below work in for `rows` rows of x (the quantised rows;
+ * 0 for sizes they do not take). Calls that may overlap need one each. */
+size_t k3g_mxfp4_work_bytes(int rows, int cols);
+/* y [rows][n] = q(x) W^T: x [rows][cols] (xdt) quantised as k3g_quant_mxfp4 does, w the n x cols
+ * matrix in the tiled layout of k3g_tile_mxfp4 (n a multiple of 16 up to 2^20), sums in fp32,
+ * y (ydt) rounded once. A row that holds an infinity or a NaN gives a row of NaN. work:
+ * k3g_mxfp4_work_bytes(rows, cols), aligned to 16 bytes, as w and y are. */
+int  k3g_matmul_mxfp4(const void *x, int xdt, int rows, int cols, const void *w, int n,
+                      void *y, int ydt, void *work, size_t work_bytes, void *stream);
+/* The same for the sorted pairs of n_experts experts: place r of expert e (off[e] <= r <
+ * off[e + 1], off as k3g_sort_tokens writes it) gets y[r] = q(x[row]) W_e^T with row =
+ * perm[r] / topk, or, without perm (NULL, topk 1), row = r: the rows are sorted already. Places
+ * from off[n_experts] on are left as they were. w: the device address of expert 0's pointer to
+ * its tiled matrix, expert e's lies e * w_step bytes on (8 for an array of pointers,
+ * sizeof(K3ExpertQ) for &experts[0].p1 of a layer's table). With w3 (NULL for none) each expert
+ * has a second such matrix and y[r] = act(q(x) W_e^T, q(x) W3_e^T), the layer's activation with
+ * caps b1, b2 (2^64 and above: uncapped, SwiGLU). An expert that has pairs but a NULL matrix
+ * gives rows of zeros. rows * topk <= 2^26. */
+int  k3g_grouped_mxfp4(const void *x, int xdt, int rows, int cols, const int32_t *perm,
+                       int topk, const int32_t *off, int n_experts, const void *const *w,
+                       const void *const *w3, int w_step, int n, float b1, float b2, void *y,
+                       int ydt, void *work, size_t work_bytes, void *stream);
+
 /* Synchronise the stream and report any error a kernel raised on the device
  * (an exhausted bounded wait, a bad expert index). Returns 0 when clean. */
 int  k3g_sync(K3gCtx *ctx, void *stream);

@@ -88,6 +88,13 @@ __device__ __forceinline__ void k3d_wait_vm(int n)
 __device__ __forceinline__ float k3d_bf16lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float k3d_bf16hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 
+/* two floats as bf16 bits, nearest even, a in the low half (v_cvt_pk_bf16_f32) */
+__device__ __forceinline__ uint32_t k3d_bf16x2(float a, float b)
+{
+    typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(k3v2f{a, b}, v2bf));
+}
+
 /* Wave-wide sum, every lane gets the total. */
 /* Exclusive scans, across a block of NW <= 64 waves, of N ints per thread at once: wave
  * scans by shuffles, the waves' totals scanned by wave 0 through lds[(NW + 1) * N]; tot

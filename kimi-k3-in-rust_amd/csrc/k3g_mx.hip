@@ -1,0 +1,440 @@
+/* k3g_mx.hip - MXFP4 beyond the layer's own weights: values quantised to it and read back, and
+ * products of activations quantised to it with weights in it.
+ *
+ * Quantisation (OCP Microscaling Formats 1.0): a block is 32 consecutive values of a row; with
+ * m their largest magnitude, E = max(floor(log2 m) - 2, -127), so m / 2^E lies in [4, 8) and
+ * E2M1's largest value, 6, is reached; the scale byte is E + 127 and a code is x / 2^E in E2M1,
+ * to nearest even, what exceeds 6 as 6. Only exponents are read, so nothing here is rounded but
+ * the codes. A block with an infinity or NaN gets scale byte 255: it is NaN as a whole.
+ *
+ * Product: y[r][i] = sum_k q(x)[row(r)][k] W[i][k], both sides in MXFP4, on
+ * v_mfma_scale_f32_16x16x128_f8f6f4 with FP4 operands, fp32 accumulation. The A operand is the
+ * tiled layout's 1 KB chunk as it lies (lane L: row L % 16, block L / 16 of the 128 columns, its
+ * scale byte with it); the B operand is the same of 16 activation rows. A row of activations is
+ * stored for that as quads of 512 columns, 272 bytes: 16 blocks of 16 bytes in column order,
+ * then 16 scale bytes, block 4 j + q at 4 q + j, so lane (row, q) gets the scales of its four
+ * chunks j in one dword; columns past the last are zero. */
+#include <stdio.h>
+
+#include "k3g_dev.h"
+#include "k3g_gemm.h"
+#include "k3g_host.h"
+#include "k3g_kernels.h"
+
+#define MX_QT 4352                   /* a tiled weight quad: 16 rows x 512 columns */
+#define MX_XQ 272                    /* an activation quad: 1 row x 512 columns */
+#define MX_MAX_ROWS (1 << 26)
+#define MX_MAX_COLS (1 << 20)
+
+typedef int mx_v8i __attribute__((ext_vector_type(8)));
+
+/* ------------------------------------------------------------- quantisation ---- */
+
+/* 8 consecutive values of a row */
+struct Mx8 {
+    float f[8];
+};
+
+__device__ __forceinline__ Mx8 mx_load8(const float *p)
+{
+    const float4 a = *(const float4 *)p, b = *(const float4 *)(p + 4);
+    return {{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+}
+
+__device__ __forceinline__ Mx8 mx_load8(const uint16_t *p)
+{
+    const uint4 a = *(const uint4 *)p;
+    return {{k3d_bf16lo(a.x), k3d_bf16hi(a.x), k3d_bf16lo(a.y), k3d_bf16hi(a.y), k3d_bf16lo(a.z),
+             k3d_bf16hi(a.z), k3d_bf16lo(a.w), k3d_bf16hi(a.w)}};
+}
+
+/* The largest of a value over the four lanes of a quad of lanes */
+__device__ __forceinline__ uint32_t mx_quad_max(uint32_t v)
+{
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));
+}
+
+/* This lane's 8 values of a block that it shares with the three other lanes of its quad: their
+ * codes, element i in nibble i, and the block's scale byte. Magnitudes are compared as bits, so
+ * a NaN is the largest of all. x / 2^E is a multiplication by 2^-E, exact down to 2^-126. */
+__device__ __forceinline__ uint32_t mx_quant8(const Mx8 &x, uint32_t &scale)
+{
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x.f[i]) & 0x7FFFFFFFu);
+    m = mx_quad_max(m);
+    const bool finite = m < 0x7F800000u;
+    const uint32_t byte = finite ? (uint32_t)max((int)(m >> 23) - 2, 0) : 127u;
+    const float inv = __uint_as_float((254u - byte) << 23);
+    uint32_t c = 0;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __builtin_amdgcn_fmed3f(x.f[i] * inv, -6.0f, 6.0f);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[0], v[1], 1.0f, 0);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2], v[3], 1.0f, 1);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[4], v[5], 1.0f, 2);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6], v[7], 1.0f, 3);
+    scale = finite ? byte : 255u;
+    return finite ? c : 0u;
+}
+
+/* Four lanes per block, 8 values a lane: loads of 16 bytes a lane and stores of 4, each row of
+ * whole blocks. */
+template <typename T>
+__global__ void __launch_bounds__(256)
+k_mx_quant(const T *__restrict__ x, size_t n8, uint8_t *__restrict__ packed,
+           uint8_t *__restrict__ scales)
+{
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n8) return;
+    uint32_t s;
+    *(uint32_t *)(packed + 4 * i) = mx_quant8(mx_load8(x + 8 * i), s);
+    if ((i & 3) == 0) scales[i >> 2] = (uint8_t)s;
+}
+
+__device__ __forceinline__ void mx_store8(float *p, const float *f)
+{
+    *(float4 *)p = make_float4(f[0], f[1], f[2], f[3]);
+    *(float4 *)(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
+}
+
+__device__ __forceinline__ void mx_store8(uint16_t *p, const float *f)
+{
+    *(uint4 *)p = make_uint4(k3d_bf16x2(f[0], f[1]), k3d_bf16x2(f[2], f[3]), k3d_bf16x2(f[4], f[5]),
+                             k3d_bf16x2(f[6], f[7]));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+k_mx_dequant(const uint8_t *__restrict__ packed, const uint8_t *__restrict__ scales, size_t n8,
+             T *__restrict__ out)
+{
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n8) return;
+    const uint32_t b = scales[i >> 2];
+    const float s = b == 255u ? __builtin_nanf("") : k3d_e8m0(b);
+    float f[8];
+    k3d_fp4x8(*(const uint32_t *)(packed + 4 * i), 1.0f, f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] *= s;
+    mx_store8(out + 8 * i, f);
+}
+
+/* x as activation quads (see the top), a wave per quad */
+template <typename T>
+__global__ void __launch_bounds__(256)
+k_mx_x(const T *__restrict__ x, size_t nquads, int nQ, int cols, uint8_t *__restrict__ xq)
+{
+    const size_t quad = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (quad >= nquads) return;
+    const int lane = threadIdx.x & 63;
+    const size_t row = quad / nQ;
+    const int col = 512 * (int)(quad - row * nQ) + 8 * lane;
+    Mx8 v = {{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}};
+    if (col < cols) v = mx_load8(x + row * cols + col);
+    uint32_t s;
+    uint8_t *o = xq + quad * MX_XQ;
+    *(uint32_t *)(o + 4 * lane) = mx_quant8(v, s);
+    const int b = lane >> 2;
+    if ((lane & 3) == 0) o[256 + 4 * (b & 3) + (b >> 2)] = (uint8_t)s;
+}
+
+/* ------------------------------------------------------------------ product ---- */
+
+struct MxProduct {
+    const uint8_t *xq;               /* activation quads of T rows */
+    int T, nQ, nK;                   /* rows; quads and 128-column chunks of a row */
+    const int32_t *perm;             /* place -> pair, or NULL: place r is row r */
+    int topk;
+    const int32_t *off;              /* [E + 1] places of each expert, or NULL: one, all places */
+    int E, P;                        /* P places at most */
+    const uint8_t *w, *w3;           /* off NULL: the matrix; else the first expert's pointer */
+    int64_t step;                    /* bytes from one expert's pointer to the next */
+    int N;
+    float b1, b2;
+    void *y;
+};
+
+/* Row tile `item` of up to TM places: expert, first place and count; false past the last. Every
+ * wave finds it by itself: a lane takes 16 experts, then a wave scan of their tile counts. The
+ * ranges are clamped to the places there are, whatever off holds. */
+template <int TM>
+__device__ __forceinline__ bool mx_tile(const MxProduct &g, int item, int &e, int &p0, int &np)
+{
+    if (!g.off) {
+        e = 0;
+        p0 = item * TM;
+        np = min(TM, g.P - p0);
+        return np > 0;
+    }
+    const int lane = threadIdx.x & 63;
+    const int per = (g.E + 63) >> 6, e0 = lane * per, e1 = min(g.E, e0 + per);
+    int n = 0;
+    for (int i = e0; i < e1; ++i) {
+        const int a = min(max(g.off[i], 0), g.P), b = min(max(g.off[i + 1], a), g.P);
+        n += (b - a + TM - 1) / TM;
+    }
+    int inc = n;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(inc, d, K3G_WAVE);
+        if (lane >= d) inc += o;
+    }
+    const uint64_t past = __ballot(inc > item);
+    if (!past) return false;
+    const int L = __ffsll((unsigned long long)past) - 1;
+    int at = gm_uniform(__shfl(inc - n, L, K3G_WAVE));
+    for (int i = L * per; i < g.E; ++i) {
+        const int a = min(max(g.off[i], 0), g.P), b = min(max(g.off[i + 1], a), g.P);
+        const int t = (b - a + TM - 1) / TM;
+        if (item < at + t) {
+            e = gm_uniform(i);
+            p0 = gm_uniform(a + (item - at) * TM);
+            np = gm_uniform(min(TM, b - p0));
+            return true;
+        }
+        at += t;
+    }
+    return false;
+}
+
+/* The activation row of a place; -1 (zeros) when perm holds no pair of these tokens. */
+__device__ __forceinline__ int mx_row(const MxProduct &g, int place)
+{
+    if (!g.perm) return place;
+    const int p = g.perm[place], t = p / g.topk;
+    return p >= 0 && t < g.T ? t : -1;
+}
+
+__device__ __forceinline__ const uint8_t *mx_matrix(const MxProduct &g, const uint8_t *w, int e)
+{
+    if (!g.off) return w;
+    return gm_uniform_ptr(*(const uint8_t *const *)(w + (size_t)e * g.step));
+}
+
+__device__ __forceinline__ k3v4f mx_mma(const uint4 &a, uint32_t sa, const uint4 &b, uint32_t sb,
+                                        const k3v4f &acc)
+{
+    const mx_v8i av = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
+    const mx_v8i bv = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc, 4, 4, 0, (int)sa, 0, (int)sb);
+}
+
+__device__ __forceinline__ void mx_put(float *o, const k3v4f &v) { *(k3v4f *)o = v; }
+__device__ __forceinline__ void mx_put(uint16_t *o, const k3v4f &v)
+{
+    *(uint2 *)o = make_uint2(k3d_bf16x2(v[0], v[1]), k3d_bf16x2(v[2], v[3]));
+}
+
+/* One wave: 16 places by 16 features. */
+template <typename Y, bool GATED>
+__global__ void __launch_bounds__(64)
+k_mx_tile(const MxProduct g)
+{
+    int e, p0, np;
+    if (!mx_tile<16>(g, blockIdx.x, e, p0, np)) return;
+    const int lane = threadIdx.x, c = lane & 15, q = lane >> 4, rb = blockIdx.y;
+    const uint8_t *w1 = mx_matrix(g, g.w, e), *w3 = GATED ? mx_matrix(g, g.w3, e) : w1;
+    k3v4f acc = {0.f, 0.f, 0.f, 0.f}, up = acc;
+    if (w1 && w3) {
+        const int row = c < np ? mx_row(g, p0 + c) : -1;
+        const uint8_t *x = g.xq + (size_t)max(row, 0) * g.nQ * MX_XQ;
+        w1 += (size_t)rb * g.nQ * MX_QT;
+        w3 += (size_t)rb * g.nQ * MX_QT;
+        for (int k = 0; k < g.nK; ++k) {
+            const int Q = k >> 2, j = k & 3;
+            uint4 b = make_uint4(0, 0, 0, 0);
+            uint32_t sb = 127;
+            if (row >= 0) {
+                b = gm_ld16(x + (size_t)Q * MX_XQ + 64 * j + 16 * q);
+                sb = x[(size_t)Q * MX_XQ + 256 + 4 * q + j];
+            }
+            const uint8_t *t1 = w1 + (size_t)Q * MX_QT, *t3 = w3 + (size_t)Q * MX_QT;
+            acc = mx_mma(gm_ld16(t1 + 1024 * j + 16 * lane), (gm_ld4(t1 + 4096 + 4 * lane) >> (8 * j)) & 255u,
+                         b, sb, acc);
+            if (GATED)
+                up = mx_mma(gm_ld16(t3 + 1024 * j + 16 * lane),
+                            (gm_ld4(t3 + 4096 + 4 * lane) >> (8 * j)) & 255u, b, sb, up);
+        }
+    }
+    if (GATED) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = k3d_act(acc[i], up[i], g.b1, g.b2);
+    }
+    if (c < np) mx_put((Y *)g.y + (size_t)(p0 + c) * g.N + 16 * rb + 4 * q, acc);
+}
+
+/* ------------------------------------------------------------- entry points ---- */
+
+static int mx_type(const char *who, int dt)
+{
+    if (dt == K3_WF32 || dt == K3_WBF16) return 0;
+    fprintf(stderr, "%s: values are fp32 (%d) or bf16 (%d), not %d\n", who, K3_WF32, K3_WBF16, dt);
+    return -1;
+}
+
+static bool mx_shape_ok(int rows, int cols)
+{
+    return rows >= 0 && rows <= MX_MAX_ROWS && cols >= 32 && cols % 32 == 0 && cols <= MX_MAX_COLS;
+}
+
+static int mx_shape(const char *who, int rows, int cols)
+{
+    if (mx_shape_ok(rows, cols)) return 0;
+    fprintf(stderr, "%s: needs 0 to %d rows and a multiple of 32 columns up to %d (%d x %d)\n", who,
+            MX_MAX_ROWS, MX_MAX_COLS, rows, cols);
+    return -1;
+}
+
+static int mx_pointer(const char *who, const char *name, const void *p, int to, bool needed)
+{
+    if ((p || !needed) && !k3h_misaligned(p, to)) return 0;
+    fprintf(stderr, "%s: %s is missing or not aligned to %d bytes\n", who, name, to);
+    return -1;
+}
+
+extern "C" int k3g_quant_mxfp4(const void *x, int dt, int rows, int cols, void *packed, void *scales,
+                               void *stream)
+{
+    const char *who = "k3g_quant_mxfp4";
+    if (mx_type(who, dt) || mx_shape(who, rows, cols) || mx_pointer(who, "x", x, 16, rows > 0) ||
+        mx_pointer(who, "packed", packed, 16, rows > 0) || mx_pointer(who, "scales", scales, 1, rows > 0))
+        return -1;
+    if (!rows) return 0;
+    K3hOn on(stream);
+    if (!on.ok) return -1;
+    const size_t n8 = (size_t)rows * cols / 8;
+    const dim3 grid((unsigned)((n8 + 255) / 256));
+    if (dt == K3_WBF16)
+        return k3h_launch(who, k_mx_quant<uint16_t>, grid, dim3(256), on.st, (const uint16_t *)x, n8,
+                          (uint8_t *)packed, (uint8_t *)scales);
+    return k3h_launch(who, k_mx_quant<float>, grid, dim3(256), on.st, (const float *)x, n8,
+                      (uint8_t *)packed, (uint8_t *)scales);
+}
+
+extern "C" int k3g_dequant_mxfp4(const void *packed, const void *scales, int rows, int cols, void *out,
+                                 int dt, void *stream)
+{
+    const char *who = "k3g_dequant_mxfp4";
+    if (mx_type(who, dt) || mx_shape(who, rows, cols) || mx_pointer(who, "out", out, 16, rows > 0) ||
+        mx_pointer(who, "packed", packed, 16, rows > 0) || mx_pointer(who, "scales", scales, 1, rows > 0))
+        return -1;
+    if (!rows) return 0;
+    K3hOn on(stream);
+    if (!on.ok) return -1;
+    const size_t n8 = (size_t)rows * cols / 8;
+    const dim3 grid((unsigned)((n8 + 255) / 256));
+    if (dt == K3_WBF16)
+        return k3h_launch(who, k_mx_dequant<uint16_t>, grid, dim3(256), on.st, (const uint8_t *)packed,
+                          (const uint8_t *)scales, n8, (uint16_t *)out);
+    return k3h_launch(who, k_mx_dequant<float>, grid, dim3(256), on.st, (const uint8_t *)packed,
+                      (const uint8_t *)scales, n8, (float *)out);
+}
+
+extern "C" size_t k3g_mxfp4_work_bytes(int rows, int cols)
+{
+    if (!mx_shape_ok(rows, cols)) return 0;
+    return (size_t)rows * ((cols + 511) / 512) * MX_XQ;
+}
+
+/* the product of checked arguments */
+static int mx_product(const char *who, MxProduct &g, const void *x, int xdt, int cols, int ydt,
+                      void *work, size_t work_bytes, void *stream)
+{
+    const size_t need = k3g_mxfp4_work_bytes(g.T, cols);
+    if (!work || k3h_misaligned(work, 16) || work_bytes < need) {
+        fprintf(stderr, "%s: needs a workspace of %zu bytes, aligned to 16 (%zu given)\n", who, need,
+                work ? work_bytes : (size_t)0);
+        return -1;
+    }
+    K3hOn on(stream);
+    if (!on.ok) return -1;
+    g.nQ = (cols + 511) / 512;
+    g.nK = (cols + 127) / 128;
+    g.xq = (const uint8_t *)work;
+    const size_t nquads = (size_t)g.T * g.nQ;
+    const dim3 xgrid((unsigned)((nquads + 3) / 4));
+    if (xdt == K3_WBF16 ? k3h_launch(who, k_mx_x<uint16_t>, xgrid, dim3(256), on.st, (const uint16_t *)x,
+                                     nquads, g.nQ, cols, (uint8_t *)work)
+                        : k3h_launch(who, k_mx_x<float>, xgrid, dim3(256), on.st, (const float *)x, nquads,
+                                     g.nQ, cols, (uint8_t *)work))
+        return -1;
+    const int tiles = g.off ? g.P / 16 + min(g.E, g.P) : (g.P + 15) / 16;
+    const dim3 grid(tiles, g.N / 16);
+    const bool bf = ydt == K3_WBF16;
+    if (g.w3)
+        return bf ? k3h_launch(who, k_mx_tile<uint16_t, true>, grid, dim3(64), on.st, (const MxProduct)g)
+                  : k3h_launch(who, k_mx_tile<float, true>, grid, dim3(64), on.st, (const MxProduct)g);
+    return bf ? k3h_launch(who, k_mx_tile<uint16_t, false>, grid, dim3(64), on.st, (const MxProduct)g)
+              : k3h_launch(who, k_mx_tile<float, false>, grid, dim3(64), on.st, (const MxProduct)g);
+}
+
+static int mx_features(const char *who, int n)
+{
+    if (n >= 16 && n % 16 == 0 && n <= MX_MAX_COLS) return 0;
+    fprintf(stderr, "%s: needs a multiple of 16 features up to %d (%d)\n", who, MX_MAX_COLS, n);
+    return -1;
+}
+
+extern "C" int k3g_matmul_mxfp4(const void *x, int xdt, int rows, int cols, const void *w, int n, void *y,
+                                int ydt, void *work, size_t work_bytes, void *stream)
+{
+    const char *who = "k3g_matmul_mxfp4";
+    if (mx_type(who, xdt) || mx_type(who, ydt) || mx_shape(who, rows, cols) || mx_features(who, n) ||
+        mx_pointer(who, "x", x, 16, rows > 0) || mx_pointer(who, "w", w, 16, rows > 0) ||
+        mx_pointer(who, "y", y, 16, rows > 0))
+        return -1;
+    if (!rows) return 0;
+    MxProduct g = {};
+    g.T = g.P = rows;
+    g.topk = g.E = 1;
+    g.w = (const uint8_t *)w;
+    g.N = n;
+    g.y = y;
+    return mx_product(who, g, x, xdt, cols, ydt, work, work_bytes, stream);
+}
+
+extern "C" int k3g_grouped_mxfp4(const void *x, int xdt, int rows, int cols, const int32_t *perm, int topk,
+                                 const int32_t *off, int n_experts, const void *const *w,
+                                 const void *const *w3, int w_step, int n, float b1, float b2, void *y,
+                                 int ydt, void *work, size_t work_bytes, void *stream)
+{
+    const char *who = "k3g_grouped_mxfp4";
+    if (mx_type(who, xdt) || mx_type(who, ydt) || mx_shape(who, rows, cols) || mx_features(who, n) ||
+        mx_pointer(who, "x", x, 16, rows > 0) || mx_pointer(who, "y", y, 16, rows > 0) ||
+        mx_pointer(who, "off", off, 4, rows > 0) || mx_pointer(who, "perm", perm, 4, false) ||
+        mx_pointer(who, "w", w, 8, rows > 0) || mx_pointer(who, "w3", w3, 8, false))
+        return -1;
+    if (n_experts < 1 || n_experts > 1024 || topk < 1 || topk > K3G_MAX_TOPK || (!perm && topk != 1) ||
+        (int64_t)rows * topk > MX_MAX_ROWS) {
+        fprintf(stderr, "%s: needs 1 to 1024 experts, 1 <= topk <= %d (1 without perm) and at most %d "
+                        "pairs (%d experts, %d x %d)\n", who, K3G_MAX_TOPK, MX_MAX_ROWS, n_experts, rows,
+                topk);
+        return -1;
+    }
+    if (w_step < 8 || w_step % 8) {
+        fprintf(stderr, "%s: w_step is a multiple of 8 bytes (%d)\n", who, w_step);
+        return -1;
+    }
+    if (w3 && !(b1 > 0.0f && b2 > 0.0f)) {
+        fprintf(stderr, "%s: the activation's caps are positive (%g, %g)\n", who, b1, b2);
+        return -1;
+    }
+    if (!rows) return 0;
+    MxProduct g = {};
+    g.T = rows;
+    g.perm = perm;
+    g.topk = topk;
+    g.off = off;
+    g.E = n_experts;
+    g.P = rows * topk;
+    g.w = (const uint8_t *)w;
+    g.w3 = (const uint8_t *)w3;
+    g.step = w_step;
+    g.N = n;
+    g.b1 = b1;
+    g.b2 = b2;
+    g.y = y;
+    return mx_product(who, g, x, xdt, cols, ydt, work, work_bytes, stream);
+}

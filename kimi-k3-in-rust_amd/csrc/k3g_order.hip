@@ -1,0 +1,512 @@
+/* k3g_order.hip - tokens in expert order and back: the sort of the (token, slot) pairs by
+ * expert, token rows gathered into that order, expert rows brought back with the router's
+ * weights, and the gradients of both. Device pointers and a stream, no context and no
+ * allocation: for callers with experts of their own.
+ *
+ * With pairs p = t * topk + j, e(p) = idx[p] and pos[p] the place of pair p among the kept
+ * pairs in (expert, pair) order:
+ *   permute          sorted[pos[p]] = x[p / topk]
+ *   its gradient     dx[t] = sum_j dsorted[pos[t, j]]
+ *   unpermute        out[t] = sum_j wt[t, j] sorted[pos[t, j]] (+ add[t])
+ *   its gradients    dsorted[pos[t, j]] = wt[t, j] dout[t],
+ *                    dwt[t, j] = sum_i sorted[pos[t, j]][i] dout[t][i]
+ * All four are walked by token: a token's row is read or written once, whatever its topk, and
+ * the slots are summed in their order in one thread, so nothing is atomic and the results do
+ * not depend on the launch. */
+#include <stdio.h>
+
+#include "k3g_dev.h"
+#include "k3g_host.h"
+#include "k3g_kernels.h"
+
+#define OD_MAX_EXPERTS 1024
+#define OD_MAX_PAIRS (1 << 26)
+#define OD_MAX_WIDTH (1 << 24)
+#define OD_THREADS 512                 /* threads of a sort block */
+#define OD_WAVES (OD_THREADS / 64)
+#define OD_CHUNKS 128                  /* chunks of a sort at most */
+
+/* ------------------------------------------------------------------------ sort ---- */
+
+/* The lanes of the wave with the same key (ballots over its bits; lanes without a key form a
+ * group of their own). */
+__device__ __forceinline__ uint64_t od_peers(int key, int nb)
+{
+    uint64_t peers = __ballot(key >= 0);
+    if (key < 0) peers = ~peers;
+    for (int b = 0; b < nb; ++b) {
+        const bool one = key >= 0 && ((key >> b) & 1);
+        const uint64_t m = __ballot(one);
+        peers &= one ? m : ~m;
+    }
+    return peers;
+}
+
+__device__ __forceinline__ int od_key(const int32_t *idx, int p, int end, int E, int *err)
+{
+    if (p >= end) return -1;
+    const int k = idx[p];
+    if (k >= E) {
+        k3d_raise(err, K3G_ERR_EXPERT_RANGE);
+        return -1;
+    }
+    return k < 0 ? -1 : k;
+}
+
+/* The pairs of each expert in each chunk of m * OD_THREADS pairs. */
+__global__ void __launch_bounds__(OD_THREADS)
+k_order_count(const int32_t *__restrict__ idx, int P, int E, int m, int32_t *__restrict__ cnt)
+{
+    __shared__ int h[OD_MAX_EXPERTS];
+    const int first = blockIdx.x * m * OD_THREADS, end = min(P, first + m * OD_THREADS);
+    for (int e = threadIdx.x; e < E; e += OD_THREADS) h[e] = 0;
+    __syncthreads();
+    for (int p = first + threadIdx.x; p < end; p += OD_THREADS) {
+        const int k = idx[p];
+        if (k >= 0 && k < E) atomicAdd(&h[k], 1);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += OD_THREADS) cnt[(size_t)blockIdx.x * E + e] = h[e];
+}
+
+/* A chunk's pairs into their places: wave w takes m * 64 consecutive pairs, 64 at a time; a
+ * pair's rank is the wave's earlier pairs of its expert (a count in LDS) plus those in lanes
+ * before it. Then, per expert, the waves' counts become running sums, the chunks before give
+ * where the chunk's first pair of it goes (counts of k_order_count; one chunk needs none), and
+ * a block scan of the totals gives where the expert begins. Between the two walks a pair's rank
+ * waits in its own entry of pos. */
+__global__ void __launch_bounds__(OD_THREADS)
+k_order_place(const int32_t *__restrict__ idx, int P, int E, int m,
+              const int32_t *__restrict__ cnt, int nch, int32_t *__restrict__ perm,
+              int32_t *__restrict__ off, int32_t *pos, int *err)
+{
+    __shared__ int wc[OD_WAVES][OD_MAX_EXPERTS];
+    __shared__ int first[OD_MAX_EXPERTS];
+    __shared__ int red[OD_WAVES + 1];
+    const int c = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    for (int e = tid; e < OD_WAVES * OD_MAX_EXPERTS; e += OD_THREADS) (&wc[0][0])[e] = 0;
+    __syncthreads();
+    const int p0 = (c * OD_WAVES + w) * m * 64, end = min(P, p0 + m * 64);
+    const int nb = 32 - __clz(E > 1 ? E - 1 : 1);
+    const uint64_t lt = (1ull << lane) - 1;
+    for (int p = p0 + lane; p - lane < end; p += 64) {
+        const int key = od_key(idx, p, end, E, err);
+        const uint64_t peers = od_peers(key, nb);
+        const int r = __popcll(peers & lt);
+        /* atomics: a wave's lanes read what its other lanes wrote a step before */
+        const int before = key >= 0 ? __hip_atomic_load(&wc[w][key], __ATOMIC_RELAXED,
+                                                        __HIP_MEMORY_SCOPE_WAVEFRONT) : 0;
+        __builtin_amdgcn_wave_barrier();
+        if (key >= 0 && r == 0)
+            __hip_atomic_store(&wc[w][key], before + __popcll(peers), __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_WAVEFRONT);
+        __builtin_amdgcn_wave_barrier();
+        if (p < end) pos[p] = key >= 0 ? before + r : -1;
+    }
+    __syncthreads();
+    constexpr int EPT = OD_MAX_EXPERTS / OD_THREADS;
+    int tot[EPT], prev[EPT], run = 0;
+#pragma unroll
+    for (int u = 0; u < EPT; ++u) {
+        const int e = EPT * tid + u;
+        tot[u] = prev[u] = 0;
+        if (e >= E) continue;
+        int s = 0;
+#pragma unroll
+        for (int q = 0; q < OD_WAVES; ++q) {
+            const int v = wc[q][e];
+            wc[q][e] = s;
+            s += v;
+        }
+        if (nch == 1) {
+            tot[u] = s;
+        } else {
+#pragma unroll 8
+            for (int q = 0; q < nch; ++q) {
+                const int v = cnt[(size_t)q * E + e];
+                if (q < c) prev[u] += v;
+                tot[u] += v;
+            }
+        }
+        run += tot[u];
+    }
+    int v[1] = {run}, all[1];
+    k3d_block_exscan_n<1, OD_WAVES>(v, all, red);
+    int at = v[0];
+#pragma unroll
+    for (int u = 0; u < EPT; ++u) {
+        const int e = EPT * tid + u;
+        if (e < E) {
+            first[e] = at + prev[u];
+            if (c == 0) off[e] = at;
+        }
+        at += tot[u];
+    }
+    if (c == 0 && tid == 0) off[E] = all[0];
+    __syncthreads();
+    for (int p = p0 + lane; p < end; p += 64) {
+        const int rank = pos[p];
+        if (rank < 0) continue;
+        const int e = idx[p], place = first[e] + wc[w][e] + rank;
+        perm[place] = p;
+        pos[p] = place;
+    }
+}
+
+/* ------------------------------------------------------------------ row vectors ---- */
+
+/* 16 bytes of a row, whatever the row's alignment (rows of an odd width begin at any element;
+ * global loads of 16 bytes take any address). */
+typedef uint32_t od_v4u __attribute__((ext_vector_type(4), aligned(2)));
+
+template <typename T> struct OdRow;
+template <> struct OdRow<float> {
+    static constexpr int V = 4;
+    static __device__ __forceinline__ void get(const od_v4u &u, float *f)
+    {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(u[i]);
+    }
+    static __device__ __forceinline__ od_v4u put(const float *f)
+    {
+        return od_v4u{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                      __float_as_uint(f[3])};
+    }
+};
+template <> struct OdRow<uint16_t> {
+    static constexpr int V = 8;
+    static __device__ __forceinline__ void get(const od_v4u &u, float *f)
+    {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = k3d_bf16lo(u[i]);
+            f[2 * i + 1] = k3d_bf16hi(u[i]);
+        }
+    }
+    static __device__ __forceinline__ od_v4u put(const float *f)
+    {
+        od_v4u u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i] = k3d_bf16x2(f[2 * i], f[2 * i + 1]);
+        return u;
+    }
+};
+
+/* Vector v of the n-element row at p: whole ones in one load or store, the last one's elements
+ * one by one when n ends inside it. */
+template <typename T>
+__device__ __forceinline__ od_v4u od_load(const T *p, int v, int n)
+{
+    constexpr int V = OdRow<T>::V;
+    if (V * (v + 1) <= n) return *(const od_v4u *)(p + V * v);
+    T e[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) e[i] = V * v + i < n ? p[V * v + i] : (T)0;
+    od_v4u u;
+    __builtin_memcpy(&u, e, 16);
+    return u;
+}
+
+template <typename T>
+__device__ __forceinline__ void od_store(T *p, int v, int n, const od_v4u &u)
+{
+    constexpr int V = OdRow<T>::V;
+    if (V * (v + 1) <= n) {
+        *(od_v4u *)(p + V * v) = u;
+        return;
+    }
+    T e[V];
+    __builtin_memcpy(e, &u, 16);
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (V * v + i < n) p[V * v + i] = e[i];
+}
+
+/* --------------------------------------------------------------------- kernels ---- */
+
+/* A block of 256 threads is `ty` tokens of `tx` vectors each (tx a power of two); the grid is
+ * (tokens, vectors). */
+struct OdGrid {
+    int T, k, n, P, tx_log;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+k_permute(const OdGrid g, const T *__restrict__ x, const int32_t *__restrict__ pos,
+          T *__restrict__ sorted)
+{
+    const int t = blockIdx.x * (256 >> g.tx_log) + (threadIdx.x >> g.tx_log);
+    const int v = (blockIdx.y << g.tx_log) + (threadIdx.x & ((1 << g.tx_log) - 1));
+    if (t >= g.T || OdRow<T>::V * v >= g.n) return;
+    const od_v4u u = od_load(x + (size_t)t * g.n, v, g.n);
+    for (int j = 0; j < g.k; ++j) {
+        const int p = pos[(size_t)t * g.k + j];
+        if ((unsigned)p < (unsigned)g.P) od_store(sorted + (size_t)p * g.n, v, g.n, u);
+    }
+}
+
+/* out[t] = sum_j w_j row_j, products and sums rounded separately in slot order as the layer's
+ * combine does, then + add[t]; without weights the gradient of k_permute. */
+template <typename T>
+__global__ void __launch_bounds__(256)
+k_unpermute(const OdGrid g, const T *__restrict__ sorted, const int32_t *__restrict__ pos,
+            const float *__restrict__ wt, const T *__restrict__ add, T *__restrict__ out)
+{
+    constexpr int V = OdRow<T>::V;
+    const int t = blockIdx.x * (256 >> g.tx_log) + (threadIdx.x >> g.tx_log);
+    const int v = (blockIdx.y << g.tx_log) + (threadIdx.x & ((1 << g.tx_log) - 1));
+    if (t >= g.T || V * v >= g.n) return;
+    float acc[V], f[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = 0.0f;
+    for (int j = 0; j < g.k; ++j) {
+        const int p = pos[(size_t)t * g.k + j];
+        if ((unsigned)p >= (unsigned)g.P) continue;
+        OdRow<T>::get(od_load(sorted + (size_t)p * g.n, v, g.n), f);
+        const float w = wt ? wt[(size_t)t * g.k + j] : 1.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] += wt ? w * f[i] : f[i];
+    }
+    if (add) {
+        OdRow<T>::get(od_load(add + (size_t)t * g.n, v, g.n), f);
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] += f[i];
+    }
+    od_store(out + (size_t)t * g.n, v, g.n, OdRow<T>::put(acc));
+}
+
+/* One block per pair: its row of dsorted and its entry of dwt. */
+template <typename T>
+__global__ void __launch_bounds__(256)
+k_unpermute_grad(const OdGrid g, const T *__restrict__ dout, const T *__restrict__ sorted,
+                 const int32_t *__restrict__ pos, const float *__restrict__ wt,
+                 T *__restrict__ dsorted, float *__restrict__ dwt)
+{
+    constexpr int V = OdRow<T>::V;
+    __shared__ float part[4];
+    const size_t pair = (size_t)blockIdx.x;
+    const int t = (int)(pair / g.k), p = pos[pair];
+    if ((unsigned)p >= (unsigned)g.P) {
+        if (dwt && threadIdx.x == 0) dwt[pair] = 0.0f;
+        return;
+    }
+    const float w = dsorted ? wt[pair] : 0.0f;
+    float s = 0.0f;
+    for (int v = threadIdx.x; V * v < g.n; v += 256) {
+        float go[V], f[V];
+        OdRow<T>::get(od_load(dout + (size_t)t * g.n, v, g.n), go);
+        if (dwt) {
+            OdRow<T>::get(od_load(sorted + (size_t)p * g.n, v, g.n), f);
+#pragma unroll
+            for (int i = 0; i < V; ++i) s += f[i] * go[i];
+        }
+        if (dsorted) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[i] = w * go[i];
+            od_store(dsorted + (size_t)p * g.n, v, g.n, OdRow<T>::put(f));
+        }
+    }
+    if (!dwt) return;
+    s = k3d_wave_sum(s);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) dwt[pair] = part[0] + part[1] + part[2] + part[3];
+}
+
+/* ------------------------------------------------------------------ entry points ---- */
+
+static int sort_chunks(int P, int *m)
+{
+    int per = 1;
+    if (P > 8 * OD_THREADS) {
+        per = (P + OD_CHUNKS * OD_THREADS - 1) / (OD_CHUNKS * OD_THREADS);
+    } else {
+        per = (P + OD_THREADS - 1) / OD_THREADS;
+        if (per < 1) per = 1;
+    }
+    *m = per;
+    return P ? (P + per * OD_THREADS - 1) / (per * OD_THREADS) : 1;
+}
+
+/* sizes every call here shares: 0 when they are ones the kernels take */
+static int bad_sizes(const char *who, int T, int topk)
+{
+    if (T < 0 || topk < 1 || topk > K3G_MAX_TOPK || (int64_t)T * topk > OD_MAX_PAIRS) {
+        fprintf(stderr, "%s: needs 0 <= tokens, 1 <= topk <= %d and at most %d pairs (%d x %d)\n", who,
+                K3G_MAX_TOPK, OD_MAX_PAIRS, T, topk);
+        return 1;
+    }
+    return 0;
+}
+
+extern "C" size_t k3g_sort_bytes(int T, int topk, int n_experts)
+{
+    if (T < 0 || topk < 1 || topk > K3G_MAX_TOPK || (int64_t)T * topk > OD_MAX_PAIRS ||
+        n_experts < 1 || n_experts > OD_MAX_EXPERTS)
+        return 0;
+    int m;
+    const int nch = sort_chunks(T * topk, &m);
+    return nch > 1 ? (size_t)nch * n_experts * sizeof(int32_t) : 0;
+}
+
+extern "C" int k3g_sort_tokens(const int32_t *idx, int T, int topk, int n_experts, int32_t *perm,
+                               int32_t *off, int32_t *pos, int *err, void *work,
+                               size_t work_bytes, void *stream)
+{
+    const char *who = "k3g_sort_tokens";
+    if (bad_sizes(who, T, topk)) return -1;
+    if (n_experts < 1 || n_experts > OD_MAX_EXPERTS) {
+        fprintf(stderr, "%s: needs 1 to %d experts (%d)\n", who, OD_MAX_EXPERTS, n_experts);
+        return -1;
+    }
+    const int P = T * topk;
+    if (!off || (P && (!idx || !perm || !pos)) || k3h_misaligned(idx, 4) || k3h_misaligned(perm, 4) ||
+        k3h_misaligned(off, 4) || k3h_misaligned(pos, 4) || k3h_misaligned(err, 4) ||
+        k3h_misaligned(work, 4)) {
+        fprintf(stderr, "%s: a pointer is missing or not aligned to 4 bytes\n", who);
+        return -1;
+    }
+    const size_t need = k3g_sort_bytes(T, topk, n_experts);
+    if (need && (!work || work_bytes < need)) {
+        fprintf(stderr, "%s: needs %zu bytes of workspace (%zu given)\n", who, need,
+                work ? work_bytes : (size_t)0);
+        return -1;
+    }
+    K3hOn on(stream);
+    if (!on.ok) return -1;
+    int m;
+    const int nch = sort_chunks(P, &m);
+    int32_t *cnt = (int32_t *)work;
+    if (nch > 1 && k3h_launch(who, k_order_count, dim3(nch), dim3(OD_THREADS), on.st, idx, P, n_experts, m,
+                              cnt))
+        return -1;
+    return k3h_launch(who, k_order_place, dim3(nch), dim3(OD_THREADS), on.st, idx, P, n_experts, m,
+                      (const int32_t *)cnt, nch, perm, off, pos, err);
+}
+
+namespace {
+
+/* The checks the row calls share; rows and tokens as an OdGrid with its launch. */
+int row_sizes(const char *who, int dt, int T, int topk, int n)
+{
+    if (bad_sizes(who, T, topk)) return -1;
+    if (dt != K3_WF32 && dt != K3_WBF16) {
+        fprintf(stderr, "%s: rows are fp32 (%d) or bf16 (%d), not %d\n", who, K3_WF32, K3_WBF16, dt);
+        return -1;
+    }
+    if (n < 1 || n > OD_MAX_WIDTH) {
+        fprintf(stderr, "%s: needs a width of 1 to %d (%d)\n", who, OD_MAX_WIDTH, n);
+        return -1;
+    }
+    return 0;
+}
+
+int row_pointer(const char *who, const char *name, const void *p, int size, bool needed)
+{
+    if (needed && !p) {
+        fprintf(stderr, "%s: %s is missing\n", who, name);
+        return -1;
+    }
+    if (k3h_misaligned(p, size)) {
+        fprintf(stderr, "%s: %s is not aligned to its elements (%d bytes)\n", who, name, size);
+        return -1;
+    }
+    return 0;
+}
+
+dim3 row_grid(OdGrid &g, int V)
+{
+    const int nv = (g.n + V - 1) / V;
+    g.tx_log = 0;
+    while (g.tx_log < 8 && (1 << g.tx_log) < nv) ++g.tx_log;
+    const int ty = 256 >> g.tx_log;
+    return dim3((g.T + ty - 1) / ty, (nv + (1 << g.tx_log) - 1) >> g.tx_log);
+}
+
+}  // namespace
+
+extern "C" int k3g_permute(const void *x, int dt, int T, int topk, int n, const int32_t *pos,
+                           void *sorted, void *stream)
+{
+    const char *who = "k3g_permute";
+    if (row_sizes(who, dt, T, topk, n)) return -1;
+    const int size = dt == K3_WBF16 ? 2 : 4;
+    if (row_pointer(who, "x", x, size, T > 0) || row_pointer(who, "pos", pos, 4, T > 0) ||
+        row_pointer(who, "sorted", sorted, size, T > 0))
+        return -1;
+    if (!T) return 0;
+    K3hOn on(stream);
+    if (!on.ok) return -1;
+    OdGrid g = {T, topk, n, T * topk, 0};
+    const dim3 grid = row_grid(g, 16 / size);
+    if (dt == K3_WBF16)
+        return k3h_launch(who, k_permute<uint16_t>, grid, dim3(256), on.st, (const OdGrid)g,
+                          (const uint16_t *)x, pos, (uint16_t *)sorted);
+    return k3h_launch(who, k_permute<float>, grid, dim3(256), on.st, (const OdGrid)g, (const float *)x,
+                      pos, (float *)sorted);
+}
+
+static int unpermute(const char *who, const void *sorted, int dt, int T, int topk, int n,
+                     const int32_t *pos, const float *wt, const void *add, void *out, void *stream)
+{
+    if (row_sizes(who, dt, T, topk, n)) return -1;
+    const int size = dt == K3_WBF16 ? 2 : 4;
+    if (row_pointer(who, "the sorted rows", sorted, size, T > 0) ||
+        row_pointer(who, "pos", pos, 4, T > 0) || row_pointer(who, "wt", wt, 4, false) ||
+        row_pointer(who, "add", add, size, false) || row_pointer(who, "the output", out, size, T > 0))
+        return -1;
+    if (!T) return 0;
+    K3hOn on(stream);
+    if (!on.ok) return -1;
+    OdGrid g = {T, topk, n, T * topk, 0};
+    const dim3 grid = row_grid(g, 16 / size);
+    if (dt == K3_WBF16)
+        return k3h_launch(who, k_unpermute<uint16_t>, grid, dim3(256), on.st, (const OdGrid)g,
+                          (const uint16_t *)sorted, pos, wt, (const uint16_t *)add, (uint16_t *)out);
+    return k3h_launch(who, k_unpermute<float>, grid, dim3(256), on.st, (const OdGrid)g,
+                      (const float *)sorted, pos, wt, (const float *)add, (float *)out);
+}
+
+extern "C" int k3g_permute_grad(const void *dsorted, int dt, int T, int topk, int n,
+                                const int32_t *pos, void *dx, void *stream)
+{
+    return unpermute("k3g_permute_grad", dsorted, dt, T, topk, n, pos, nullptr, nullptr, dx, stream);
+}
+
+extern "C" int k3g_unpermute(const void *sorted, int dt, int T, int topk, int n, const int32_t *pos,
+                             const float *wt, const void *add, void *out, void *stream)
+{
+    if (T > 0 && !wt) {
+        fprintf(stderr, "k3g_unpermute: wt is missing\n");
+        return -1;
+    }
+    return unpermute("k3g_unpermute", sorted, dt, T, topk, n, pos, wt, add, out, stream);
+}
+
+extern "C" int k3g_unpermute_grad(const void *dout, const void *sorted, int dt, int T, int topk,
+                                  int n, const int32_t *pos, const float *wt, void *dsorted,
+                                  float *dwt, void *stream)
+{
+    const char *who = "k3g_unpermute_grad";
+    if (row_sizes(who, dt, T, topk, n)) return -1;
+    const int size = dt == K3_WBF16 ? 2 : 4;
+    if (row_pointer(who, "dout", dout, size, T > 0) || row_pointer(who, "pos", pos, 4, T > 0) ||
+        row_pointer(who, "sorted", sorted, size, T > 0 && dwt) ||
+        row_pointer(who, "wt", wt, 4, T > 0 && dsorted) ||
+        row_pointer(who, "dsorted", dsorted, size, false) || row_pointer(who, "dwt", dwt, 4, false))
+        return -1;
+    if (!dsorted && !dwt) {
+        fprintf(stderr, "%s: neither gradient is asked for\n", who);
+        return -1;
+    }
+    if (!T) return 0;
+    K3hOn on(stream);
+    if (!on.ok) return -1;
+    const OdGrid g = {T, topk, n, T * topk, 0};
+    if (dt == K3_WBF16)
+        return k3h_launch(who, k_unpermute_grad<uint16_t>, dim3(g.P), dim3(256), on.st, g,
+                          (const uint16_t *)dout, (const uint16_t *)sorted, pos, wt, (uint16_t *)dsorted,
+                          dwt);
+    return k3h_launch(who, k_unpermute_grad<float>, dim3(g.P), dim3(256), on.st, g, (const float *)dout,
+                      (const float *)sorted, pos, wt, (float *)dsorted, dwt);
+}

@@ -221,6 +221,28 @@ def lib() -> C.CDLL:
         L.k3g_combine.restype = i
         L.k3g_moe_noalloc.argtypes = [C.POINTER(K3gLayer), vp, i, vp, vp, vp, vp, vp]
         L.k3g_moe_noalloc.restype = i
+        L.k3g_sort_bytes.argtypes = [i, i, i]
+        L.k3g_sort_bytes.restype = sz
+        L.k3g_sort_tokens.argtypes = [vp, i, i, i, vp, vp, vp, vp, vp, sz, vp]
+        L.k3g_sort_tokens.restype = i
+        for name in ("k3g_permute", "k3g_permute_grad"):
+            getattr(L, name).argtypes = [vp, i, i, i, i, vp, vp, vp]
+            getattr(L, name).restype = i
+        L.k3g_unpermute.argtypes = [vp, i, i, i, i, vp, vp, vp, vp, vp]
+        L.k3g_unpermute.restype = i
+        L.k3g_unpermute_grad.argtypes = [vp, vp, i, i, i, i, vp, vp, vp, vp, vp]
+        L.k3g_unpermute_grad.restype = i
+        L.k3g_quant_mxfp4.argtypes = [vp, i, i, i, vp, vp, vp]
+        L.k3g_quant_mxfp4.restype = i
+        L.k3g_dequant_mxfp4.argtypes = [vp, vp, i, i, vp, i, vp]
+        L.k3g_dequant_mxfp4.restype = i
+        L.k3g_mxfp4_work_bytes.argtypes = [i, i]
+        L.k3g_mxfp4_work_bytes.restype = sz
+        L.k3g_matmul_mxfp4.argtypes = [vp, i, i, i, vp, i, vp, i, vp, sz, vp]
+        L.k3g_matmul_mxfp4.restype = i
+        L.k3g_grouped_mxfp4.argtypes = [vp, i, i, i, vp, i, vp, i, vp, vp, i, i, f, f, vp, i, vp,
+                                        sz, vp]
+        L.k3g_grouped_mxfp4.restype = i
         L.k3g_sync.argtypes = [vp, vp]
         L.k3g_sync.restype = i
         L.k3s_byte.argtypes = [u64, u64, u64]
