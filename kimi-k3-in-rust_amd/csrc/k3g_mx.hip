@@ -26,6 +26,13 @@
 #define MX_MAX_ROWS (1 << 26)
 #define MX_MAX_COLS (1 << 20)
 
+#ifndef MX_FEW
+#define MX_FEW 8
+#endif
+#ifndef MX_TM128
+#define MX_TM128 48
+#endif
+
 typedef int mx_v8i __attribute__((ext_vector_type(8)));
 
 /* ------------------------------------------------------------- quantisation ---- */
@@ -121,18 +128,18 @@ k_mx_dequant(const uint8_t *__restrict__ packed, const uint8_t *__restrict__ sca
     mx_store8(out + 8 * i, f);
 }
 
-/* x as activation quads (see the top), a wave per quad */
+/* x as activation quads (see the top), a wave per quad, and a row of zeros behind them */
 template <typename T>
 __global__ void __launch_bounds__(256)
 k_mx_x(const T *__restrict__ x, size_t nquads, int nQ, int cols, uint8_t *__restrict__ xq)
 {
     const size_t quad = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (quad >= nquads) return;
+    if (quad >= nquads + nQ) return;
     const int lane = threadIdx.x & 63;
     const size_t row = quad / nQ;
     const int col = 512 * (int)(quad - row * nQ) + 8 * lane;
     Mx8 v = {{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}};
-    if (col < cols) v = mx_load8(x + row * cols + col);
+    if (col < cols && quad < nquads) v = mx_load8(x + row * cols + col);
     uint32_t s;
     uint8_t *o = xq + quad * MX_XQ;
     *(uint32_t *)(o + 4 * lane) = mx_quant8(v, s);
@@ -265,6 +272,218 @@ k_mx_tile(const MxProduct g)
     if (c < np) mx_put((Y *)g.y + (size_t)(p0 + c) * g.N + 16 * rb + 4 * q, acc);
 }
 
+/* ---- many rows: a workgroup of four waves takes up to TM places by 4 x 64 features (gated: 4 x
+ * 32 of each matrix). The activation quads of its places go to LDS by DMA, two stages of one quad;
+ * the 16-byte unit u of row r lies at slot u ^ (r % 16) of the row's 256 bytes, so the 16 rows of
+ * an operand read 16 different slots. Weights go straight from memory to registers, four chunks
+ * ahead: no two waves of a workgroup share them. */
+
+template <int J>
+__device__ __forceinline__ k3v4f mx_mma4(const gm_v4u &a, uint32_t sa, const gm_v4u &b, uint32_t sb,
+                                         const k3v4f &acc)
+{
+    const mx_v8i av = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
+    const mx_v8i bv = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc, 4, 4, J, (int)sa, J, (int)sb);
+}
+
+template <int TM>
+struct MxWave {
+    static constexpr int SCALES = TM * 256, STAGE = TM * MX_XQ;
+    const uint8_t *w[4];               /* the row blocks' first quads */
+    const uint8_t *xq;                 /* the activations; in units of 16 bytes from there: */
+    uint32_t x[TM / 16];               /* of each 16 rows the unit this lane copies */
+    uint32_t xs;                       /* the scales this lane copies (waves below TM / 64) */
+    uint32_t lds;
+    const uint8_t *ldsp;
+    int lane, wave, nQ, nK;
+};
+
+/* v, worked out from here on: an address made of it is not kept in registers over a loop (64-bit
+ * ones of every weight and activation pointer took 25 registers more than there are) */
+__device__ __forceinline__ uint32_t mx_here(uint32_t v)
+{
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+/* NB blocks of 16 places */
+template <int TM, int NB>
+__device__ __forceinline__ void mx_gemm_sums(const MxWave<TM> &t, k3v4f (&acc)[4][NB])
+{
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int n = 0; n < NB; ++n) acc[r][n] = k3v4f{0.f, 0.f, 0.f, 0.f};
+    const int c = t.lane & 15, q = t.lane >> 4;
+    gm_v4u a[4][4];
+    uint32_t sA[4], sN[4];
+    auto load = [&](int Q, auto jc) {
+        constexpr int J = decltype(jc)::value;
+        const uint32_t at = mx_here(16 * t.lane);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) a[J][r] = *(gm_g4)(t.w[r] + (size_t)Q * MX_QT + 1024 * J + at);
+    };
+    auto load_scales = [&](int Q, uint32_t (&s)[4]) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[r] = gm_ld4(t.w[r] + (size_t)Q * MX_QT + 4096 + mx_here(4 * t.lane));
+    };
+    auto dma = [&](int Q) {
+        const uint32_t st = t.lds + (Q & 1) * t.STAGE;
+        const uint8_t *from = t.xq + (size_t)Q * MX_XQ;
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+            gm_dma16(from + (uint64_t)mx_here(t.x[i]) * 16, st + 4096 * i + 1024 * t.wave);
+        if (64 * t.wave < 16 * NB)
+            gm_dma16(from + (uint64_t)mx_here(t.xs) * 16, st + t.SCALES + 1024 * t.wave);
+    };
+    auto chunk = [&](const uint8_t *st, const uint32_t (&sB)[NB], auto jc) {
+        constexpr int J = decltype(jc)::value;
+        const uint8_t *row = st + 256 * c + 16 * ((4 * J + q) ^ c);
+        /* read one block ahead of its products */
+        gm_v4u b[2];
+        b[0] = *(const gm_v4u *)row;
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            if (n + 1 < NB) b[(n + 1) & 1] = *(const gm_v4u *)(row + 4096 * (n + 1));
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[r][n] = mx_mma4<J>(a[J][r], sA[r], b[n & 1], sB[n], acc[r][n]);
+        }
+    };
+    auto quad = [&](int Q, auto more) {
+        constexpr bool MORE = decltype(more)::value;
+        /* this quad's copies are older than the 20 weight loads issued since */
+        gm_wait_vm<20>();
+        __syncthreads();
+        if (MORE) {
+            dma(Q + 1);
+            load_scales(Q + 1, sN);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        const uint8_t *st = t.ldsp + (Q & 1) * t.STAGE;
+        uint32_t sB[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+            sB[n] = *(const uint32_t *)(st + t.SCALES + 256 * n + 16 * c + 4 * q);
+        const int left = MORE ? 4 : t.nK - 4 * Q;
+        chunk(st, sB, GmInt<0>{});
+        if (MORE) load(Q + 1, GmInt<0>{});
+        if (left > 1) chunk(st, sB, GmInt<1>{});
+        if (MORE) load(Q + 1, GmInt<1>{});
+        if (left > 2) chunk(st, sB, GmInt<2>{});
+        if (MORE) load(Q + 1, GmInt<2>{});
+        if (left > 3) chunk(st, sB, GmInt<3>{});
+        if (MORE) {
+            load(Q + 1, GmInt<3>{});
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sA[r] = sN[r];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    dma(0);
+    load_scales(0, sA);
+    load(0, GmInt<0>{});
+    load(0, GmInt<1>{});
+    load(0, GmInt<2>{});
+    load(0, GmInt<3>{});
+    for (int Q = 0; Q + 1 < t.nQ; ++Q) quad(Q, GmInt<1>{});
+    quad(t.nQ - 1, GmInt<0>{});
+}
+
+template <typename Y, bool GATED, int TM, int NB>
+__device__ __forceinline__ void mx_gemm_tile(const MxProduct &g, const MxWave<TM> &t, int p0, int np,
+                                             int rb0)
+{
+    k3v4f acc[4][NB];
+    mx_gemm_sums<TM, NB>(t, acc);
+    const int c = t.lane & 15, q = t.lane >> 4, nrb = g.N / 16;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+        if (16 * n + c >= np) continue;
+        Y *o = (Y *)g.y + (size_t)(p0 + 16 * n + c) * g.N + 4 * q;
+#pragma unroll
+        for (int r = 0; r < (GATED ? 2 : 4); ++r) {
+            if (rb0 + r >= nrb) continue;
+            k3v4f v = acc[r][n];
+            if (GATED) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = k3d_act(v[i], acc[r + 2][n][i], g.b1, g.b2);
+            }
+            mx_put(o + 16 * (rb0 + r), v);
+        }
+    }
+}
+
+/* Workgroup b runs on XCD b % 8. One matrix: each XCD takes an eighth of the (feature tile, row
+ * tile) pairs, so a matrix's tiles are read by one L2. Experts: row tiles two by two to the XCDs,
+ * a feature tile of both at a time, so an expert's second tile finds its weights in that L2. */
+template <int TM>
+__device__ __forceinline__ bool mx_item(const MxProduct &g, int nft, int &ft, int &e, int &p0, int &np)
+{
+    const int xcd = blockIdx.x & 7, s = blockIdx.x >> 3;
+    if (!g.off) {
+        const int tiles = (g.P + TM - 1) / TM, items = tiles * nft, per = (items + 7) / 8;
+        const int i = xcd * per + s;
+        if (s >= per || i >= items) return false;
+        ft = i / tiles;
+        return mx_tile<TM>(g, i - ft * tiles, e, p0, np);
+    }
+    const int grp = s / (2 * nft), in = s - grp * 2 * nft;
+    ft = in >> 1;
+    return mx_tile<TM>(g, 2 * (8 * grp + xcd) + (in & 1), e, p0, np);
+}
+
+template <typename Y, bool GATED, int TM>
+__global__ void __launch_bounds__(256, 2)
+k_mx_gemm(const MxProduct g)
+{
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * MxWave<TM>::STAGE];
+    constexpr int RB = GATED ? 2 : 4;           /* row blocks of a wave in a matrix */
+    const int nrb = g.N / 16, nft = (nrb + 4 * RB - 1) / (4 * RB);
+    int ft, e, p0, np;
+    if (!mx_item<TM>(g, nft, ft, e, p0, np)) return;
+    MxWave<TM> t;
+    t.lane = threadIdx.x & 63;
+    t.wave = gm_uniform(threadIdx.x >> 6);
+    t.nQ = g.nQ;
+    t.nK = g.nK;
+    t.xq = g.xq;
+    t.lds = (uint32_t)(uintptr_t)(k3lds)lds;
+    t.ldsp = lds;
+    const uint8_t *w1 = mx_matrix(g, g.w, e), *w3 = GATED ? mx_matrix(g, g.w3, e) : w1;
+    const int rb0 = (4 * ft + t.wave) * RB;
+    const uint32_t row16 = g.nQ * (MX_XQ / 16);
+    if (!w1 || !w3) {                           /* no matrix: rows of zeros */
+        const int n0 = 64 * RB * ft, n = min(64 * RB, g.N - n0);
+        for (int i = threadIdx.x; i < np * n; i += 256)
+            ((Y *)g.y)[(size_t)(p0 + i / n) * g.N + n0 + i % n] = (Y)0;
+        return;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int rb = rb0 + (GATED ? r & 1 : r);
+        t.w[r] = gm_uniform_ptr((GATED && r >= 2 ? w3 : w1) + (rb >= nrb ? 0 : (size_t)rb * g.nQ * MX_QT));
+    }
+    auto source = [&](int r) {
+        const int row = mx_row(g, p0 + min(r, np - 1));
+        return (uint32_t)(row < 0 ? g.T : row) * row16;
+    };
+    const int nb = (np + 15) / 16, sub = 4 * t.wave + (t.lane >> 4);
+#pragma unroll
+    for (int i = 0; i < TM / 16; ++i) t.x[i] = source(16 * i + sub) + ((t.lane & 15) ^ sub);
+    t.xs = source(64 * t.wave + t.lane) + 16;
+    if constexpr (TM == 128) {
+        if (nb > 6) return mx_gemm_tile<Y, GATED, TM, 8>(g, t, p0, np, rb0);
+        if (nb > 4) return mx_gemm_tile<Y, GATED, TM, 6>(g, t, p0, np, rb0);
+    }
+    if constexpr (TM >= 64) {
+        if (nb > 2) return mx_gemm_tile<Y, GATED, TM, 4>(g, t, p0, np, rb0);
+    }
+    if (nb > 1) return mx_gemm_tile<Y, GATED, TM, 2>(g, t, p0, np, rb0);
+    mx_gemm_tile<Y, GATED, TM, 1>(g, t, p0, np, rb0);
+}
+
 /* ------------------------------------------------------------- entry points ---- */
 
 static int mx_type(const char *who, int dt)
@@ -334,8 +553,11 @@ extern "C" int k3g_dequant_mxfp4(const void *packed, const void *scales, int row
 
 extern "C" size_t k3g_mxfp4_work_bytes(int rows, int cols)
 {
-    if (!mx_shape_ok(rows, cols)) return 0;
-    return (size_t)rows * ((cols + 511) / 512) * MX_XQ;
+    if (!mx_shape_ok(rows, cols) || !rows) return 0;
+    /* and a row of zeros behind them, for places without one; the kernels count it in 32 bits of
+     * 16 bytes each */
+    const size_t n = ((size_t)rows + 1) * ((cols + 511) / 512) * MX_XQ;
+    return n >> 36 ? 0 : n;
 }
 
 /* the product of checked arguments */
@@ -343,6 +565,10 @@ static int mx_product(const char *who, MxProduct &g, const void *x, int xdt, int
                       void *work, size_t work_bytes, void *stream)
 {
     const size_t need = k3g_mxfp4_work_bytes(g.T, cols);
+    if (!need) {
+        fprintf(stderr, "%s: %d x %d activations do not fit 64 GiB in MXFP4\n", who, g.T, cols);
+        return -1;
+    }
     if (!work || k3h_misaligned(work, 16) || work_bytes < need) {
         fprintf(stderr, "%s: needs a workspace of %zu bytes, aligned to 16 (%zu given)\n", who, need,
                 work ? work_bytes : (size_t)0);
@@ -354,20 +580,30 @@ static int mx_product(const char *who, MxProduct &g, const void *x, int xdt, int
     g.nK = (cols + 127) / 128;
     g.xq = (const uint8_t *)work;
     const size_t nquads = (size_t)g.T * g.nQ;
-    const dim3 xgrid((unsigned)((nquads + 3) / 4));
+    const dim3 xgrid((unsigned)((nquads + g.nQ + 3) / 4));
     if (xdt == K3_WBF16 ? k3h_launch(who, k_mx_x<uint16_t>, xgrid, dim3(256), on.st, (const uint16_t *)x,
                                      nquads, g.nQ, cols, (uint8_t *)work)
                         : k3h_launch(who, k_mx_x<float>, xgrid, dim3(256), on.st, (const float *)x, nquads,
                                      g.nQ, cols, (uint8_t *)work))
         return -1;
-    const int tiles = g.off ? g.P / 16 + min(g.E, g.P) : (g.P + 15) / 16;
-    const dim3 grid(tiles, g.N / 16);
-    const bool bf = ydt == K3_WBF16;
-    if (g.w3)
-        return bf ? k3h_launch(who, k_mx_tile<uint16_t, true>, grid, dim3(64), on.st, (const MxProduct)g)
-                  : k3h_launch(who, k_mx_tile<float, true>, grid, dim3(64), on.st, (const MxProduct)g);
-    return bf ? k3h_launch(who, k_mx_tile<uint16_t, false>, grid, dim3(64), on.st, (const MxProduct)g)
-              : k3h_launch(who, k_mx_tile<float, false>, grid, dim3(64), on.st, (const MxProduct)g);
+    const bool bf = ydt == K3_WBF16, gated = g.w3 != nullptr;
+    const int met = g.off ? min(g.E, g.P) : 1;      /* experts with rows, at most */
+    if (g.P <= MX_FEW * met) {
+        const dim3 grid(g.off ? g.P / 16 + met : (g.P + 15) / 16, g.N / 16);
+        auto *k = bf ? (gated ? k_mx_tile<uint16_t, true> : k_mx_tile<uint16_t, false>)
+                     : (gated ? k_mx_tile<float, true> : k_mx_tile<float, false>);
+        return k3h_launch(who, k, grid, dim3(64), on.st, (const MxProduct)g);
+    }
+    const int nft = (g.N + (gated ? 127 : 255)) / (gated ? 128 : 256);
+    const int tm = g.P > MX_TM128 * met ? 128 : 64;
+    /* workgroups of an XCD (mx_item) */
+    const int64_t tiles = g.off ? g.P / tm + met : (g.P + tm - 1) / tm;
+    const int64_t per = g.off ? (tiles + 15) / 16 * 2 * nft : (tiles * nft + 7) / 8;
+    auto *k = tm == 128 ? (bf ? (gated ? k_mx_gemm<uint16_t, true, 128> : k_mx_gemm<uint16_t, false, 128>)
+                              : (gated ? k_mx_gemm<float, true, 128> : k_mx_gemm<float, false, 128>))
+                        : (bf ? (gated ? k_mx_gemm<uint16_t, true, 64> : k_mx_gemm<uint16_t, false, 64>)
+                              : (gated ? k_mx_gemm<float, true, 64> : k_mx_gemm<float, false, 64>));
+    return k3h_launch(who, k, dim3((unsigned)(8 * per)), dim3(256), on.st, (const MxProduct)g);
 }
 
 static int mx_features(const char *who, int n)
