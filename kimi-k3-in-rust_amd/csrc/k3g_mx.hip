@@ -26,13 +26,6 @@
 #define MX_MAX_ROWS (1 << 26)
 #define MX_MAX_COLS (1 << 20)
 
-#ifndef MX_FEW
-#define MX_FEW 8
-#endif
-#ifndef MX_TM128
-#define MX_TM128 48
-#endif
-
 typedef int mx_v8i __attribute__((ext_vector_type(8)));
 
 /* ------------------------------------------------------------- quantisation ---- */
@@ -150,8 +143,9 @@ k_mx_x(const T *__restrict__ x, size_t nquads, int nQ, int cols, uint8_t *__rest
 /* ------------------------------------------------------------------ product ---- */
 
 struct MxProduct {
-    const uint8_t *xq;               /* activation quads of T rows */
-    int T, nQ, nK;                   /* rows; quads and 128-column chunks of a row */
+    const uint8_t *xq;               /* activation quads of T rows and a row of zeros */
+    const void *x;                   /* the rows themselves */
+    int T, cols, nQ, nK;             /* rows; columns, quads and 128-column chunks of a row */
     const int32_t *perm;             /* place -> pair, or NULL: place r is row r */
     int topk;
     const int32_t *off;              /* [E + 1] places of each expert, or NULL: one, all places */
@@ -220,63 +214,11 @@ __device__ __forceinline__ const uint8_t *mx_matrix(const MxProduct &g, const ui
     return gm_uniform_ptr(*(const uint8_t *const *)(w + (size_t)e * g.step));
 }
 
-__device__ __forceinline__ k3v4f mx_mma(const uint4 &a, uint32_t sa, const uint4 &b, uint32_t sb,
-                                        const k3v4f &acc)
-{
-    const mx_v8i av = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
-    const mx_v8i bv = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc, 4, 4, 0, (int)sa, 0, (int)sb);
-}
-
 __device__ __forceinline__ void mx_put(float *o, const k3v4f &v) { *(k3v4f *)o = v; }
 __device__ __forceinline__ void mx_put(uint16_t *o, const k3v4f &v)
 {
     *(uint2 *)o = make_uint2(k3d_bf16x2(v[0], v[1]), k3d_bf16x2(v[2], v[3]));
 }
-
-/* One wave: 16 places by 16 features. */
-template <typename Y, bool GATED>
-__global__ void __launch_bounds__(64)
-k_mx_tile(const MxProduct g)
-{
-    int e, p0, np;
-    if (!mx_tile<16>(g, blockIdx.x, e, p0, np)) return;
-    const int lane = threadIdx.x, c = lane & 15, q = lane >> 4, rb = blockIdx.y;
-    const uint8_t *w1 = mx_matrix(g, g.w, e), *w3 = GATED ? mx_matrix(g, g.w3, e) : w1;
-    k3v4f acc = {0.f, 0.f, 0.f, 0.f}, up = acc;
-    if (w1 && w3) {
-        const int row = c < np ? mx_row(g, p0 + c) : -1;
-        const uint8_t *x = g.xq + (size_t)max(row, 0) * g.nQ * MX_XQ;
-        w1 += (size_t)rb * g.nQ * MX_QT;
-        w3 += (size_t)rb * g.nQ * MX_QT;
-        for (int k = 0; k < g.nK; ++k) {
-            const int Q = k >> 2, j = k & 3;
-            uint4 b = make_uint4(0, 0, 0, 0);
-            uint32_t sb = 127;
-            if (row >= 0) {
-                b = gm_ld16(x + (size_t)Q * MX_XQ + 64 * j + 16 * q);
-                sb = x[(size_t)Q * MX_XQ + 256 + 4 * q + j];
-            }
-            const uint8_t *t1 = w1 + (size_t)Q * MX_QT, *t3 = w3 + (size_t)Q * MX_QT;
-            acc = mx_mma(gm_ld16(t1 + 1024 * j + 16 * lane), (gm_ld4(t1 + 4096 + 4 * lane) >> (8 * j)) & 255u,
-                         b, sb, acc);
-            if (GATED)
-                up = mx_mma(gm_ld16(t3 + 1024 * j + 16 * lane),
-                            (gm_ld4(t3 + 4096 + 4 * lane) >> (8 * j)) & 255u, b, sb, up);
-        }
-    }
-    if (GATED) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = k3d_act(acc[i], up[i], g.b1, g.b2);
-    }
-    if (c < np) mx_put((Y *)g.y + (size_t)(p0 + c) * g.N + 16 * rb + 4 * q, acc);
-}
-
-/* ---- many rows: a workgroup of four waves takes up to TM places by 4 x 64 features (gated: 4 x
- * 32 of each matrix). The activation quads of its places go to LDS by DMA, two stages of one quad;
- * the 16-byte unit u of row r lies at slot u ^ (r % 16) of the row's 256 bytes, so the 16 rows of
- * an operand read 16 different slots. Weights go straight from memory to registers, four chunks
- * ahead: no two waves of a workgroup share them. */
 
 template <int J>
 __device__ __forceinline__ k3v4f mx_mma4(const gm_v4u &a, uint32_t sa, const gm_v4u &b, uint32_t sb,
@@ -286,6 +228,227 @@ __device__ __forceinline__ k3v4f mx_mma4(const gm_v4u &a, uint32_t sa, const gm_
     const mx_v8i bv = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc, 4, 4, J, (int)sa, J, (int)sb);
 }
+
+/* v, worked out from here on: an address made of it is not kept in registers over a loop (64-bit
+ * ones of every weight and activation pointer took 25 registers more than there are) */
+__device__ __forceinline__ uint32_t mx_here(uint32_t v)
+{
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+/* Workgroup b runs on XCD b % 8. One matrix: each XCD takes an eighth of the (feature tile, row
+ * tile) pairs, so a matrix's tiles are read by one L2. Experts: the feature tiles are dealt to the
+ * XCDs one by one, each with two row tiles one after the other, so an expert's second row tile
+ * finds its weights in that L2, and a few experts still fill every XCD. */
+template <int TM>
+__device__ __forceinline__ bool mx_item(const MxProduct &g, int nft, int &ft, int &e, int &p0, int &np)
+{
+    const int xcd = blockIdx.x & 7, s = blockIdx.x >> 3;
+    if (!g.off) {
+        const int tiles = (g.P + TM - 1) / TM, items = tiles * nft, per = (items + 7) / 8;
+        const int i = xcd * per + s;
+        if (s >= per || i >= items) return false;
+        ft = i / tiles;
+        return mx_tile<TM>(g, i - ft * tiles, e, p0, np);
+    }
+    const int i = 8 * (s >> 1) + xcd, pair = i / nft;
+    ft = i - pair * nft;
+    return mx_tile<TM>(g, 2 * pair + (s & 1), e, p0, np);
+}
+
+/* np rows of zeros from p0 on, features n0 .. n0 + n (an expert without a matrix) */
+template <typename Y, int THREADS>
+__device__ __forceinline__ void mx_zeros(const MxProduct &g, int p0, int np, int n0, int n)
+{
+    n = min(n, g.N - n0);
+    for (int i = threadIdx.x; i < np * n; i += THREADS)
+        ((Y *)g.y)[(size_t)(p0 + i / n) * g.N + n0 + i % n] = (Y)0;
+}
+
+/* ---- few rows: a workgroup of WV waves takes 16 NB places by U row blocks of 16 features (gated:
+ * U / 2 of each matrix), and the waves share the columns: wave v sums quads v, v + WV, ..., so all
+ * the weights of a row block are asked for at once however few row blocks there are. The partial
+ * sums meet in LDS and are added in the order of the waves. Both operands come straight from
+ * memory, a quad ahead.
+ *
+ * X: what x is: activation quads, or (a few tokens, NB 1) fp32 or bf16 values that every workgroup
+ * quantises by itself, a quad of each row at a time by the wave that needs it: one launch less,
+ * for 8 loads and about 40 operations a row and quad beside the 4 KB of each row block. */
+struct MxQuads;
+
+template <typename X, int U, int NB>
+struct MxFew {
+    const uint8_t *w[U];               /* the row blocks' first quads */
+    uint32_t x[NB];                    /* this lane's row, in units of 16 bytes (X quads) */
+    const X *row;                      /* x itself */
+    uint8_t *lds;                      /* this wave's quads of 16 rows (X values) */
+    int lane, np, p0;
+};
+
+template <typename X, int WV, int U, int NB>
+__device__ __forceinline__ void mx_few_sums(const MxProduct &g, const MxFew<X, U, NB> &t, int wave,
+                                            k3v4f (&acc)[U][NB])
+{
+    constexpr bool QUADS = __is_same(X, MxQuads);
+    static_assert(QUADS || NB == 1, "values only with one block of rows");
+    const int c = t.lane & 15, q = t.lane >> 4;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int n = 0; n < NB; ++n) acc[u][n] = k3v4f{0.f, 0.f, 0.f, 0.f};
+    gm_v4u a[4][U], b[4][NB];
+    uint32_t sA[2][U], sB[2][NB];
+    auto load = [&](int Q, auto jc) {
+        constexpr int J = decltype(jc)::value;
+        const uint32_t at = mx_here(16 * t.lane);
+#pragma unroll
+        for (int u = 0; u < U; ++u) a[J][u] = *(gm_g4)(t.w[u] + (size_t)Q * MX_QT + 1024 * J + at);
+        if constexpr (QUADS) {
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+                b[J][n] = *(gm_g4)(g.xq + (size_t)Q * MX_XQ + (uint64_t)mx_here(t.x[n]) * 16 + 64 * J + 16 * q);
+        }
+    };
+    auto load_scales = [&](int Q, uint32_t (&s)[U], uint32_t (&sb)[NB]) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) s[u] = gm_ld4(t.w[u] + (size_t)Q * MX_QT + 4096 + mx_here(4 * t.lane));
+        if constexpr (QUADS) {
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+                sb[n] = gm_ld4(g.xq + (size_t)Q * MX_XQ + (uint64_t)mx_here(t.x[n]) * 16 + 256 + 4 * q);
+        }
+    };
+    /* this quad of every row into LDS, unit u of row r at slot u ^ r, the scales behind */
+    auto values = [&](int Q) {
+        if constexpr (!QUADS) {
+            const int col = 512 * Q + 8 * t.lane, blk = t.lane >> 2, cols = g.cols;
+            gm_wave_sync();
+            for (int r = 0; r < t.np; ++r) {
+                const int row = gm_uniform(mx_row(g, t.p0 + r));
+                Mx8 v = {{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}};
+                if (col < cols && row >= 0) v = mx_load8(t.row + (size_t)row * cols + col);
+                uint32_t s;
+                const uint32_t code = mx_quant8(v, s);
+                *(uint32_t *)(t.lds + 256 * r + 16 * (blk ^ r) + 4 * (t.lane & 3)) = code;
+                if ((t.lane & 3) == 0) t.lds[4096 + 16 * r + 4 * (blk & 3) + (blk >> 2)] = (uint8_t)s;
+            }
+            gm_wave_sync();
+            sB[0][0] = *(const uint32_t *)(t.lds + 4096 + 16 * c + 4 * q);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[j][0] = *(const gm_v4u *)(t.lds + 256 * c + 16 * ((4 * j + q) ^ c));
+        }
+    };
+    auto chunk = [&](auto jc) {
+        constexpr int J = decltype(jc)::value;
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int u = 0; u < U; ++u) acc[u][n] = mx_mma4<J>(a[J][u], sA[0][u], b[J][n], sB[0][n], acc[u][n]);
+    };
+    if (wave >= g.nQ) return;
+    load_scales(wave, sA[0], sB[0]);
+    load(wave, GmInt<0>{});
+    load(wave, GmInt<1>{});
+    load(wave, GmInt<2>{});
+    load(wave, GmInt<3>{});
+    int Q = wave;
+    for (; Q + WV < g.nQ; Q += WV) {
+        load_scales(Q + WV, sA[1], sB[1]);
+        values(Q);
+        chunk(GmInt<0>{});
+        load(Q + WV, GmInt<0>{});
+        chunk(GmInt<1>{});
+        load(Q + WV, GmInt<1>{});
+        chunk(GmInt<2>{});
+        load(Q + WV, GmInt<2>{});
+        chunk(GmInt<3>{});
+        load(Q + WV, GmInt<3>{});
+#pragma unroll
+        for (int u = 0; u < U; ++u) sA[0][u] = sA[1][u];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) sB[0][n] = sB[1][n];
+    }
+    values(Q);
+    const int left = g.nK - 4 * Q;
+    chunk(GmInt<0>{});
+    if (left > 1) chunk(GmInt<1>{});
+    if (left > 2) chunk(GmInt<2>{});
+    if (left > 3) chunk(GmInt<3>{});
+}
+
+template <typename X, typename Y, bool GATED, int WV, int U, int NB>
+__global__ void __launch_bounds__(64 * WV)
+k_mx_few(const MxProduct g)
+{
+    constexpr bool QUADS = __is_same(X, MxQuads);
+    constexpr int RB = GATED ? U / 2 : U, SUMS = WV * U * NB * 1024, VALUES = QUADS ? 0 : WV * MX_QT;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[SUMS > VALUES ? SUMS : VALUES];
+    const int nrb = g.N / 16, nft = (nrb + RB - 1) / RB;
+    int ft, e, p0, np;
+    if (!mx_item<16 * NB>(g, nft, ft, e, p0, np)) return;
+    const uint8_t *w1 = mx_matrix(g, g.w, e), *w3 = GATED ? mx_matrix(g, g.w3, e) : w1;
+    if (!w1 || !w3) {
+        mx_zeros<Y, 64 * WV>(g, p0, np, 16 * RB * ft, 16 * RB);
+        return;
+    }
+    const int wave = gm_uniform(threadIdx.x >> 6);
+    MxFew<X, U, NB> t;
+    t.lane = threadIdx.x & 63;
+    const int c = t.lane & 15, q = t.lane >> 4;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int rb = RB * ft + u % RB;
+        t.w[u] = gm_uniform_ptr((u >= RB ? w3 : w1) + (rb >= nrb ? 0 : (size_t)rb * g.nQ * MX_QT));
+    }
+    if constexpr (QUADS) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            const int row = mx_row(g, p0 + min(16 * n + c, np - 1));
+            t.x[n] = (uint32_t)(row < 0 ? g.T : row) * (g.nQ * (MX_XQ / 16));
+        }
+    } else {
+        t.row = (const X *)g.x;
+        t.lds = lds + wave * MX_QT;
+    }
+    t.np = np;
+    t.p0 = p0;
+    k3v4f acc[U][NB];
+    mx_few_sums<X, WV, U, NB>(g, t, wave, acc);
+    /* the waves' sums: tile (u, n) of wave v at (v U NB + u NB + n) KB, 16 bytes a lane */
+    if constexpr (!QUADS) __syncthreads();
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+            *(k3v4f *)(lds + 1024 * ((wave * U + u) * NB + n) + 16 * t.lane) = acc[u][n];
+    __syncthreads();
+    auto total = [&](int u, int n) {
+        k3v4f s = *(const k3v4f *)(lds + 1024 * (u * NB + n) + 16 * t.lane);
+#pragma unroll
+        for (int v = 1; v < WV; ++v)
+            if (v < g.nQ) s += *(const k3v4f *)(lds + 1024 * ((v * U + u) * NB + n) + 16 * t.lane);
+        return s;
+    };
+#pragma unroll
+    for (int i0 = 0; i0 < RB * NB; i0 += WV) {
+        const int i = i0 + wave, r = i / NB, n = i - r * NB;
+        if (i >= RB * NB || RB * ft + r >= nrb || 16 * n + c >= np) continue;
+        k3v4f v = total(r, n);
+        if (GATED) {
+            const k3v4f up = total(RB + r, n);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = k3d_act(v[j], up[j], g.b1, g.b2);
+        }
+        mx_put((Y *)g.y + (size_t)(p0 + 16 * n + c) * g.N + 16 * (RB * ft + r) + 4 * q, v);
+    }
+}
+
+/* ---- many rows: a workgroup of four waves takes up to TM places by 4 x 64 features (gated: 4 x
+ * 32 of each matrix). The activation quads of its places go to LDS by DMA, two stages of one quad;
+ * the 16-byte unit u of row r lies at slot u ^ (r % 16) of the row's 256 bytes, so the 16 rows of
+ * an operand read 16 different slots. Weights go straight from memory to registers, four chunks
+ * ahead: no two waves of a workgroup share them. */
 
 template <int TM>
 struct MxWave {
@@ -298,14 +461,6 @@ struct MxWave {
     const uint8_t *ldsp;
     int lane, wave, nQ, nK;
 };
-
-/* v, worked out from here on: an address made of it is not kept in registers over a loop (64-bit
- * ones of every weight and activation pointer took 25 registers more than there are) */
-__device__ __forceinline__ uint32_t mx_here(uint32_t v)
-{
-    asm volatile("" : "+v"(v));
-    return v;
-}
 
 /* NB blocks of 16 places */
 template <int TM, int NB>
@@ -415,25 +570,6 @@ __device__ __forceinline__ void mx_gemm_tile(const MxProduct &g, const MxWave<TM
     }
 }
 
-/* Workgroup b runs on XCD b % 8. One matrix: each XCD takes an eighth of the (feature tile, row
- * tile) pairs, so a matrix's tiles are read by one L2. Experts: row tiles two by two to the XCDs,
- * a feature tile of both at a time, so an expert's second tile finds its weights in that L2. */
-template <int TM>
-__device__ __forceinline__ bool mx_item(const MxProduct &g, int nft, int &ft, int &e, int &p0, int &np)
-{
-    const int xcd = blockIdx.x & 7, s = blockIdx.x >> 3;
-    if (!g.off) {
-        const int tiles = (g.P + TM - 1) / TM, items = tiles * nft, per = (items + 7) / 8;
-        const int i = xcd * per + s;
-        if (s >= per || i >= items) return false;
-        ft = i / tiles;
-        return mx_tile<TM>(g, i - ft * tiles, e, p0, np);
-    }
-    const int grp = s / (2 * nft), in = s - grp * 2 * nft;
-    ft = in >> 1;
-    return mx_tile<TM>(g, 2 * (8 * grp + xcd) + (in & 1), e, p0, np);
-}
-
 template <typename Y, bool GATED, int TM>
 __global__ void __launch_bounds__(256, 2)
 k_mx_gemm(const MxProduct g)
@@ -454,10 +590,8 @@ k_mx_gemm(const MxProduct g)
     const uint8_t *w1 = mx_matrix(g, g.w, e), *w3 = GATED ? mx_matrix(g, g.w3, e) : w1;
     const int rb0 = (4 * ft + t.wave) * RB;
     const uint32_t row16 = g.nQ * (MX_XQ / 16);
-    if (!w1 || !w3) {                           /* no matrix: rows of zeros */
-        const int n0 = 64 * RB * ft, n = min(64 * RB, g.N - n0);
-        for (int i = threadIdx.x; i < np * n; i += 256)
-            ((Y *)g.y)[(size_t)(p0 + i / n) * g.N + n0 + i % n] = (Y)0;
+    if (!w1 || !w3) {
+        mx_zeros<Y, 256>(g, p0, np, 64 * RB * ft, 64 * RB);
         return;
     }
 #pragma unroll
@@ -560,6 +694,99 @@ extern "C" size_t k3g_mxfp4_work_bytes(int rows, int cols)
     return n >> 36 ? 0 : n;
 }
 
+/* Which kernel a product runs on: rows of a tile, its row blocks (of each matrix), the waves that
+ * share its columns (0: k_mx_gemm), and whether x is quantised inside it. */
+struct MxPlan {
+    int tm, rb, wv;
+    bool values;
+};
+
+/* workgroups of tiles of tm rows by rb row blocks, as many as mx_item may be asked for */
+static int64_t mx_grid(const MxProduct &g, int tm, int rb)
+{
+    const int64_t nft = (g.N / 16 + rb - 1) / rb;
+    if (!g.off) return ((g.P + tm - 1) / tm * nft + 7) / 8 * 8;
+    const int64_t tiles = g.P / tm + min(g.E, g.P);
+    return ((tiles + 1) / 2 * nft + 7) / 8 * 16;
+}
+
+/* A larger tile reads less, a smaller one makes more workgroups: the largest tile that still gives
+ * most CUs one (us, whole calls, bf16).
+ * One matrix, 7168 columns, 3584 features unless said: 1 row: quantised inside 5.5, before 7.2; 4:
+ * 7.6 and 7.7; 8: 10.8 and 7.5. 16 rows: 8 waves x 1 row block 8.5, 4 x 2 9.5, 4 x 4 12.4; 32 rows:
+ * 11.3, 9.2, 12.0; 64 rows: 16.6, 12.9, 11.7; 128 rows: 4 x 4 by 16 rows 16.4, by 32 14.1, by 64
+ * 19.2; 256 rows: 26.2, 21.8, 19.3, k_mx_gemm 27.9; 512 rows: by 64 33.9, k_mx_gemm 29.1. 6144
+ * features: 512 rows, k_mx_gemm by 64 29.7, by 128 38.7; 1024 rows 49.0, 42.4.
+ * Experts: a few tokens meet about one row an expert, and the weights are all there is to wait for
+ * (8 tokens x 8 by 384 experts of 7168 -> 2 x 2048: inside 138, before 139, k_mx_gemm 150; 1 token:
+ * 22.6, 24.7, 26.1); where 16 tokens meet 8 experts quantising inside costs 16.8 against 11.9. 64
+ * tokens x 2 by 8 experts of 4096 -> 2 x 1408: 4 x 4 by 16 rows 15.1, k_mx_gemm 19.5; 256: 25.6, by
+ * 32 24.9, k_mx_gemm by 64 27.6; 1024: 53.9, k_mx_gemm by 64 40.5, by 128 51.9; 4096 x 8 by 384 of
+ * 2048 -> 7168: k_mx_gemm by 64 815, by 128 741. */
+static MxPlan mx_plan(const MxProduct &g, bool gated)
+{
+    const int RB = gated ? 2 : 4;
+    if (!g.off) {
+        if (g.P <= 4) return {16, 1, 8, true};
+        if (mx_grid(g, 128, 16) >= 160) return {128, 16, 0, false};
+        if (mx_grid(g, 64, 16) >= 96) return {64, 16, 0, false};
+        if (mx_grid(g, 64, 4) >= 192) return {64, 4, 4, false};
+        if (mx_grid(g, 32, 4) >= 192) return {32, 4, 4, false};
+        if (mx_grid(g, 16, 4) >= 192) return {16, 4, 4, false};
+        if (mx_grid(g, 16, 2) >= 192) return {16, 2, 4, false};
+        return {16, 1, 8, false};
+    }
+    const int met = min(g.E, g.P), mean = (g.P + met - 1) / met;
+    if (g.T <= 16 && mean <= 2) return {16, RB, 4, true};
+    /* row tiles there will be, about: one an expert or more */
+    const int64_t nft = (g.N / 16 + 4 * RB - 1) / (4 * RB);
+    if (mean > 48 && max(met, g.P / 128) * nft >= 256) return {128, 4 * RB, 0, false};
+    if (max(met, g.P / 64) * nft >= 256) return {64, 4 * RB, 0, false};
+    return {mean > 16 ? 32 : 16, RB, 4, false};
+}
+
+template <typename X, typename Y, bool GATED, int WV, int U, int NB>
+static int mx_run_few(const char *who, const MxProduct &g, hipStream_t st)
+{
+    const dim3 grid((unsigned)mx_grid(g, 16 * NB, GATED ? U / 2 : U));
+    return k3h_launch(who, k_mx_few<X, Y, GATED, WV, U, NB>, grid, dim3(64 * WV), st, (MxProduct)g);
+}
+
+template <typename Y, bool GATED, int TM>
+static int mx_run_gemm(const char *who, const MxProduct &g, hipStream_t st)
+{
+    const dim3 grid((unsigned)mx_grid(g, TM, GATED ? 8 : 16));
+    return k3h_launch(who, k_mx_gemm<Y, GATED, TM>, grid, dim3(256), st, (MxProduct)g);
+}
+
+template <typename X>
+static int mx_launch_values(const char *who, const MxProduct &g, const MxPlan &p, bool bf, bool gated,
+                            hipStream_t st)
+{
+    if (gated) return bf ? mx_run_few<X, uint16_t, true, 4, 4, 1>(who, g, st)
+                         : mx_run_few<X, float, true, 4, 4, 1>(who, g, st);
+    if (p.wv == 8) return bf ? mx_run_few<X, uint16_t, false, 8, 1, 1>(who, g, st)
+                             : mx_run_few<X, float, false, 8, 1, 1>(who, g, st);
+    return bf ? mx_run_few<X, uint16_t, false, 4, 4, 1>(who, g, st)
+              : mx_run_few<X, float, false, 4, 4, 1>(who, g, st);
+}
+
+template <typename Y>
+static int mx_launch(const char *who, const MxProduct &g, const MxPlan &p, bool gated, hipStream_t st)
+{
+    if (!p.wv) {
+        if (gated) return p.tm == 128 ? mx_run_gemm<Y, true, 128>(who, g, st) : mx_run_gemm<Y, true, 64>(who, g, st);
+        return p.tm == 128 ? mx_run_gemm<Y, false, 128>(who, g, st) : mx_run_gemm<Y, false, 64>(who, g, st);
+    }
+    if (gated) return p.tm == 32 ? mx_run_few<MxQuads, Y, true, 4, 4, 2>(who, g, st)
+                                 : mx_run_few<MxQuads, Y, true, 4, 4, 1>(who, g, st);
+    if (p.wv == 8) return mx_run_few<MxQuads, Y, false, 8, 1, 1>(who, g, st);
+    if (p.rb == 2) return mx_run_few<MxQuads, Y, false, 4, 2, 1>(who, g, st);
+    if (p.tm == 64) return mx_run_few<MxQuads, Y, false, 4, 4, 4>(who, g, st);
+    return p.tm == 32 ? mx_run_few<MxQuads, Y, false, 4, 4, 2>(who, g, st)
+                      : mx_run_few<MxQuads, Y, false, 4, 4, 1>(who, g, st);
+}
+
 /* the product of checked arguments */
 static int mx_product(const char *who, MxProduct &g, const void *x, int xdt, int cols, int ydt,
                       void *work, size_t work_bytes, void *stream)
@@ -579,6 +806,13 @@ static int mx_product(const char *who, MxProduct &g, const void *x, int xdt, int
     g.nQ = (cols + 511) / 512;
     g.nK = (cols + 127) / 128;
     g.xq = (const uint8_t *)work;
+    g.x = x;
+    g.cols = cols;
+    const bool bf = ydt == K3_WBF16, gated = g.w3 != nullptr;
+    const MxPlan plan = mx_plan(g, gated);
+    if (plan.values)
+        return xdt == K3_WBF16 ? mx_launch_values<uint16_t>(who, g, plan, bf, gated, on.st)
+                               : mx_launch_values<float>(who, g, plan, bf, gated, on.st);
     const size_t nquads = (size_t)g.T * g.nQ;
     const dim3 xgrid((unsigned)((nquads + g.nQ + 3) / 4));
     if (xdt == K3_WBF16 ? k3h_launch(who, k_mx_x<uint16_t>, xgrid, dim3(256), on.st, (const uint16_t *)x,
@@ -586,24 +820,7 @@ static int mx_product(const char *who, MxProduct &g, const void *x, int xdt, int
                         : k3h_launch(who, k_mx_x<float>, xgrid, dim3(256), on.st, (const float *)x, nquads,
                                      g.nQ, cols, (uint8_t *)work))
         return -1;
-    const bool bf = ydt == K3_WBF16, gated = g.w3 != nullptr;
-    const int met = g.off ? min(g.E, g.P) : 1;      /* experts with rows, at most */
-    if (g.P <= MX_FEW * met) {
-        const dim3 grid(g.off ? g.P / 16 + met : (g.P + 15) / 16, g.N / 16);
-        auto *k = bf ? (gated ? k_mx_tile<uint16_t, true> : k_mx_tile<uint16_t, false>)
-                     : (gated ? k_mx_tile<float, true> : k_mx_tile<float, false>);
-        return k3h_launch(who, k, grid, dim3(64), on.st, (const MxProduct)g);
-    }
-    const int nft = (g.N + (gated ? 127 : 255)) / (gated ? 128 : 256);
-    const int tm = g.P > MX_TM128 * met ? 128 : 64;
-    /* workgroups of an XCD (mx_item) */
-    const int64_t tiles = g.off ? g.P / tm + met : (g.P + tm - 1) / tm;
-    const int64_t per = g.off ? (tiles + 15) / 16 * 2 * nft : (tiles * nft + 7) / 8;
-    auto *k = tm == 128 ? (bf ? (gated ? k_mx_gemm<uint16_t, true, 128> : k_mx_gemm<uint16_t, false, 128>)
-                              : (gated ? k_mx_gemm<float, true, 128> : k_mx_gemm<float, false, 128>))
-                        : (bf ? (gated ? k_mx_gemm<uint16_t, true, 64> : k_mx_gemm<uint16_t, false, 64>)
-                              : (gated ? k_mx_gemm<float, true, 64> : k_mx_gemm<float, false, 64>));
-    return k3h_launch(who, k, dim3((unsigned)(8 * per)), dim3(256), on.st, (const MxProduct)g);
+    return bf ? mx_launch<uint16_t>(who, g, plan, gated, on.st) : mx_launch<float>(who, g, plan, gated, on.st);
 }
 
 static int mx_features(const char *who, int n)
