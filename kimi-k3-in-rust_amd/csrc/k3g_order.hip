@@ -42,15 +42,12 @@ __device__ __forceinline__ uint64_t od_peers(int key, int nb)
     return peers;
 }
 
-__device__ __forceinline__ int od_key(const int32_t *idx, int p, int end, int E, int *err)
+/* An expert number, -1 for a dropped pair's and, reported, for one past the experts. */
+__device__ __forceinline__ int od_valid(int k, int E, int *err)
 {
-    if (p >= end) return -1;
-    const int k = idx[p];
-    if (k >= E) {
-        k3d_raise(err, K3G_ERR_EXPERT_RANGE);
-        return -1;
-    }
-    return k < 0 ? -1 : k;
+    if (k < E) return k < 0 ? -1 : k;
+    k3d_raise(err, K3G_ERR_EXPERT_RANGE);
+    return -1;
 }
 
 /* The pairs of each expert in each chunk of m * OD_THREADS pairs. */
@@ -61,9 +58,13 @@ k_order_count(const int32_t *__restrict__ idx, int P, int E, int m, int32_t *__r
     const int first = blockIdx.x * m * OD_THREADS, end = min(P, first + m * OD_THREADS);
     for (int e = threadIdx.x; e < E; e += OD_THREADS) h[e] = 0;
     __syncthreads();
-    for (int p = first + threadIdx.x; p < end; p += OD_THREADS) {
-        const int k = idx[p];
-        if (k >= 0 && k < E) atomicAdd(&h[k], 1);
+    for (int p = first + threadIdx.x; p < end; p += 4 * OD_THREADS) {
+        int k[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) k[i] = p + i * OD_THREADS < end ? idx[p + i * OD_THREADS] : -1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (k[i] >= 0 && k[i] < E) atomicAdd(&h[k[i]], 1);
     }
     __syncthreads();
     for (int e = threadIdx.x; e < E; e += OD_THREADS) cnt[(size_t)blockIdx.x * E + e] = h[e];
@@ -71,45 +72,79 @@ k_order_count(const int32_t *__restrict__ idx, int P, int E, int m, int32_t *__r
 
 /* A chunk's pairs into their places: wave w takes m * 64 consecutive pairs, 64 at a time; a
  * pair's rank is the wave's earlier pairs of its expert (a count in LDS) plus those in lanes
- * before it. Then, per expert, the waves' counts become running sums, the chunks before give
- * where the chunk's first pair of it goes (counts of k_order_count; one chunk needs none), and
- * a block scan of the totals gives where the expert begins. Between the two walks a pair's rank
- * waits in its own entry of pos. */
+ * before it. Then, a thread an expert, the waves' counts become running sums, the chunks before
+ * give where the chunk's first pair of it goes (counts of k_order_count; one chunk needs none),
+ * and a block scan of the totals gives where the expert begins.
+ * M > 0: m = M, and a thread's experts and ranks stay in registers, every load asked for before
+ * the first is used (3,702 pairs in one block 11.4 -> 5.2 us). M = 0: any m; a pair's rank waits in
+ * its own entry of pos between the two walks. */
+template <int M>
 __global__ void __launch_bounds__(OD_THREADS)
-k_order_place(const int32_t *__restrict__ idx, int P, int E, int m,
+k_order_place(const int32_t *__restrict__ idx, int P, int E, int any_m,
               const int32_t *__restrict__ cnt, int nch, int32_t *__restrict__ perm,
               int32_t *__restrict__ off, int32_t *pos, int *err)
 {
     __shared__ int wc[OD_WAVES][OD_MAX_EXPERTS];
     __shared__ int first[OD_MAX_EXPERTS];
-    __shared__ int red[OD_WAVES + 1];
+    __shared__ int red[(OD_WAVES + 1) * 2];
     const int c = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    for (int e = tid; e < OD_WAVES * OD_MAX_EXPERTS; e += OD_THREADS) (&wc[0][0])[e] = 0;
-    __syncthreads();
+    const int m = M ? M : any_m;
     const int p0 = (c * OD_WAVES + w) * m * 64, end = min(P, p0 + m * 64);
-    const int nb = 32 - __clz(E > 1 ? E - 1 : 1);
-    const uint64_t lt = (1ull << lane) - 1;
-    for (int p = p0 + lane; p - lane < end; p += 64) {
-        const int key = od_key(idx, p, end, E, err);
-        const uint64_t peers = od_peers(key, nb);
-        const int r = __popcll(peers & lt);
-        /* atomics: a wave's lanes read what its other lanes wrote a step before */
-        const int before = key >= 0 ? __hip_atomic_load(&wc[w][key], __ATOMIC_RELAXED,
-                                                        __HIP_MEMORY_SCOPE_WAVEFRONT) : 0;
-        __builtin_amdgcn_wave_barrier();
-        if (key >= 0 && r == 0)
-            __hip_atomic_store(&wc[w][key], before + __popcll(peers), __ATOMIC_RELAXED,
-                               __HIP_MEMORY_SCOPE_WAVEFRONT);
-        __builtin_amdgcn_wave_barrier();
-        if (p < end) pos[p] = key >= 0 ? before + r : -1;
+    int key[M ? M : 1], rank[M ? M : 1];
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+        const int p = p0 + 64 * i + lane;
+        key[i] = p < end ? idx[p] : -1;
     }
-    __syncthreads();
     constexpr int EPT = OD_MAX_EXPERTS / OD_THREADS;
-    int tot[EPT], prev[EPT], run = 0;
+    int tot[EPT], prev[EPT];
 #pragma unroll
     for (int u = 0; u < EPT; ++u) {
-        const int e = EPT * tid + u;
+        const int e = tid + OD_THREADS * u;
         tot[u] = prev[u] = 0;
+        if (e >= E) continue;
+#pragma unroll
+        for (int q = 0; q < OD_WAVES; ++q) wc[q][e] = 0;
+        if (nch == 1) continue;
+#pragma unroll 16
+        for (int q = 0; q < nch; ++q) {
+            const int v = cnt[(size_t)q * E + e];
+            if (q < c) prev[u] += v;
+            tot[u] += v;
+        }
+    }
+    __syncthreads();
+    const int nb = 32 - __clz(E > 1 ? E - 1 : 1);
+    const uint64_t lt = (1ull << lane) - 1;
+    /* rank among the wave's pairs so far; atomics: lanes read what others wrote a step before */
+    auto place = [&](int k) {
+        const uint64_t peers = od_peers(k, nb);
+        const int r = __popcll(peers & lt);
+        const int before = k >= 0 ? __hip_atomic_load(&wc[w][k], __ATOMIC_RELAXED,
+                                                      __HIP_MEMORY_SCOPE_WAVEFRONT) : 0;
+        __builtin_amdgcn_wave_barrier();
+        if (k >= 0 && r == 0)
+            __hip_atomic_store(&wc[w][k], before + __popcll(peers), __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_WAVEFRONT);
+        __builtin_amdgcn_wave_barrier();
+        return before + r;
+    };
+    if constexpr (M > 0) {
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            key[i] = od_valid(key[i], E, err);
+            rank[i] = place(key[i]);
+        }
+    } else {
+        for (int p = p0 + lane; p - lane < end; p += 64) {
+            const int k = od_valid(p < end ? idx[p] : -1, E, err), r = place(k);
+            if (p < end) pos[p] = k >= 0 ? r : -1;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < EPT; ++u) {
+        const int e = tid + OD_THREADS * u;
         if (e >= E) continue;
         int s = 0;
 #pragma unroll
@@ -118,38 +153,40 @@ k_order_place(const int32_t *__restrict__ idx, int P, int E, int m,
             wc[q][e] = s;
             s += v;
         }
-        if (nch == 1) {
-            tot[u] = s;
-        } else {
-#pragma unroll 8
-            for (int q = 0; q < nch; ++q) {
-                const int v = cnt[(size_t)q * E + e];
-                if (q < c) prev[u] += v;
-                tot[u] += v;
-            }
-        }
-        run += tot[u];
+        if (nch == 1) tot[u] = s;
     }
-    int v[1] = {run}, all[1];
-    k3d_block_exscan_n<1, OD_WAVES>(v, all, red);
-    int at = v[0];
+    int v[EPT], all[EPT], at = 0;
+#pragma unroll
+    for (int u = 0; u < EPT; ++u) v[u] = tot[u];
+    k3d_block_exscan_n<EPT, OD_WAVES>(v, all, red);
 #pragma unroll
     for (int u = 0; u < EPT; ++u) {
-        const int e = EPT * tid + u;
+        const int e = tid + OD_THREADS * u;
         if (e < E) {
-            first[e] = at + prev[u];
-            if (c == 0) off[e] = at;
+            first[e] = at + v[u] + prev[u];
+            if (c == 0) off[e] = at + v[u];
         }
-        at += tot[u];
+        at += all[u];
     }
-    if (c == 0 && tid == 0) off[E] = all[0];
+    if (c == 0 && tid == 0) off[E] = at;
     __syncthreads();
-    for (int p = p0 + lane; p < end; p += 64) {
-        const int rank = pos[p];
-        if (rank < 0) continue;
-        const int e = idx[p], place = first[e] + wc[w][e] + rank;
-        perm[place] = p;
-        pos[p] = place;
+    if constexpr (M > 0) {
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            const int p = p0 + 64 * i + lane;
+            if (p >= end) continue;
+            const int at = key[i] >= 0 ? first[key[i]] + wc[w][key[i]] + rank[i] : -1;
+            if (at >= 0) perm[at] = p;
+            pos[p] = at;
+        }
+    } else {
+        for (int p = p0 + lane; p < end; p += 64) {
+            const int r = pos[p];
+            if (r < 0) continue;
+            const int e = idx[p], at = first[e] + wc[w][e] + r;
+            perm[at] = p;
+            pos[p] = at;
+        }
     }
 }
 
@@ -224,81 +261,114 @@ __device__ __forceinline__ void od_store(T *p, int v, int n, const od_v4u &u)
 
 /* --------------------------------------------------------------------- kernels ---- */
 
-/* A block of 256 threads is `ty` tokens of `tx` vectors each (tx a power of two); the grid is
+/* A block of 256 threads is 256 >> tx_log tokens of 1 << tx_log vectors each; the grid is
  * (tokens, vectors). */
 struct OdGrid {
     int T, k, n, P, tx_log;
 };
 
-template <typename T>
+/* This thread's token and vector; false past the last. WIDE: a wave has one token, which is then
+ * known to be the same in every lane (its places and weights come by scalar loads). */
+template <typename T, bool WIDE>
+__device__ __forceinline__ bool od_mine(const OdGrid &g, int &t, int &v)
+{
+    t = blockIdx.x * (256 >> g.tx_log) + (threadIdx.x >> g.tx_log);
+    if (WIDE) t = __builtin_amdgcn_readfirstlane(t);
+    v = (blockIdx.y << g.tx_log) + (threadIdx.x & ((1 << g.tx_log) - 1));
+    return t < g.T && OdRow<T>::V * v < g.n;
+}
+
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256)
 k_permute(const OdGrid g, const T *__restrict__ x, const int32_t *__restrict__ pos,
           T *__restrict__ sorted)
 {
-    const int t = blockIdx.x * (256 >> g.tx_log) + (threadIdx.x >> g.tx_log);
-    const int v = (blockIdx.y << g.tx_log) + (threadIdx.x & ((1 << g.tx_log) - 1));
-    if (t >= g.T || OdRow<T>::V * v >= g.n) return;
+    int t, v;
+    if (!od_mine<T, WIDE>(g, t, v)) return;
     const od_v4u u = od_load(x + (size_t)t * g.n, v, g.n);
+    const int32_t *pt = pos + (size_t)t * g.k;
+#pragma unroll 4
     for (int j = 0; j < g.k; ++j) {
-        const int p = pos[(size_t)t * g.k + j];
+        const int p = pt[j];
         if ((unsigned)p < (unsigned)g.P) od_store(sorted + (size_t)p * g.n, v, g.n, u);
     }
 }
 
 /* out[t] = sum_j w_j row_j, products and sums rounded separately in slot order as the layer's
- * combine does, then + add[t]; without weights the gradient of k_permute. */
-template <typename T>
+ * combine does, then + add[t]; without weights the gradient of k_permute. Eight rows are asked
+ * for before the first is added (one after the other the 16 rows of a decoding token took 6.2 us). */
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256)
 k_unpermute(const OdGrid g, const T *__restrict__ sorted, const int32_t *__restrict__ pos,
             const float *__restrict__ wt, const T *__restrict__ add, T *__restrict__ out)
 {
-    constexpr int V = OdRow<T>::V;
-    const int t = blockIdx.x * (256 >> g.tx_log) + (threadIdx.x >> g.tx_log);
-    const int v = (blockIdx.y << g.tx_log) + (threadIdx.x & ((1 << g.tx_log) - 1));
-    if (t >= g.T || V * v >= g.n) return;
+    constexpr int V = OdRow<T>::V, AHEAD = 8;
+    int t, v;
+    if (!od_mine<T, WIDE>(g, t, v)) return;
+    const int32_t *pt = pos + (size_t)t * g.k;
+    const float *wrow = wt + (size_t)t * g.k;
     float acc[V], f[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.0f;
-    for (int j = 0; j < g.k; ++j) {
-        const int p = pos[(size_t)t * g.k + j];
-        if ((unsigned)p >= (unsigned)g.P) continue;
-        OdRow<T>::get(od_load(sorted + (size_t)p * g.n, v, g.n), f);
-        const float w = wt ? wt[(size_t)t * g.k + j] : 1.0f;
+    od_v4u extra = {0, 0, 0, 0};
+    if (add) extra = od_load(add + (size_t)t * g.n, v, g.n);
+    for (int j0 = 0; j0 < g.k; j0 += AHEAD) {
+        int p[AHEAD];
+        float w[AHEAD];
+        od_v4u u[AHEAD];
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] += wt ? w * f[i] : f[i];
+        for (int i = 0; i < AHEAD; ++i) {
+            p[i] = j0 + i < g.k ? pt[j0 + i] : -1;
+            w[i] = wt && j0 + i < g.k ? wrow[j0 + i] : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if ((unsigned)p[i] < (unsigned)g.P) u[i] = od_load(sorted + (size_t)p[i] * g.n, v, g.n);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if ((unsigned)p[i] >= (unsigned)g.P) continue;
+            OdRow<T>::get(u[i], f);
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[e] += wt ? w[i] * f[e] : f[e];
+        }
     }
     if (add) {
-        OdRow<T>::get(od_load(add + (size_t)t * g.n, v, g.n), f);
+        OdRow<T>::get(extra, f);
 #pragma unroll
         for (int i = 0; i < V; ++i) acc[i] += f[i];
     }
     od_store(out + (size_t)t * g.n, v, g.n, OdRow<T>::put(acc));
 }
 
-/* One block per pair: its row of dsorted and its entry of dwt. */
-template <typename T>
+/* WV waves per pair (a block of four): its row of dsorted and its entry of dwt, the pairs of a
+ * token on one XCD (block b runs on XCD b % 8), whose L2 then serves the token's dout. */
+template <typename T, int WV>
 __global__ void __launch_bounds__(256)
 k_unpermute_grad(const OdGrid g, const T *__restrict__ dout, const T *__restrict__ sorted,
                  const int32_t *__restrict__ pos, const float *__restrict__ wt,
                  T *__restrict__ dsorted, float *__restrict__ dwt)
 {
-    constexpr int V = OdRow<T>::V;
+    constexpr int V = OdRow<T>::V, PER = 4 / WV;
     __shared__ float part[4];
-    const size_t pair = (size_t)blockIdx.x;
-    const int t = (int)(pair / g.k), p = pos[pair];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & (64 * WV - 1);
+    const int xcd = blockIdx.x & 7, s = (blockIdx.x >> 3) * PER + wave / WV;
+    const int t = 8 * (s / g.k) + xcd, j = s % g.k;
+    if (t >= g.T) return;
+    const size_t pair = (size_t)t * g.k + j;
+    const int p = pos[pair];
     if ((unsigned)p >= (unsigned)g.P) {
-        if (dwt && threadIdx.x == 0) dwt[pair] = 0.0f;
+        if (dwt && lane == 0) dwt[pair] = 0.0f;
         return;
     }
     const float w = dsorted ? wt[pair] : 0.0f;
-    float s = 0.0f;
-    for (int v = threadIdx.x; V * v < g.n; v += 256) {
+    float sum = 0.0f;
+    for (int v = lane; V * v < g.n; v += 64 * WV) {
         float go[V], f[V];
         OdRow<T>::get(od_load(dout + (size_t)t * g.n, v, g.n), go);
         if (dwt) {
             OdRow<T>::get(od_load(sorted + (size_t)p * g.n, v, g.n), f);
 #pragma unroll
-            for (int i = 0; i < V; ++i) s += f[i] * go[i];
+            for (int i = 0; i < V; ++i) sum += f[i] * go[i];
         }
         if (dsorted) {
 #pragma unroll
@@ -307,22 +377,28 @@ k_unpermute_grad(const OdGrid g, const T *__restrict__ dout, const T *__restrict
         }
     }
     if (!dwt) return;
-    s = k3d_wave_sum(s);
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+    sum = k3d_wave_sum(sum);
+    if (WV == 1) {
+        if (lane == 0) dwt[pair] = sum;
+        return;
+    }
+    if ((threadIdx.x & 63) == 0) part[wave] = sum;
     __syncthreads();
     if (threadIdx.x == 0) dwt[pair] = part[0] + part[1] + part[2] + part[3];
 }
 
 /* ------------------------------------------------------------------ entry points ---- */
 
+/* Chunks of the sort and the multiple m of OD_THREADS pairs that each has. Up to 4096 pairs one
+ * block does all; past that a chunk is 2048 or 4096 pairs, or what makes 128 chunks: every chunk
+ * reads the counts of all (32,768 pairs in 64 chunks took 9.4 us, in 16 4.4). */
 static int sort_chunks(int P, int *m)
 {
-    int per = 1;
+    int per = P <= OD_THREADS ? 1 : P <= 2 * OD_THREADS ? 2 : P <= 4 * OD_THREADS ? 4 : 8;
     if (P > 8 * OD_THREADS) {
-        per = (P + OD_CHUNKS * OD_THREADS - 1) / (OD_CHUNKS * OD_THREADS);
-    } else {
-        per = (P + OD_THREADS - 1) / OD_THREADS;
-        if (per < 1) per = 1;
+        if (P <= 32 * 4 * OD_THREADS) per = 4;
+        else if (P > OD_CHUNKS * 8 * OD_THREADS)
+            per = (P + OD_CHUNKS * OD_THREADS - 1) / (OD_CHUNKS * OD_THREADS);
     }
     *m = per;
     return P ? (P + per * OD_THREADS - 1) / (per * OD_THREADS) : 1;
@@ -380,7 +456,9 @@ extern "C" int k3g_sort_tokens(const int32_t *idx, int T, int topk, int n_expert
     if (nch > 1 && k3h_launch(who, k_order_count, dim3(nch), dim3(OD_THREADS), on.st, idx, P, n_experts, m,
                               cnt))
         return -1;
-    return k3h_launch(who, k_order_place, dim3(nch), dim3(OD_THREADS), on.st, idx, P, n_experts, m,
+    auto *place = m == 1 ? k_order_place<1> : m == 2 ? k_order_place<2> : m == 4 ? k_order_place<4>
+                : m == 8 ? k_order_place<8> : k_order_place<0>;
+    return k3h_launch(who, place, dim3(nch), dim3(OD_THREADS), on.st, idx, P, n_experts, m,
                       (const int32_t *)cnt, nch, perm, off, pos, err);
 }
 
@@ -440,9 +518,9 @@ extern "C" int k3g_permute(const void *x, int dt, int T, int topk, int n, const 
     OdGrid g = {T, topk, n, T * topk, 0};
     const dim3 grid = row_grid(g, 16 / size);
     if (dt == K3_WBF16)
-        return k3h_launch(who, k_permute<uint16_t>, grid, dim3(256), on.st, (const OdGrid)g,
+        return k3h_launch(who, g.tx_log >= 6 ? k_permute<uint16_t, true> : k_permute<uint16_t, false>, grid, dim3(256), on.st, (const OdGrid)g,
                           (const uint16_t *)x, pos, (uint16_t *)sorted);
-    return k3h_launch(who, k_permute<float>, grid, dim3(256), on.st, (const OdGrid)g, (const float *)x,
+    return k3h_launch(who, g.tx_log >= 6 ? k_permute<float, true> : k_permute<float, false>, grid, dim3(256), on.st, (const OdGrid)g, (const float *)x,
                       pos, (float *)sorted);
 }
 
@@ -461,9 +539,9 @@ static int unpermute(const char *who, const void *sorted, int dt, int T, int top
     OdGrid g = {T, topk, n, T * topk, 0};
     const dim3 grid = row_grid(g, 16 / size);
     if (dt == K3_WBF16)
-        return k3h_launch(who, k_unpermute<uint16_t>, grid, dim3(256), on.st, (const OdGrid)g,
+        return k3h_launch(who, g.tx_log >= 6 ? k_unpermute<uint16_t, true> : k_unpermute<uint16_t, false>, grid, dim3(256), on.st, (const OdGrid)g,
                           (const uint16_t *)sorted, pos, wt, (const uint16_t *)add, (uint16_t *)out);
-    return k3h_launch(who, k_unpermute<float>, grid, dim3(256), on.st, (const OdGrid)g,
+    return k3h_launch(who, g.tx_log >= 6 ? k_unpermute<float, true> : k_unpermute<float, false>, grid, dim3(256), on.st, (const OdGrid)g,
                       (const float *)sorted, pos, wt, (const float *)add, (float *)out);
 }
 
@@ -503,10 +581,14 @@ extern "C" int k3g_unpermute_grad(const void *dout, const void *sorted, int dt, 
     K3hOn on(stream);
     if (!on.ok) return -1;
     const OdGrid g = {T, topk, n, T * topk, 0};
+    /* short rows: a wave each */
+    const bool wave = n <= 128 * (16 / size);
+    const int64_t slots = (int64_t)((T + 7) / 8) * topk;
+    const dim3 grid((unsigned)(8 * (wave ? (slots + 3) / 4 : slots)));
     if (dt == K3_WBF16)
-        return k3h_launch(who, k_unpermute_grad<uint16_t>, dim3(g.P), dim3(256), on.st, g,
-                          (const uint16_t *)dout, (const uint16_t *)sorted, pos, wt, (uint16_t *)dsorted,
-                          dwt);
-    return k3h_launch(who, k_unpermute_grad<float>, dim3(g.P), dim3(256), on.st, g, (const float *)dout,
-                      (const float *)sorted, pos, wt, (float *)dsorted, dwt);
+        return k3h_launch(who, wave ? k_unpermute_grad<uint16_t, 1> : k_unpermute_grad<uint16_t, 4>, grid,
+                          dim3(256), on.st, g, (const uint16_t *)dout, (const uint16_t *)sorted, pos, wt,
+                          (uint16_t *)dsorted, dwt);
+    return k3h_launch(who, wave ? k_unpermute_grad<float, 1> : k_unpermute_grad<float, 4>, grid, dim3(256),
+                      on.st, g, (const float *)dout, (const float *)sorted, pos, wt, (float *)dsorted, dwt);
 }
