@@ -502,7 +502,7 @@ int  k3g_moe_noalloc(const K3gLayer *L, const float *x, int T, float *out, int32
  * (NULL = the null stream), launched on the stream's device, where every pointer must be
  * readable. Rows are fp32 (K3_WF32) or bf16 (K3_WBF16), tagged by dt, contiguous, of any width
  * n from 1 to 2^24, at any address their elements may have; sums are fp32 in a fixed order and
- * rounded once, to nearest even. 1 <= topk <= 64, T topk <= 2^26 pairs; T = 0 is a call without
+ * rounded once, to nearest even. 1 <= topk <= 64, T topk <= 2^23 pairs; T = 0 is a call without
  * rows. Outputs must not overlap inputs. Each returns 0, or -1 with a message for arguments it
  * does not take (nothing is launched then).
  *
@@ -561,7 +561,8 @@ int  k3g_dequant_mxfp4(const void *packed, const void *scales, int rows, int col
                        int dt, void *stream);
 
 /* Bytes of device memory the products below work in for `rows` rows of x (the quantised rows;
- * 0 for sizes they do not take). Calls that may overlap need one each. */
+ * 0 for sizes they do not take: (rows + 1) * ceil(cols / 512) is below 2^26). Calls that may
+ * overlap need one each. */
 size_t k3g_mxfp4_work_bytes(int rows, int cols);
 /* y [rows][n] = q(x) W^T: x [rows][cols] (xdt) quantised as k3g_quant_mxfp4 does, w the n x cols
  * matrix in the tiled layout of k3g_tile_mxfp4 (n a multiple of 16 up to 2^20), sums in fp32,
@@ -577,7 +578,7 @@ int  k3g_matmul_mxfp4(const void *x, int xdt, int rows, int cols, const void *w,
  * sizeof(K3ExpertQ) for &experts[0].p1 of a layer's table). With w3 (NULL for none) each expert
  * has a second such matrix and y[r] = act(q(x) W_e^T, q(x) W3_e^T), the layer's activation with
  * caps b1, b2 (2^64 and above: uncapped, SwiGLU). An expert that has pairs but a NULL matrix
- * gives rows of zeros. rows * topk <= 2^26. */
+ * gives rows of zeros. rows * topk <= 2^23. */
 int  k3g_grouped_mxfp4(const void *x, int xdt, int rows, int cols, const int32_t *perm,
                        int topk, const int32_t *off, int n_experts, const void *const *w,
                        const void *const *w3, int w_step, int n, float b1, float b2, void *y,

@@ -25,27 +25,50 @@
 #define MX_XQ 272                    /* an activation quad: 1 row x 512 columns */
 #define MX_MAX_ROWS (1 << 26)
 #define MX_MAX_COLS (1 << 20)
+#define MX_MAX_PAIRS (1 << 23)
+#define MX_MAX_QUADS (1 << 26)       /* activation quads of a call: k_mx_x has 64 threads each */
+#define MX_MAX_BLOCKS (1 << 23)      /* a launch has fewer than 2^32 threads */
 
 typedef int mx_v8i __attribute__((ext_vector_type(8)));
 
 /* ------------------------------------------------------------- quantisation ---- */
 
-/* 8 consecutive values of a row */
+/* 8 consecutive values of a row. STREAM: not to be kept in the caches, for values that are more than
+ * the 256 MB of the last-level cache holds (MX_STREAM; 32768 x 7168 bf16 values there and back 221 ->
+ * 178 us). */
+#define MX_STREAM ((size_t)256 << 20)
+
 struct Mx8 {
     float f[8];
 };
 
-__device__ __forceinline__ Mx8 mx_load8(const float *p)
+template <bool STREAM>
+__device__ __forceinline__ gm_v4u mx_get(const void *p)
 {
-    const float4 a = *(const float4 *)p, b = *(const float4 *)(p + 4);
-    return {{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+    return STREAM ? __builtin_nontemporal_load((const gm_v4u *)p) : *(const gm_v4u *)p;
 }
 
+template <bool STREAM>
+__device__ __forceinline__ void mx_set(void *p, const gm_v4u &v)
+{
+    if (STREAM) __builtin_nontemporal_store(v, (gm_v4u *)p);
+    else *(gm_v4u *)p = v;
+}
+
+template <bool STREAM = false>
+__device__ __forceinline__ Mx8 mx_load8(const float *p)
+{
+    const gm_v4u a = mx_get<STREAM>(p), b = mx_get<STREAM>(p + 4);
+    return {{__uint_as_float(a[0]), __uint_as_float(a[1]), __uint_as_float(a[2]), __uint_as_float(a[3]),
+             __uint_as_float(b[0]), __uint_as_float(b[1]), __uint_as_float(b[2]), __uint_as_float(b[3])}};
+}
+
+template <bool STREAM = false>
 __device__ __forceinline__ Mx8 mx_load8(const uint16_t *p)
 {
-    const uint4 a = *(const uint4 *)p;
-    return {{k3d_bf16lo(a.x), k3d_bf16hi(a.x), k3d_bf16lo(a.y), k3d_bf16hi(a.y), k3d_bf16lo(a.z),
-             k3d_bf16hi(a.z), k3d_bf16lo(a.w), k3d_bf16hi(a.w)}};
+    const gm_v4u a = mx_get<STREAM>(p);
+    return {{k3d_bf16lo(a[0]), k3d_bf16hi(a[0]), k3d_bf16lo(a[1]), k3d_bf16hi(a[1]), k3d_bf16lo(a[2]),
+             k3d_bf16hi(a[2]), k3d_bf16lo(a[3]), k3d_bf16hi(a[3])}};
 }
 
 /* The largest of a value over the four lanes of a quad of lanes */
@@ -81,44 +104,48 @@ __device__ __forceinline__ uint32_t mx_quant8(const Mx8 &x, uint32_t &scale)
 
 /* Four lanes per block, 8 values a lane: loads of 16 bytes a lane and stores of 4, each row of
  * whole blocks. */
-template <typename T>
+template <typename T, bool STREAM>
 __global__ void __launch_bounds__(256)
 k_mx_quant(const T *__restrict__ x, size_t n8, uint8_t *__restrict__ packed,
            uint8_t *__restrict__ scales)
 {
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n8) return;
-    uint32_t s;
-    *(uint32_t *)(packed + 4 * i) = mx_quant8(mx_load8(x + 8 * i), s);
-    if ((i & 3) == 0) scales[i >> 2] = (uint8_t)s;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n8; i += (size_t)gridDim.x * 256) {
+        uint32_t s;
+        *(uint32_t *)(packed + 4 * i) = mx_quant8(mx_load8<STREAM>(x + 8 * i), s);
+        if ((i & 3) == 0) scales[i >> 2] = (uint8_t)s;
+    }
 }
 
+template <bool STREAM>
 __device__ __forceinline__ void mx_store8(float *p, const float *f)
 {
-    *(float4 *)p = make_float4(f[0], f[1], f[2], f[3]);
-    *(float4 *)(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
+    mx_set<STREAM>(p, gm_v4u{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                             __float_as_uint(f[3])});
+    mx_set<STREAM>(p + 4, gm_v4u{__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]),
+                                 __float_as_uint(f[7])});
 }
 
+template <bool STREAM>
 __device__ __forceinline__ void mx_store8(uint16_t *p, const float *f)
 {
-    *(uint4 *)p = make_uint4(k3d_bf16x2(f[0], f[1]), k3d_bf16x2(f[2], f[3]), k3d_bf16x2(f[4], f[5]),
-                             k3d_bf16x2(f[6], f[7]));
+    mx_set<STREAM>(p, gm_v4u{k3d_bf16x2(f[0], f[1]), k3d_bf16x2(f[2], f[3]), k3d_bf16x2(f[4], f[5]),
+                             k3d_bf16x2(f[6], f[7])});
 }
 
-template <typename T>
+template <typename T, bool STREAM>
 __global__ void __launch_bounds__(256)
 k_mx_dequant(const uint8_t *__restrict__ packed, const uint8_t *__restrict__ scales, size_t n8,
              T *__restrict__ out)
 {
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n8) return;
-    const uint32_t b = scales[i >> 2];
-    const float s = b == 255u ? __builtin_nanf("") : k3d_e8m0(b);
-    float f[8];
-    k3d_fp4x8(*(const uint32_t *)(packed + 4 * i), 1.0f, f);
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n8; i += (size_t)gridDim.x * 256) {
+        const uint32_t b = scales[i >> 2];
+        const float s = b == 255u ? __builtin_nanf("") : k3d_e8m0(b);
+        float f[8];
+        k3d_fp4x8(*(const uint32_t *)(packed + 4 * i), 1.0f, f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] *= s;
-    mx_store8(out + 8 * i, f);
+        for (int j = 0; j < 8; ++j) f[j] *= s;
+        mx_store8<STREAM>(out + 8 * i, f);
+    }
 }
 
 /* x as activation quads (see the top), a wave per quad, and a row of zeros behind them */
@@ -658,11 +685,12 @@ extern "C" int k3g_quant_mxfp4(const void *x, int dt, int rows, int cols, void *
     K3hOn on(stream);
     if (!on.ok) return -1;
     const size_t n8 = (size_t)rows * cols / 8;
-    const dim3 grid((unsigned)((n8 + 255) / 256));
+    const dim3 grid((unsigned)min((n8 + 255) / 256, (size_t)MX_MAX_BLOCKS));
+    const bool big = n8 * (dt == K3_WBF16 ? 16 : 32) > MX_STREAM;
     if (dt == K3_WBF16)
-        return k3h_launch(who, k_mx_quant<uint16_t>, grid, dim3(256), on.st, (const uint16_t *)x, n8,
+        return k3h_launch(who, big ? k_mx_quant<uint16_t, true> : k_mx_quant<uint16_t, false>, grid, dim3(256), on.st, (const uint16_t *)x, n8,
                           (uint8_t *)packed, (uint8_t *)scales);
-    return k3h_launch(who, k_mx_quant<float>, grid, dim3(256), on.st, (const float *)x, n8,
+    return k3h_launch(who, big ? k_mx_quant<float, true> : k_mx_quant<float, false>, grid, dim3(256), on.st, (const float *)x, n8,
                       (uint8_t *)packed, (uint8_t *)scales);
 }
 
@@ -677,21 +705,21 @@ extern "C" int k3g_dequant_mxfp4(const void *packed, const void *scales, int row
     K3hOn on(stream);
     if (!on.ok) return -1;
     const size_t n8 = (size_t)rows * cols / 8;
-    const dim3 grid((unsigned)((n8 + 255) / 256));
+    const dim3 grid((unsigned)min((n8 + 255) / 256, (size_t)MX_MAX_BLOCKS));
+    const bool big = n8 * (dt == K3_WBF16 ? 16 : 32) > MX_STREAM;
     if (dt == K3_WBF16)
-        return k3h_launch(who, k_mx_dequant<uint16_t>, grid, dim3(256), on.st, (const uint8_t *)packed,
+        return k3h_launch(who, big ? k_mx_dequant<uint16_t, true> : k_mx_dequant<uint16_t, false>, grid, dim3(256), on.st, (const uint8_t *)packed,
                           (const uint8_t *)scales, n8, (uint16_t *)out);
-    return k3h_launch(who, k_mx_dequant<float>, grid, dim3(256), on.st, (const uint8_t *)packed,
+    return k3h_launch(who, big ? k_mx_dequant<float, true> : k_mx_dequant<float, false>, grid, dim3(256), on.st, (const uint8_t *)packed,
                       (const uint8_t *)scales, n8, (float *)out);
 }
 
 extern "C" size_t k3g_mxfp4_work_bytes(int rows, int cols)
 {
     if (!mx_shape_ok(rows, cols) || !rows) return 0;
-    /* and a row of zeros behind them, for places without one; the kernels count it in 32 bits of
-     * 16 bytes each */
-    const size_t n = ((size_t)rows + 1) * ((cols + 511) / 512) * MX_XQ;
-    return n >> 36 ? 0 : n;
+    /* and a row of zeros behind them, for places without one */
+    const size_t quads = ((size_t)rows + 1) * ((cols + 511) / 512);
+    return quads < MX_MAX_QUADS ? quads * MX_XQ : 0;
 }
 
 /* Which kernel a product runs on: rows of a tile, its row blocks (of each matrix), the waves that
@@ -699,6 +727,7 @@ extern "C" size_t k3g_mxfp4_work_bytes(int rows, int cols)
 struct MxPlan {
     int tm, rb, wv;
     bool values;
+    unsigned blocks;
 };
 
 /* workgroups of tiles of tm rows by rb row blocks, as many as mx_item may be asked for */
@@ -727,64 +756,62 @@ static MxPlan mx_plan(const MxProduct &g, bool gated)
 {
     const int RB = gated ? 2 : 4;
     if (!g.off) {
-        if (g.P <= 4) return {16, 1, 8, true};
-        if (mx_grid(g, 128, 16) >= 160) return {128, 16, 0, false};
-        if (mx_grid(g, 64, 16) >= 96) return {64, 16, 0, false};
-        if (mx_grid(g, 64, 4) >= 192) return {64, 4, 4, false};
-        if (mx_grid(g, 32, 4) >= 192) return {32, 4, 4, false};
-        if (mx_grid(g, 16, 4) >= 192) return {16, 4, 4, false};
-        if (mx_grid(g, 16, 2) >= 192) return {16, 2, 4, false};
-        return {16, 1, 8, false};
+        if (g.P <= 4) return {16, 1, 8, true, 0};
+        if (mx_grid(g, 128, 16) >= 160) return {128, 16, 0, false, 0};
+        if (mx_grid(g, 64, 16) >= 96) return {64, 16, 0, false, 0};
+        if (mx_grid(g, 64, 4) >= 192) return {64, 4, 4, false, 0};
+        if (mx_grid(g, 32, 4) >= 192) return {32, 4, 4, false, 0};
+        if (mx_grid(g, 16, 4) >= 192) return {16, 4, 4, false, 0};
+        if (mx_grid(g, 16, 2) >= 192) return {16, 2, 4, false, 0};
+        return {16, 1, 8, false, 0};
     }
     const int met = min(g.E, g.P), mean = (g.P + met - 1) / met;
-    if (g.T <= 16 && mean <= 2) return {16, RB, 4, true};
+    if (g.T <= 16 && mean <= 2) return {16, RB, 4, true, 0};
     /* row tiles there will be, about: one an expert or more */
     const int64_t nft = (g.N / 16 + 4 * RB - 1) / (4 * RB);
-    if (mean > 48 && max(met, g.P / 128) * nft >= 256) return {128, 4 * RB, 0, false};
-    if (max(met, g.P / 64) * nft >= 256) return {64, 4 * RB, 0, false};
-    return {mean > 16 ? 32 : 16, RB, 4, false};
+    if (mean > 48 && max(met, g.P / 128) * nft >= 256) return {128, 4 * RB, 0, false, 0};
+    if (max(met, g.P / 64) * nft >= 256) return {64, 4 * RB, 0, false, 0};
+    return {mean > 16 ? 32 : 16, RB, 4, false, 0};
 }
 
 template <typename X, typename Y, bool GATED, int WV, int U, int NB>
-static int mx_run_few(const char *who, const MxProduct &g, hipStream_t st)
+static int mx_run_few(const char *who, const MxProduct &g, const MxPlan &p, hipStream_t st)
 {
-    const dim3 grid((unsigned)mx_grid(g, 16 * NB, GATED ? U / 2 : U));
-    return k3h_launch(who, k_mx_few<X, Y, GATED, WV, U, NB>, grid, dim3(64 * WV), st, (MxProduct)g);
+    return k3h_launch(who, k_mx_few<X, Y, GATED, WV, U, NB>, dim3(p.blocks), dim3(64 * WV), st, (MxProduct)g);
 }
 
 template <typename Y, bool GATED, int TM>
-static int mx_run_gemm(const char *who, const MxProduct &g, hipStream_t st)
+static int mx_run_gemm(const char *who, const MxProduct &g, const MxPlan &p, hipStream_t st)
 {
-    const dim3 grid((unsigned)mx_grid(g, TM, GATED ? 8 : 16));
-    return k3h_launch(who, k_mx_gemm<Y, GATED, TM>, grid, dim3(256), st, (MxProduct)g);
+    return k3h_launch(who, k_mx_gemm<Y, GATED, TM>, dim3(p.blocks), dim3(256), st, (MxProduct)g);
 }
 
 template <typename X>
 static int mx_launch_values(const char *who, const MxProduct &g, const MxPlan &p, bool bf, bool gated,
                             hipStream_t st)
 {
-    if (gated) return bf ? mx_run_few<X, uint16_t, true, 4, 4, 1>(who, g, st)
-                         : mx_run_few<X, float, true, 4, 4, 1>(who, g, st);
-    if (p.wv == 8) return bf ? mx_run_few<X, uint16_t, false, 8, 1, 1>(who, g, st)
-                             : mx_run_few<X, float, false, 8, 1, 1>(who, g, st);
-    return bf ? mx_run_few<X, uint16_t, false, 4, 4, 1>(who, g, st)
-              : mx_run_few<X, float, false, 4, 4, 1>(who, g, st);
+    if (gated) return bf ? mx_run_few<X, uint16_t, true, 4, 4, 1>(who, g, p, st)
+                         : mx_run_few<X, float, true, 4, 4, 1>(who, g, p, st);
+    if (p.wv == 8) return bf ? mx_run_few<X, uint16_t, false, 8, 1, 1>(who, g, p, st)
+                             : mx_run_few<X, float, false, 8, 1, 1>(who, g, p, st);
+    return bf ? mx_run_few<X, uint16_t, false, 4, 4, 1>(who, g, p, st)
+              : mx_run_few<X, float, false, 4, 4, 1>(who, g, p, st);
 }
 
 template <typename Y>
 static int mx_launch(const char *who, const MxProduct &g, const MxPlan &p, bool gated, hipStream_t st)
 {
     if (!p.wv) {
-        if (gated) return p.tm == 128 ? mx_run_gemm<Y, true, 128>(who, g, st) : mx_run_gemm<Y, true, 64>(who, g, st);
-        return p.tm == 128 ? mx_run_gemm<Y, false, 128>(who, g, st) : mx_run_gemm<Y, false, 64>(who, g, st);
+        if (gated) return p.tm == 128 ? mx_run_gemm<Y, true, 128>(who, g, p, st) : mx_run_gemm<Y, true, 64>(who, g, p, st);
+        return p.tm == 128 ? mx_run_gemm<Y, false, 128>(who, g, p, st) : mx_run_gemm<Y, false, 64>(who, g, p, st);
     }
-    if (gated) return p.tm == 32 ? mx_run_few<MxQuads, Y, true, 4, 4, 2>(who, g, st)
-                                 : mx_run_few<MxQuads, Y, true, 4, 4, 1>(who, g, st);
-    if (p.wv == 8) return mx_run_few<MxQuads, Y, false, 8, 1, 1>(who, g, st);
-    if (p.rb == 2) return mx_run_few<MxQuads, Y, false, 4, 2, 1>(who, g, st);
-    if (p.tm == 64) return mx_run_few<MxQuads, Y, false, 4, 4, 4>(who, g, st);
-    return p.tm == 32 ? mx_run_few<MxQuads, Y, false, 4, 4, 2>(who, g, st)
-                      : mx_run_few<MxQuads, Y, false, 4, 4, 1>(who, g, st);
+    if (gated) return p.tm == 32 ? mx_run_few<MxQuads, Y, true, 4, 4, 2>(who, g, p, st)
+                                 : mx_run_few<MxQuads, Y, true, 4, 4, 1>(who, g, p, st);
+    if (p.wv == 8) return mx_run_few<MxQuads, Y, false, 8, 1, 1>(who, g, p, st);
+    if (p.rb == 2) return mx_run_few<MxQuads, Y, false, 4, 2, 1>(who, g, p, st);
+    if (p.tm == 64) return mx_run_few<MxQuads, Y, false, 4, 4, 4>(who, g, p, st);
+    return p.tm == 32 ? mx_run_few<MxQuads, Y, false, 4, 4, 2>(who, g, p, st)
+                      : mx_run_few<MxQuads, Y, false, 4, 4, 1>(who, g, p, st);
 }
 
 /* the product of checked arguments */
@@ -793,7 +820,8 @@ static int mx_product(const char *who, MxProduct &g, const void *x, int xdt, int
 {
     const size_t need = k3g_mxfp4_work_bytes(g.T, cols);
     if (!need) {
-        fprintf(stderr, "%s: %d x %d activations do not fit 64 GiB in MXFP4\n", who, g.T, cols);
+        fprintf(stderr, "%s: %d x %d activations are more than %d blocks of 512\n", who, g.T, cols,
+                MX_MAX_QUADS);
         return -1;
     }
     if (!work || k3h_misaligned(work, 16) || work_bytes < need) {
@@ -809,7 +837,13 @@ static int mx_product(const char *who, MxProduct &g, const void *x, int xdt, int
     g.x = x;
     g.cols = cols;
     const bool bf = ydt == K3_WBF16, gated = g.w3 != nullptr;
-    const MxPlan plan = mx_plan(g, gated);
+    MxPlan plan = mx_plan(g, gated);
+    const int64_t blocks = mx_grid(g, plan.tm, plan.rb);
+    if (blocks * 512 > UINT32_MAX) {
+        fprintf(stderr, "%s: %d places by %d features are more than a launch takes\n", who, g.P, g.N);
+        return -1;
+    }
+    plan.blocks = (unsigned)blocks;
     if (plan.values)
         return xdt == K3_WBF16 ? mx_launch_values<uint16_t>(who, g, plan, bf, gated, on.st)
                                : mx_launch_values<float>(who, g, plan, bf, gated, on.st);
@@ -860,9 +894,9 @@ extern "C" int k3g_grouped_mxfp4(const void *x, int xdt, int rows, int cols, con
         mx_pointer(who, "w", w, 8, rows > 0) || mx_pointer(who, "w3", w3, 8, false))
         return -1;
     if (n_experts < 1 || n_experts > 1024 || topk < 1 || topk > K3G_MAX_TOPK || (!perm && topk != 1) ||
-        (int64_t)rows * topk > MX_MAX_ROWS) {
+        (int64_t)rows * topk > MX_MAX_PAIRS) {
         fprintf(stderr, "%s: needs 1 to 1024 experts, 1 <= topk <= %d (1 without perm) and at most %d "
-                        "pairs (%d experts, %d x %d)\n", who, K3G_MAX_TOPK, MX_MAX_ROWS, n_experts, rows,
+                        "pairs (%d experts, %d x %d)\n", who, K3G_MAX_TOPK, MX_MAX_PAIRS, n_experts, rows,
                 topk);
         return -1;
     }

@@ -20,7 +20,7 @@
 #include "k3g_kernels.h"
 
 #define OD_MAX_EXPERTS 1024
-#define OD_MAX_PAIRS (1 << 26)
+#define OD_MAX_PAIRS (1 << 23)         /* a block of 256 threads each makes fewer than 2^32 */
 #define OD_MAX_WIDTH (1 << 24)
 #define OD_THREADS 512                 /* threads of a sort block */
 #define OD_WAVES (OD_THREADS / 64)
@@ -230,12 +230,21 @@ template <> struct OdRow<uint16_t> {
 };
 
 /* Vector v of the n-element row at p: whole ones in one load or store, the last one's elements
- * one by one when n ends inside it. */
-template <typename T>
+ * one by one when n ends inside it. STREAM: marked as not to be kept in the caches. The sorted rows
+ * are read or written once in a call; where they are more than the 256 MB of the last-level cache
+ * (OD_STREAM), keeping them only drives other rows out and their write-back meets the next reads
+ * (4,096 x 8 bf16 rows of 7168 there and back 238 -> 217 us, 2,000 x 16 fp32 rows of 3584 back 94
+ * -> 83); fewer may still be there for the caller's next kernel. */
+#define OD_STREAM ((size_t)256 << 20)
+
+template <bool STREAM = false, typename T>
 __device__ __forceinline__ od_v4u od_load(const T *p, int v, int n)
 {
     constexpr int V = OdRow<T>::V;
-    if (V * (v + 1) <= n) return *(const od_v4u *)(p + V * v);
+    if (V * (v + 1) <= n) {
+        const od_v4u *a = (const od_v4u *)(p + V * v);
+        return STREAM ? __builtin_nontemporal_load(a) : *a;
+    }
     T e[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) e[i] = V * v + i < n ? p[V * v + i] : (T)0;
@@ -244,12 +253,14 @@ __device__ __forceinline__ od_v4u od_load(const T *p, int v, int n)
     return u;
 }
 
-template <typename T>
+template <bool STREAM = false, typename T>
 __device__ __forceinline__ void od_store(T *p, int v, int n, const od_v4u &u)
 {
     constexpr int V = OdRow<T>::V;
     if (V * (v + 1) <= n) {
-        *(od_v4u *)(p + V * v) = u;
+        od_v4u *a = (od_v4u *)(p + V * v);
+        if (STREAM) __builtin_nontemporal_store(u, a);
+        else *a = u;
         return;
     }
     T e[V];
@@ -278,7 +289,7 @@ __device__ __forceinline__ bool od_mine(const OdGrid &g, int &t, int &v)
     return t < g.T && OdRow<T>::V * v < g.n;
 }
 
-template <typename T, bool WIDE>
+template <typename T, bool WIDE, bool STREAM>
 __global__ void __launch_bounds__(256)
 k_permute(const OdGrid g, const T *__restrict__ x, const int32_t *__restrict__ pos,
           T *__restrict__ sorted)
@@ -290,14 +301,14 @@ k_permute(const OdGrid g, const T *__restrict__ x, const int32_t *__restrict__ p
 #pragma unroll 4
     for (int j = 0; j < g.k; ++j) {
         const int p = pt[j];
-        if ((unsigned)p < (unsigned)g.P) od_store(sorted + (size_t)p * g.n, v, g.n, u);
+        if ((unsigned)p < (unsigned)g.P) od_store<STREAM>(sorted + (size_t)p * g.n, v, g.n, u);
     }
 }
 
 /* out[t] = sum_j w_j row_j, products and sums rounded separately in slot order as the layer's
  * combine does, then + add[t]; without weights the gradient of k_permute. Eight rows are asked
  * for before the first is added (one after the other the 16 rows of a decoding token took 6.2 us). */
-template <typename T, bool WIDE>
+template <typename T, bool WIDE, bool STREAM>
 __global__ void __launch_bounds__(256)
 k_unpermute(const OdGrid g, const T *__restrict__ sorted, const int32_t *__restrict__ pos,
             const float *__restrict__ wt, const T *__restrict__ add, T *__restrict__ out)
@@ -323,7 +334,7 @@ k_unpermute(const OdGrid g, const T *__restrict__ sorted, const int32_t *__restr
         }
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i)
-            if ((unsigned)p[i] < (unsigned)g.P) u[i] = od_load(sorted + (size_t)p[i] * g.n, v, g.n);
+            if ((unsigned)p[i] < (unsigned)g.P) u[i] = od_load<STREAM>(sorted + (size_t)p[i] * g.n, v, g.n);
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
             if ((unsigned)p[i] >= (unsigned)g.P) continue;
@@ -342,7 +353,7 @@ k_unpermute(const OdGrid g, const T *__restrict__ sorted, const int32_t *__restr
 
 /* WV waves per pair (a block of four): its row of dsorted and its entry of dwt, the pairs of a
  * token on one XCD (block b runs on XCD b % 8), whose L2 then serves the token's dout. */
-template <typename T, int WV>
+template <typename T, int WV, bool STREAM>
 __global__ void __launch_bounds__(256)
 k_unpermute_grad(const OdGrid g, const T *__restrict__ dout, const T *__restrict__ sorted,
                  const int32_t *__restrict__ pos, const float *__restrict__ wt,
@@ -366,14 +377,14 @@ k_unpermute_grad(const OdGrid g, const T *__restrict__ dout, const T *__restrict
         float go[V], f[V];
         OdRow<T>::get(od_load(dout + (size_t)t * g.n, v, g.n), go);
         if (dwt) {
-            OdRow<T>::get(od_load(sorted + (size_t)p * g.n, v, g.n), f);
+            OdRow<T>::get(od_load<STREAM>(sorted + (size_t)p * g.n, v, g.n), f);
 #pragma unroll
             for (int i = 0; i < V; ++i) sum += f[i] * go[i];
         }
         if (dsorted) {
 #pragma unroll
             for (int i = 0; i < V; ++i) f[i] = w * go[i];
-            od_store(dsorted + (size_t)p * g.n, v, g.n, OdRow<T>::put(f));
+            od_store<STREAM>(dsorted + (size_t)p * g.n, v, g.n, OdRow<T>::put(f));
         }
     }
     if (!dwt) return;
@@ -464,6 +475,13 @@ extern "C" int k3g_sort_tokens(const int32_t *idx, int T, int topk, int n_expert
 
 namespace {
 
+/* The instance for these rows: WIDE when a wave has one token, STREAM when the sorted rows are more
+ * than the last-level cache holds. */
+#define OD_PICK(K, T, g)                                                                       \
+    ((size_t)(g).P * (g).n * sizeof(T) > OD_STREAM                                             \
+         ? ((g).tx_log >= 6 ? K<T, true, true> : K<T, false, true>)                            \
+         : ((g).tx_log >= 6 ? K<T, true, false> : K<T, false, false>))
+
 /* The checks the row calls share; rows and tokens as an OdGrid with its launch. */
 int row_sizes(const char *who, int dt, int T, int topk, int n)
 {
@@ -518,9 +536,9 @@ extern "C" int k3g_permute(const void *x, int dt, int T, int topk, int n, const 
     OdGrid g = {T, topk, n, T * topk, 0};
     const dim3 grid = row_grid(g, 16 / size);
     if (dt == K3_WBF16)
-        return k3h_launch(who, g.tx_log >= 6 ? k_permute<uint16_t, true> : k_permute<uint16_t, false>, grid, dim3(256), on.st, (const OdGrid)g,
+        return k3h_launch(who, OD_PICK(k_permute, uint16_t, g), grid, dim3(256), on.st, (const OdGrid)g,
                           (const uint16_t *)x, pos, (uint16_t *)sorted);
-    return k3h_launch(who, g.tx_log >= 6 ? k_permute<float, true> : k_permute<float, false>, grid, dim3(256), on.st, (const OdGrid)g, (const float *)x,
+    return k3h_launch(who, OD_PICK(k_permute, float, g), grid, dim3(256), on.st, (const OdGrid)g, (const float *)x,
                       pos, (float *)sorted);
 }
 
@@ -539,9 +557,9 @@ static int unpermute(const char *who, const void *sorted, int dt, int T, int top
     OdGrid g = {T, topk, n, T * topk, 0};
     const dim3 grid = row_grid(g, 16 / size);
     if (dt == K3_WBF16)
-        return k3h_launch(who, g.tx_log >= 6 ? k_unpermute<uint16_t, true> : k_unpermute<uint16_t, false>, grid, dim3(256), on.st, (const OdGrid)g,
+        return k3h_launch(who, OD_PICK(k_unpermute, uint16_t, g), grid, dim3(256), on.st, (const OdGrid)g,
                           (const uint16_t *)sorted, pos, wt, (const uint16_t *)add, (uint16_t *)out);
-    return k3h_launch(who, g.tx_log >= 6 ? k_unpermute<float, true> : k_unpermute<float, false>, grid, dim3(256), on.st, (const OdGrid)g,
+    return k3h_launch(who, OD_PICK(k_unpermute, float, g), grid, dim3(256), on.st, (const OdGrid)g,
                       (const float *)sorted, pos, wt, (const float *)add, (float *)out);
 }
 
@@ -585,10 +603,15 @@ extern "C" int k3g_unpermute_grad(const void *dout, const void *sorted, int dt, 
     const bool wave = n <= 128 * (16 / size);
     const int64_t slots = (int64_t)((T + 7) / 8) * topk;
     const dim3 grid((unsigned)(8 * (wave ? (slots + 3) / 4 : slots)));
-    if (dt == K3_WBF16)
-        return k3h_launch(who, wave ? k_unpermute_grad<uint16_t, 1> : k_unpermute_grad<uint16_t, 4>, grid,
-                          dim3(256), on.st, g, (const uint16_t *)dout, (const uint16_t *)sorted, pos, wt,
-                          (uint16_t *)dsorted, dwt);
-    return k3h_launch(who, wave ? k_unpermute_grad<float, 1> : k_unpermute_grad<float, 4>, grid, dim3(256),
-                      on.st, g, (const float *)dout, (const float *)sorted, pos, wt, (float *)dsorted, dwt);
+    const bool big = (size_t)g.P * n * size > OD_STREAM;
+    if (dt == K3_WBF16) {
+        auto *k = big ? (wave ? k_unpermute_grad<uint16_t, 1, true> : k_unpermute_grad<uint16_t, 4, true>)
+                         : (wave ? k_unpermute_grad<uint16_t, 1, false> : k_unpermute_grad<uint16_t, 4, false>);
+        return k3h_launch(who, k, grid, dim3(256), on.st, g, (const uint16_t *)dout, (const uint16_t *)sorted,
+                          pos, wt, (uint16_t *)dsorted, dwt);
+    }
+    auto *k = big ? (wave ? k_unpermute_grad<float, 1, true> : k_unpermute_grad<float, 4, true>)
+                     : (wave ? k_unpermute_grad<float, 1, false> : k_unpermute_grad<float, 4, false>);
+    return k3h_launch(who, k, grid, dim3(256), on.st, g, (const float *)dout, (const float *)sorted, pos, wt,
+                      (float *)dsorted, dwt);
 }

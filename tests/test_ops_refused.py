@@ -20,7 +20,7 @@ SORT = dict(idx=A, T=4, topk=8, n_experts=64, perm=A, off=A, pos=A, err=None, wo
 
 
 @pytest.mark.parametrize("change,what", [
-    (dict(T=-1), "tokens"), (dict(topk=0), "topk"), (dict(topk=65), "topk"), (dict(T=1 << 26), "pairs"),
+    (dict(T=-1), "tokens"), (dict(topk=0), "topk"), (dict(topk=65), "topk"), (dict(T=1 << 21), "pairs"),
     (dict(n_experts=0), "experts"), (dict(n_experts=1025), "experts"), (dict(idx=None), "missing"),
     (dict(perm=None), "missing"), (dict(off=None), "missing"), (dict(pos=None), "missing"), (dict(idx=A + 2), "aligned"),
     (dict(err=A + 1), "aligned"), (dict(T=4096), "workspace"), (dict(T=4096, work=A, work_bytes=16), "workspace"),
@@ -33,7 +33,7 @@ def test_sort_bytes():
     f = k3moe.lib().k3g_sort_bytes
     assert f(512, 8, 384) == 0 and f(0, 8, 384) == 0
     assert f(4096, 8, 384) > 0
-    assert f(-1, 8, 384) == 0 and f(4096, 65, 384) == 0 and f(4096, 8, 1025) == 0 and f(1 << 26, 2, 8) == 0
+    assert f(-1, 8, 384) == 0 and f(4096, 65, 384) == 0 and f(4096, 8, 1025) == 0 and f(1 << 23, 2, 8) == 0
 
 
 ROWS = dict(x=A, dt=F32, T=4, topk=8, n=64, pos=A, y=A, stream=None)
@@ -44,7 +44,7 @@ ROWS = dict(x=A, dt=F32, T=4, topk=8, n=64, pos=A, y=A, stream=None)
     (dict(dt=2), "fp32"), (dict(T=-1), "tokens"), (dict(topk=0), "topk"), (dict(n=0), "width"),
     (dict(n=(1 << 24) + 1), "width"), (dict(x=None), "missing"), (dict(pos=None), "missing"), (dict(y=None), "missing"),
     (dict(x=A + 2), "aligned"), (dict(dt=BF16, y=A + 1), "aligned"), (dict(pos=A + 2), "aligned"),
-    (dict(T=1 << 25, topk=4), "pairs"),
+    (dict(T=1 << 22, topk=4), "pairs"),
 ])
 def test_rows(capfd, name, change, what):
     refused(capfd, getattr(k3moe.lib(), name)(*dict(ROWS, **change).values()), what)
@@ -95,7 +95,8 @@ MM = dict(x=A, xdt=F32, rows=4, cols=64, w=A, n=32, y=A, ydt=F32, work=A, work_b
     (dict(xdt=2), "fp32"), (dict(ydt=9), "fp32"), (dict(cols=16), "columns"), (dict(n=8), "features"),
     (dict(n=24), "features"), (dict(n=0), "features"), (dict(w=None), "missing"), (dict(w=A + 8), "aligned"),
     (dict(y=A + 4), "aligned"), (dict(work=None), "workspace"), (dict(work_bytes=100), "workspace"),
-    (dict(work=A + 8), "workspace"), (dict(rows=-3), "rows"),
+    (dict(work=A + 8), "workspace"), (dict(rows=-3), "rows"), (dict(rows=1 << 26), "blocks"),
+    (dict(rows=1 << 25, n=1 << 20, work_bytes=1 << 40), "a launch takes"),
 ])
 def test_matmul(capfd, change, what):
     refused(capfd, k3moe.lib().k3g_matmul_mxfp4(*dict(MM, **change).values()), what)
@@ -109,7 +110,7 @@ GR = dict(x=A, xdt=BF16, rows=4, cols=64, perm=A, topk=2, off=A, n_experts=8, w=
     (dict(n_experts=0), "experts"), (dict(n_experts=1025), "experts"), (dict(topk=0), "topk"), (dict(topk=65), "topk"),
     (dict(perm=None), "topk"), (dict(off=None), "missing"), (dict(w=None), "missing"), (dict(w3=A + 4), "aligned"),
     (dict(w_step=4), "w_step"), (dict(w_step=12), "w_step"), (dict(b1=0.0), "caps"), (dict(b2=float("nan")), "caps"),
-    (dict(rows=1 << 25, topk=4), "pairs"), (dict(n=40), "features"), (dict(cols=100), "columns"),
+    (dict(rows=1 << 22, topk=4), "pairs"), (dict(n=40), "features"), (dict(cols=100), "columns"),
     (dict(work_bytes=0), "workspace"),
 ])
 def test_grouped(capfd, change, what):
@@ -119,6 +120,7 @@ def test_grouped(capfd, change, what):
 def test_work_bytes():
     f = k3moe.lib().k3g_mxfp4_work_bytes
     assert f(0, 64) == 0 and f(3, 48) == 0 and f(-1, 64) == 0
+    assert f((1 << 26) - 2, 512) > 0 and f((1 << 26) - 1, 512) == 0 and f(1 << 20, 1 << 20) == 0
     assert 0 < f(1, 32) <= f(2, 32) <= f(2, 544)
 
 
