@@ -265,7 +265,8 @@ __device__ __forceinline__ uint32_t mx_here(uint32_t v)
 }
 
 /* Workgroup b runs on XCD b % 8. One matrix: each XCD takes an eighth of the (feature tile, row
- * tile) pairs, so a matrix's tiles are read by one L2. Experts: the feature tiles are dealt to the
+ * tile) pairs in bands of 8 row tiles, so the 64 that run on it at a time are about 8 x 8 and read
+ * a sixteenth of what they would alone from past its L2. Experts: the feature tiles are dealt to the
  * XCDs one by one, each with two row tiles one after the other, so an expert's second row tile
  * finds its weights in that L2, and a few experts still fill every XCD. */
 template <int TM>
@@ -276,8 +277,9 @@ __device__ __forceinline__ bool mx_item(const MxProduct &g, int nft, int &ft, in
         const int tiles = (g.P + TM - 1) / TM, items = tiles * nft, per = (items + 7) / 8;
         const int i = xcd * per + s;
         if (s >= per || i >= items) return false;
-        ft = i / tiles;
-        return mx_tile<TM>(g, i - ft * tiles, e, p0, np);
+        const int band = i / (8 * nft), in = i - band * 8 * nft, wide = min(8, tiles - 8 * band);
+        ft = in / wide;
+        return mx_tile<TM>(g, 8 * band + in - ft * wide, e, p0, np);
     }
     const int i = 8 * (s >> 1) + xcd, pair = i / nft;
     ft = i - pair * nft;
@@ -473,14 +475,32 @@ k_mx_few(const MxProduct g)
 
 /* ---- many rows: a workgroup of four waves takes up to TM places by 4 x 64 features (gated: 4 x
  * 32 of each matrix). The activation quads of its places go to LDS by DMA, two stages of one quad;
- * the 16-byte unit u of row r lies at slot u ^ (r % 16) of the row's 256 bytes, so the 16 rows of
- * an operand read 16 different slots. Weights go straight from memory to registers, four chunks
- * ahead: no two waves of a workgroup share them. */
+ * the 16-byte unit u of row r lies at slot u ^ (r % 16) of the row's 256 bytes, so 16 rows of an
+ * operand read 16 different slots. Weights go straight from memory to registers, a quad ahead: no
+ * two waves of a workgroup share them.
+ *
+ * The products are v_mfma_scale_f32_32x32x64_f8f6f4: an instruction with scales takes longer to
+ * issue than the 16 cycles the 16x16x128 form keeps the matrix cores (from registers alone, one
+ * or two waves a SIMD, 5.4 and 6.9 PFLOP/s against 8.2 and 9.3). Its A operand is half a chunk of
+ * two row blocks: lane (d, hi) = (L % 32, L / 32) holds MX block 2 h + hi of the matrix row
+ * that lies 16 (d / 4 % 2) + 4 (d / 8) + d % 4 from the first. In that order of rows a lane's 16
+ * sums are 16 features in a row, 16 hi on, of place d. */
+typedef float mx_v16f __attribute__((ext_vector_type(16)));
+
+template <int J>
+__device__ __forceinline__ mx_v16f mx_mma32(const gm_v4u &a, uint32_t sa, const gm_v4u &b, uint32_t sb,
+                                            const mx_v16f &acc)
+{
+    const mx_v8i av = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
+    const mx_v8i bv = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, acc, 4, 4, J, (int)sa, J, (int)sb);
+}
 
 template <int TM>
 struct MxWave {
     static constexpr int SCALES = TM * 256, STAGE = TM * MX_XQ;
-    const uint8_t *w[4];               /* the row blocks' first quads */
+    const uint8_t *w[2];               /* two pairs of row blocks: the first's first quad, */
+    uint32_t at[2], sat[2];            /* this lane's codes and scales from there */
     const uint8_t *xq;                 /* the activations; in units of 16 bytes from there: */
     uint32_t x[TM / 16];               /* of each 16 rows the unit this lane copies */
     uint32_t xs;                       /* the scales this lane copies (waves below TM / 64) */
@@ -489,49 +509,63 @@ struct MxWave {
     int lane, wave, nQ, nK;
 };
 
-/* NB blocks of 16 places */
+/* NB blocks of 32 places */
 template <int TM, int NB>
-__device__ __forceinline__ void mx_gemm_sums(const MxWave<TM> &t, k3v4f (&acc)[4][NB])
+__device__ __forceinline__ void mx_gemm_sums(const MxWave<TM> &t, mx_v16f (&acc)[2][NB])
 {
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int n = 0; n < NB; ++n) acc[r][n] = k3v4f{0.f, 0.f, 0.f, 0.f};
-    const int c = t.lane & 15, q = t.lane >> 4;
-    gm_v4u a[4][4];
-    uint32_t sA[4], sN[4];
+        for (int n = 0; n < NB; ++n) acc[r][n] = mx_v16f{};
+    const int d = t.lane & 31, hi = t.lane >> 5;
+    gm_v4u a[4][2][2];
+    uint32_t sA[2][2], sN[2][2];
     auto load = [&](int Q, auto jc) {
         constexpr int J = decltype(jc)::value;
-        const uint32_t at = mx_here(16 * t.lane);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) a[J][r] = *(gm_g4)(t.w[r] + (size_t)Q * MX_QT + 1024 * J + at);
+        for (int r = 0; r < 2; ++r) {
+            const uint32_t at = mx_here(t.at[r]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                a[J][h][r] = *(gm_g4)(t.w[r] + (size_t)Q * MX_QT + 1024 * J + 512 * h + at);
+        }
     };
-    auto load_scales = [&](int Q, uint32_t (&s)[4]) {
+    auto load_scales = [&](int Q, uint32_t (&s)[2][2]) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[r] = gm_ld4(t.w[r] + (size_t)Q * MX_QT + 4096 + mx_here(4 * t.lane));
+        for (int r = 0; r < 2; ++r) {
+            const uint32_t at = mx_here(t.sat[r]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) s[h][r] = gm_ld4(t.w[r] + (size_t)Q * MX_QT + 4096 + 128 * h + at);
+        }
     };
     auto dma = [&](int Q) {
         const uint32_t st = t.lds + (Q & 1) * t.STAGE;
         const uint8_t *from = t.xq + (size_t)Q * MX_XQ;
 #pragma unroll
-        for (int i = 0; i < NB; ++i)
+        for (int i = 0; i < 2 * NB; ++i)
             gm_dma16(from + (uint64_t)mx_here(t.x[i]) * 16, st + 4096 * i + 1024 * t.wave);
-        if (64 * t.wave < 16 * NB)
+        if (64 * t.wave < 32 * NB)
             gm_dma16(from + (uint64_t)mx_here(t.xs) * 16, st + t.SCALES + 1024 * t.wave);
     };
-    auto chunk = [&](const uint8_t *st, const uint32_t (&sB)[NB], auto jc) {
+    /* operands are read one block ahead of their products, over the chunks of a quad */
+    gm_v4u b[2];
+    auto read = [&](const uint8_t *st, int jh, int n) {
+        return *(const gm_v4u *)(st + 256 * d + 16 * ((2 * jh + hi) ^ (d & 15)) + 8192 * n);
+    };
+    auto chunk = [&](const uint8_t *st, const uint32_t (&sB)[2][NB], auto jc) {
         constexpr int J = decltype(jc)::value;
-        const uint8_t *row = st + 256 * c + 16 * ((4 * J + q) ^ c);
-        /* read one block ahead of its products */
-        gm_v4u b[2];
-        b[0] = *(const gm_v4u *)row;
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            if (n + 1 < NB) b[(n + 1) & 1] = *(const gm_v4u *)(row + 4096 * (n + 1));
-            __builtin_amdgcn_sched_barrier(0);
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[r][n] = mx_mma4<J>(a[J][r], sA[r], b[n & 1], sB[n], acc[r][n]);
-        }
+            for (int n = 0; n < NB; ++n) {
+                const int i = (2 * J + h) * NB + n;
+                if (i + 1 < 8 * NB)
+                    b[(i + 1) & 1] = n + 1 < NB ? read(st, 2 * J + h, n + 1) : read(st, 2 * J + h + 1, 0);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+                    acc[r][n] = mx_mma32<J>(a[J][h][r], sA[h][r], b[i & 1], sB[h][n], acc[r][n]);
+            }
     };
     auto quad = [&](int Q, auto more) {
         constexpr bool MORE = decltype(more)::value;
@@ -544,11 +578,14 @@ __device__ __forceinline__ void mx_gemm_sums(const MxWave<TM> &t, k3v4f (&acc)[4
         }
         __builtin_amdgcn_sched_barrier(0);
         const uint8_t *st = t.ldsp + (Q & 1) * t.STAGE;
-        uint32_t sB[NB];
+        uint32_t sB[2][NB];
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
-            sB[n] = *(const uint32_t *)(st + t.SCALES + 256 * n + 16 * c + 4 * q);
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+                sB[h][n] = *(const uint32_t *)(st + t.SCALES + 512 * n + 16 * d + 8 * h + 4 * hi);
         const int left = MORE ? 4 : t.nK - 4 * Q;
+        b[0] = read(st, 0, 0);
         chunk(st, sB, GmInt<0>{});
         if (MORE) load(Q + 1, GmInt<0>{});
         if (left > 1) chunk(st, sB, GmInt<1>{});
@@ -559,7 +596,7 @@ __device__ __forceinline__ void mx_gemm_sums(const MxWave<TM> &t, k3v4f (&acc)[4
         if (MORE) {
             load(Q + 1, GmInt<3>{});
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sA[r] = sN[r];
+            for (int i = 0; i < 4; ++i) sA[i >> 1][i & 1] = sN[i >> 1][i & 1];
         }
         __builtin_amdgcn_sched_barrier(0);
     };
@@ -573,26 +610,42 @@ __device__ __forceinline__ void mx_gemm_sums(const MxWave<TM> &t, k3v4f (&acc)[4
     quad(t.nQ - 1, GmInt<0>{});
 }
 
+__device__ __forceinline__ void mx_put16(float *o, const mx_v16f &v)
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *(k3v4f *)(o + 4 * i) = k3v4f{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+}
+
+__device__ __forceinline__ void mx_put16(uint16_t *o, const mx_v16f &v)
+{
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        *(gm_v4u *)(o + 8 * i) = gm_v4u{k3d_bf16x2(v[8 * i], v[8 * i + 1]), k3d_bf16x2(v[8 * i + 2], v[8 * i + 3]),
+                                        k3d_bf16x2(v[8 * i + 4], v[8 * i + 5]),
+                                        k3d_bf16x2(v[8 * i + 6], v[8 * i + 7])};
+}
+
 template <typename Y, bool GATED, int TM, int NB>
 __device__ __forceinline__ void mx_gemm_tile(const MxProduct &g, const MxWave<TM> &t, int p0, int np,
                                              int rb0)
 {
-    k3v4f acc[4][NB];
+    mx_v16f acc[2][NB];
     mx_gemm_sums<TM, NB>(t, acc);
-    const int c = t.lane & 15, q = t.lane >> 4, nrb = g.N / 16;
+    const int d = t.lane & 31, hi = t.lane >> 5, nrb = g.N / 16;
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
-        if (16 * n + c >= np) continue;
-        Y *o = (Y *)g.y + (size_t)(p0 + 16 * n + c) * g.N + 4 * q;
+        if (32 * n + d >= np) continue;
+        Y *o = (Y *)g.y + (size_t)(p0 + 32 * n + d) * g.N;
 #pragma unroll
-        for (int r = 0; r < (GATED ? 2 : 4); ++r) {
-            if (rb0 + r >= nrb) continue;
-            k3v4f v = acc[r][n];
+        for (int r = 0; r < (GATED ? 1 : 2); ++r) {
+            const int rb = rb0 + 2 * r + hi;
+            if (rb >= nrb) continue;
+            mx_v16f v = acc[r][n];
             if (GATED) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = k3d_act(v[i], acc[r + 2][n][i], g.b1, g.b2);
+                for (int i = 0; i < 16; ++i) v[i] = k3d_act(v[i], acc[1][n][i], g.b1, g.b2);
             }
-            mx_put(o + 16 * (rb0 + r), v);
+            mx_put16(o + 16 * rb, v);
         }
     }
 }
@@ -621,27 +674,29 @@ k_mx_gemm(const MxProduct g)
         mx_zeros<Y, 256>(g, p0, np, 64 * RB * ft, 64 * RB);
         return;
     }
+    const int d = t.lane & 31, hi = t.lane >> 5, row = 4 * (d >> 3) + (d & 3);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int rb = rb0 + (GATED ? r & 1 : r);
-        t.w[r] = gm_uniform_ptr((GATED && r >= 2 ? w3 : w1) + (rb >= nrb ? 0 : (size_t)rb * g.nQ * MX_QT));
+    for (int r = 0; r < 2; ++r) {
+        /* row blocks past the last are read as the first one and never stored */
+        const int rb = rb0 + (GATED ? 0 : 2 * r);
+        t.w[r] = gm_uniform_ptr((GATED && r ? w3 : w1) + (rb >= nrb ? 0 : (size_t)rb * g.nQ * MX_QT));
+        const uint32_t second = rb + 1 < nrb ? ((d >> 2) & 1) * (uint32_t)g.nQ * MX_QT : 0;
+        t.at[r] = second + 16 * row + 256 * hi;
+        t.sat[r] = second + 4 * row + 64 * hi;
     }
     auto source = [&](int r) {
         const int row = mx_row(g, p0 + min(r, np - 1));
         return (uint32_t)(row < 0 ? g.T : row) * row16;
     };
-    const int nb = (np + 15) / 16, sub = 4 * t.wave + (t.lane >> 4);
+    const int nb = (np + 31) / 32, sub = 4 * t.wave + (t.lane >> 4);
 #pragma unroll
     for (int i = 0; i < TM / 16; ++i) t.x[i] = source(16 * i + sub) + ((t.lane & 15) ^ sub);
     t.xs = source(64 * t.wave + t.lane) + 16;
     if constexpr (TM == 128) {
-        if (nb > 6) return mx_gemm_tile<Y, GATED, TM, 8>(g, t, p0, np, rb0);
-        if (nb > 4) return mx_gemm_tile<Y, GATED, TM, 6>(g, t, p0, np, rb0);
+        if (nb == 4) return mx_gemm_tile<Y, GATED, TM, 4>(g, t, p0, np, rb0);
+        if (nb == 3) return mx_gemm_tile<Y, GATED, TM, 3>(g, t, p0, np, rb0);
     }
-    if constexpr (TM >= 64) {
-        if (nb > 2) return mx_gemm_tile<Y, GATED, TM, 4>(g, t, p0, np, rb0);
-    }
-    if (nb > 1) return mx_gemm_tile<Y, GATED, TM, 2>(g, t, p0, np, rb0);
+    if (nb == 2) return mx_gemm_tile<Y, GATED, TM, 2>(g, t, p0, np, rb0);
     mx_gemm_tile<Y, GATED, TM, 1>(g, t, p0, np, rb0);
 }
 
