@@ -496,13 +496,14 @@ __device__ __forceinline__ mx_v16f mx_mma32(const gm_v4u &a, uint32_t sa, const 
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, acc, 4, 4, J, (int)sa, J, (int)sb);
 }
 
-template <int TM>
+template <int TM, int WV>
 struct MxWave {
     static constexpr int SCALES = TM * 256, STAGE = TM * MX_XQ;
+    static constexpr int COPIES = (TM / 4 + WV - 1) / WV;      /* of 4 rows, by each wave */
     const uint8_t *w[2];               /* two pairs of row blocks: the first's first quad, */
     uint32_t at[2], sat[2];            /* this lane's codes and scales from there */
     const uint8_t *xq;                 /* the activations; in units of 16 bytes from there: */
-    uint32_t x[TM / 16];               /* of each 16 rows the unit this lane copies */
+    uint32_t x[COPIES];                /* the units this lane copies: rows 4 (wave + WV i) .. + 3 */
     uint32_t xs;                       /* the scales this lane copies (waves below TM / 64) */
     uint32_t lds;
     const uint8_t *ldsp;
@@ -510,8 +511,8 @@ struct MxWave {
 };
 
 /* NB blocks of 32 places */
-template <int TM, int NB>
-__device__ __forceinline__ void mx_gemm_sums(const MxWave<TM> &t, mx_v16f (&acc)[2][NB])
+template <int TM, int WV, int NB>
+__device__ __forceinline__ void mx_gemm_sums(const MxWave<TM, WV> &t, mx_v16f (&acc)[2][NB])
 {
 #pragma unroll
     for (int r = 0; r < 2; ++r)
@@ -542,12 +543,16 @@ __device__ __forceinline__ void mx_gemm_sums(const MxWave<TM> &t, mx_v16f (&acc)
         const uint32_t st = t.lds + (Q & 1) * t.STAGE;
         const uint8_t *from = t.xq + (size_t)Q * MX_XQ;
 #pragma unroll
-        for (int i = 0; i < 2 * NB; ++i)
-            gm_dma16(from + (uint64_t)mx_here(t.x[i]) * 16, st + 4096 * i + 1024 * t.wave);
+        for (int i = 0; WV * i < 8 * NB; ++i) {
+            const int at = WV * i + t.wave;
+            if (WV * (i + 1) <= 8 * NB || at < 8 * NB)
+                gm_dma16(from + (uint64_t)mx_here(t.x[i]) * 16, st + 1024 * at);
+        }
         if (64 * t.wave < 32 * NB)
             gm_dma16(from + (uint64_t)mx_here(t.xs) * 16, st + t.SCALES + 1024 * t.wave);
     };
-    /* operands are read one block ahead of their products, over the chunks of a quad */
+    /* operands are read one block ahead of their products, over the chunks of a quad (two and three
+     * ahead are no faster: 8192 rows by 8192 x 8192 in 314, 316 and 319 us) */
     gm_v4u b[2];
     auto read = [&](const uint8_t *st, int jh, int n) {
         return *(const gm_v4u *)(st + 256 * d + 16 * ((2 * jh + hi) ^ (d & 15)) + 8192 * n);
@@ -559,8 +564,7 @@ __device__ __forceinline__ void mx_gemm_sums(const MxWave<TM> &t, mx_v16f (&acc)
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
                 const int i = (2 * J + h) * NB + n;
-                if (i + 1 < 8 * NB)
-                    b[(i + 1) & 1] = n + 1 < NB ? read(st, 2 * J + h, n + 1) : read(st, 2 * J + h + 1, 0);
+                if (i + 1 < 8 * NB) b[(i + 1) & 1] = read(st, (i + 1) / NB, (i + 1) % NB);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int r = 0; r < 2; ++r)
@@ -625,12 +629,12 @@ __device__ __forceinline__ void mx_put16(uint16_t *o, const mx_v16f &v)
                                         k3d_bf16x2(v[8 * i + 6], v[8 * i + 7])};
 }
 
-template <typename Y, bool GATED, int TM, int NB>
-__device__ __forceinline__ void mx_gemm_tile(const MxProduct &g, const MxWave<TM> &t, int p0, int np,
+template <typename Y, bool GATED, int NB, int TM, int WV>
+__device__ __forceinline__ void mx_gemm_tile(const MxProduct &g, const MxWave<TM, WV> &t, int p0, int np,
                                              int rb0)
 {
     mx_v16f acc[2][NB];
-    mx_gemm_sums<TM, NB>(t, acc);
+    mx_gemm_sums<TM, WV, NB>(t, acc);
     const int d = t.lane & 31, hi = t.lane >> 5, nrb = g.N / 16;
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
@@ -650,16 +654,16 @@ __device__ __forceinline__ void mx_gemm_tile(const MxProduct &g, const MxWave<TM
     }
 }
 
-template <typename Y, bool GATED, int TM>
-__global__ void __launch_bounds__(256, 2)
+template <typename Y, bool GATED, int TM, int WV>
+__global__ void __launch_bounds__(64 * WV, 2)
 k_mx_gemm(const MxProduct g)
 {
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * MxWave<TM>::STAGE];
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * MxWave<TM, WV>::STAGE];
     constexpr int RB = GATED ? 2 : 4;           /* row blocks of a wave in a matrix */
-    const int nrb = g.N / 16, nft = (nrb + 4 * RB - 1) / (4 * RB);
+    const int nrb = g.N / 16, nft = (nrb + WV * RB - 1) / (WV * RB);
     int ft, e, p0, np;
     if (!mx_item<TM>(g, nft, ft, e, p0, np)) return;
-    MxWave<TM> t;
+    MxWave<TM, WV> t;
     t.lane = threadIdx.x & 63;
     t.wave = gm_uniform(threadIdx.x >> 6);
     t.nQ = g.nQ;
@@ -668,10 +672,10 @@ k_mx_gemm(const MxProduct g)
     t.lds = (uint32_t)(uintptr_t)(k3lds)lds;
     t.ldsp = lds;
     const uint8_t *w1 = mx_matrix(g, g.w, e), *w3 = GATED ? mx_matrix(g, g.w3, e) : w1;
-    const int rb0 = (4 * ft + t.wave) * RB;
+    const int rb0 = (WV * ft + t.wave) * RB;
     const uint32_t row16 = g.nQ * (MX_XQ / 16);
     if (!w1 || !w3) {
-        mx_zeros<Y, 256>(g, p0, np, 64 * RB * ft, 64 * RB);
+        mx_zeros<Y, 64 * WV>(g, p0, np, 16 * WV * RB * ft, 16 * WV * RB);
         return;
     }
     const int d = t.lane & 31, hi = t.lane >> 5, row = 4 * (d >> 3) + (d & 3);
@@ -688,16 +692,19 @@ k_mx_gemm(const MxProduct g)
         const int row = mx_row(g, p0 + min(r, np - 1));
         return (uint32_t)(row < 0 ? g.T : row) * row16;
     };
-    const int nb = (np + 31) / 32, sub = 4 * t.wave + (t.lane >> 4);
+    const int nb = (np + 31) / 32;
 #pragma unroll
-    for (int i = 0; i < TM / 16; ++i) t.x[i] = source(16 * i + sub) + ((t.lane & 15) ^ sub);
+    for (int i = 0; i < t.COPIES; ++i) {
+        const int r = 4 * (WV * i + t.wave) + (t.lane >> 4);
+        t.x[i] = source(r) + ((t.lane & 15) ^ (r & 15));
+    }
     t.xs = source(64 * t.wave + t.lane) + 16;
     if constexpr (TM == 128) {
-        if (nb == 4) return mx_gemm_tile<Y, GATED, TM, 4>(g, t, p0, np, rb0);
-        if (nb == 3) return mx_gemm_tile<Y, GATED, TM, 3>(g, t, p0, np, rb0);
+        if (nb == 4) return mx_gemm_tile<Y, GATED, 4>(g, t, p0, np, rb0);
+        if (nb == 3) return mx_gemm_tile<Y, GATED, 3>(g, t, p0, np, rb0);
     }
-    if (nb == 2) return mx_gemm_tile<Y, GATED, TM, 2>(g, t, p0, np, rb0);
-    mx_gemm_tile<Y, GATED, TM, 1>(g, t, p0, np, rb0);
+    if (nb == 2) return mx_gemm_tile<Y, GATED, 2>(g, t, p0, np, rb0);
+    mx_gemm_tile<Y, GATED, 1>(g, t, p0, np, rb0);
 }
 
 /* ------------------------------------------------------------- entry points ---- */
@@ -778,7 +785,8 @@ extern "C" size_t k3g_mxfp4_work_bytes(int rows, int cols)
 }
 
 /* Which kernel a product runs on: rows of a tile, its row blocks (of each matrix), the waves that
- * share its columns (0: k_mx_gemm), and whether x is quantised inside it. */
+ * share its columns (0: k_mx_gemm, a wave per four row blocks, or two of each matrix), and whether x
+ * is quantised inside it. */
 struct MxPlan {
     int tm, rb, wv;
     bool values;
@@ -794,13 +802,20 @@ static int64_t mx_grid(const MxProduct &g, int tm, int rb)
     return ((tiles + 1) / 2 * nft + 7) / 8 * 16;
 }
 
-/* A larger tile reads less, a smaller one makes more workgroups: the largest tile that still gives
- * most CUs one (us, whole calls, bf16).
- * One matrix, 7168 columns, 3584 features unless said: 1 row: quantised inside 5.5, before 7.2; 4:
- * 7.6 and 7.7; 8: 10.8 and 7.5. 16 rows: 8 waves x 1 row block 8.5, 4 x 2 9.5, 4 x 4 12.4; 32 rows:
- * 11.3, 9.2, 12.0; 64 rows: 16.6, 12.9, 11.7; 128 rows: 4 x 4 by 16 rows 16.4, by 32 14.1, by 64
- * 19.2; 256 rows: 26.2, 21.8, 19.3, k_mx_gemm 27.9; 512 rows: by 64 33.9, k_mx_gemm 29.1. 6144
- * features: 512 rows, k_mx_gemm by 64 29.7, by 128 38.7; 1024 rows 49.0, 42.4.
+/* One matrix: a CU's workgroups take turns on what bounds them (its matrix cores, the data that
+ * its L1 returns), so a call lasts as long as the CU with the most, ceil(workgroups / 256) times the
+ * time of one. That time, in us at 7168 columns beside about 6 of quantisation and launch, is `us`:
+ * the tile with the smallest product is taken. Whole calls, us, bf16, tiles in the table's order:
+ *   16 rows by 3584            23.4  .     23.3  .     14.3  10.9  12.4  9.5   8.5
+ *   64 rows                    28.9  .     28.6  .     20.2  14.4  11.7  12.9  16.6
+ *   256 rows                   33.7  30.7  26.6  23.0  19.5  21.8  26.2  30.2  42.6
+ *   512 rows by 6144           34.9  32.5  28.2  25.5  48.1  50.8  63.5  89.1  135
+ *   1024 rows                  37.7  36.5  45.6  39.9  85.6
+ *   2048 rows                  66.1  60.9  70.1  74.0  162
+ *   4096 rows by 7168          130   139   153   166   365
+ * Up to four rows are quantised inside (1 row 5.5 against 7.2, 4 rows 7.6 and 7.7, 8 rows 10.8 and
+ * 7.5).
+ *
  * Experts: a few tokens meet about one row an expert, and the weights are all there is to wait for
  * (8 tokens x 8 by 384 experts of 7168 -> 2 x 2048: inside 138, before 139, k_mx_gemm 150; 1 token:
  * 22.6, 24.7, 26.1); where 16 tokens meet 8 experts quantising inside costs 16.8 against 11.9. 64
@@ -809,16 +824,23 @@ static int64_t mx_grid(const MxProduct &g, int tm, int rb)
  * 2048 -> 7168: k_mx_gemm by 64 815, by 128 741. */
 static MxPlan mx_plan(const MxProduct &g, bool gated)
 {
+    static const struct { int tm, rb, wv; float us; } tiles[] = {
+        {128, 16, 0, 28.f}, {128, 12, 0, 25.f}, {64, 16, 0, 20.f}, {64, 12, 0, 17.f}, {64, 4, 4, 13.5f},
+        {32, 4, 4, 8.f},    {16, 4, 4, 5.5f},   {16, 2, 4, 3.4f},  {16, 1, 8, 2.6f},
+    };
     const int RB = gated ? 2 : 4;
     if (!g.off) {
         if (g.P <= 4) return {16, 1, 8, true, 0};
-        if (mx_grid(g, 128, 16) >= 160) return {128, 16, 0, false, 0};
-        if (mx_grid(g, 64, 16) >= 96) return {64, 16, 0, false, 0};
-        if (mx_grid(g, 64, 4) >= 192) return {64, 4, 4, false, 0};
-        if (mx_grid(g, 32, 4) >= 192) return {32, 4, 4, false, 0};
-        if (mx_grid(g, 16, 4) >= 192) return {16, 4, 4, false, 0};
-        if (mx_grid(g, 16, 2) >= 192) return {16, 2, 4, false, 0};
-        return {16, 1, 8, false, 0};
+        MxPlan best = {};
+        float least = 0.0f;
+        for (const auto &t : tiles) {
+            const float us = (float)((mx_grid(g, t.tm, t.rb) + 255) / 256) * t.us;
+            if (!best.tm || us < least) {
+                best = {t.tm, t.rb, t.wv, false, 0};
+                least = us;
+            }
+        }
+        return best;
     }
     const int met = min(g.E, g.P), mean = (g.P + met - 1) / met;
     if (g.T <= 16 && mean <= 2) return {16, RB, 4, true, 0};
@@ -835,10 +857,10 @@ static int mx_run_few(const char *who, const MxProduct &g, const MxPlan &p, hipS
     return k3h_launch(who, k_mx_few<X, Y, GATED, WV, U, NB>, dim3(p.blocks), dim3(64 * WV), st, (MxProduct)g);
 }
 
-template <typename Y, bool GATED, int TM>
+template <typename Y, bool GATED, int TM, int WV>
 static int mx_run_gemm(const char *who, const MxProduct &g, const MxPlan &p, hipStream_t st)
 {
-    return k3h_launch(who, k_mx_gemm<Y, GATED, TM>, dim3(p.blocks), dim3(256), st, (MxProduct)g);
+    return k3h_launch(who, k_mx_gemm<Y, GATED, TM, WV>, dim3(p.blocks), dim3(64 * WV), st, (MxProduct)g);
 }
 
 template <typename X>
@@ -857,8 +879,12 @@ template <typename Y>
 static int mx_launch(const char *who, const MxProduct &g, const MxPlan &p, bool gated, hipStream_t st)
 {
     if (!p.wv) {
-        if (gated) return p.tm == 128 ? mx_run_gemm<Y, true, 128>(who, g, p, st) : mx_run_gemm<Y, true, 64>(who, g, p, st);
-        return p.tm == 128 ? mx_run_gemm<Y, false, 128>(who, g, p, st) : mx_run_gemm<Y, false, 64>(who, g, p, st);
+        if (gated) return p.tm == 128 ? mx_run_gemm<Y, true, 128, 4>(who, g, p, st)
+                                      : mx_run_gemm<Y, true, 64, 4>(who, g, p, st);
+        if (p.rb == 12) return p.tm == 128 ? mx_run_gemm<Y, false, 128, 3>(who, g, p, st)
+                                           : mx_run_gemm<Y, false, 64, 3>(who, g, p, st);
+        return p.tm == 128 ? mx_run_gemm<Y, false, 128, 4>(who, g, p, st)
+                           : mx_run_gemm<Y, false, 64, 4>(who, g, p, st);
     }
     if (gated) return p.tm == 32 ? mx_run_few<MxQuads, Y, true, 4, 4, 2>(who, g, p, st)
                                  : mx_run_few<MxQuads, Y, true, 4, 4, 1>(who, g, p, st);
