@@ -26,6 +26,7 @@
 #define MX_MAX_ROWS (1 << 26)
 #define MX_MAX_COLS (1 << 20)
 #define MX_MAX_PAIRS (1 << 23)
+#define MX_MAX_EXPERTS 1024
 #define MX_MAX_QUADS (1 << 26)       /* activation quads of a call: k_mx_x has 64 threads each */
 #define MX_MAX_BLOCKS (1 << 23)      /* a launch has fewer than 2^32 threads */
 
@@ -182,11 +183,13 @@ struct MxProduct {
     int N;
     float b1, b2;
     void *y;
+    bool stream;                     /* y is more than the last-level cache holds */
 };
 
 /* Row tile `item` of up to TM places: expert, first place and count; false past the last. Every
- * wave finds it by itself: a lane takes 16 experts, then a wave scan of their tile counts. The
- * ranges are clamped to the places there are, whatever off holds. */
+ * wave finds it by itself: a lane takes up to 16 experts, all their ranges asked for at once (one
+ * after the other they were 3 us of a workgroup's time), a wave scan of the lanes' tile counts
+ * finds the lane that has it. The ranges are clamped to the places there are, whatever off holds. */
 template <int TM>
 __device__ __forceinline__ bool mx_tile(const MxProduct &g, int item, int &e, int &p0, int &np)
 {
@@ -197,11 +200,17 @@ __device__ __forceinline__ bool mx_tile(const MxProduct &g, int item, int &e, in
         return np > 0;
     }
     const int lane = threadIdx.x & 63;
-    const int per = (g.E + 63) >> 6, e0 = lane * per, e1 = min(g.E, e0 + per);
-    int n = 0;
-    for (int i = e0; i < e1; ++i) {
-        const int a = min(max(g.off[i], 0), g.P), b = min(max(g.off[i + 1], a), g.P);
-        n += (b - a + TM - 1) / TM;
+    constexpr int MOST = MX_MAX_EXPERTS / 64;
+    const int per = (g.E + 63) >> 6, e0 = lane * per;
+    int at[MOST + 1], n = 0;
+#pragma unroll
+    for (int i = 0; i <= MOST; ++i)
+        if (i <= per) at[i] = g.off[min(e0 + i, g.E)];
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+        if (i >= per) continue;
+        at[i] = min(max(at[i], 0), g.P);
+        n += (min(max(at[i + 1], at[i]), g.P) - at[i] + TM - 1) / TM;
     }
     int inc = n;
 #pragma unroll
@@ -211,28 +220,41 @@ __device__ __forceinline__ bool mx_tile(const MxProduct &g, int item, int &e, in
     }
     const uint64_t past = __ballot(inc > item);
     if (!past) return false;
-    const int L = __ffsll((unsigned long long)past) - 1;
-    int at = gm_uniform(__shfl(inc - n, L, K3G_WAVE));
-    for (int i = L * per; i < g.E; ++i) {
-        const int a = min(max(g.off[i], 0), g.P), b = min(max(g.off[i + 1], a), g.P);
-        const int t = (b - a + TM - 1) / TM;
-        if (item < at + t) {
-            e = gm_uniform(i);
-            p0 = gm_uniform(a + (item - at) * TM);
-            np = gm_uniform(min(TM, b - p0));
-            return true;
+    int left = item - (inc - n), fe = 0, fp = 0, fn = 0;
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+        if (i >= per) continue;
+        const int rows = min(max(at[i + 1], at[i]), g.P) - at[i], t = (rows + TM - 1) / TM;
+        if (left >= 0 && left < t) {
+            fe = e0 + i;
+            fp = at[i] + left * TM;
+            fn = min(TM, rows - left * TM);
         }
-        at += t;
+        left -= t;
     }
-    return false;
+    const int L = __ffsll((unsigned long long)past) - 1;
+    e = __builtin_amdgcn_readlane(fe, L);
+    p0 = __builtin_amdgcn_readlane(fp, L);
+    np = __builtin_amdgcn_readlane(fn, L);
+    return true;
 }
 
-/* The activation row of a place; -1 (zeros) when perm holds no pair of these tokens. */
-__device__ __forceinline__ int mx_row(const MxProduct &g, int place)
+/* What perm says of a place (the place itself without one), and the activation row that is: -1
+ * (zeros) for no pair of these tokens. */
+__device__ __forceinline__ int mx_pair(const MxProduct &g, int place) { return g.perm ? g.perm[place] : place; }
+
+__device__ __forceinline__ int mx_row(const MxProduct &g, int pair)
 {
-    if (!g.perm) return place;
-    const int p = g.perm[place], t = p / g.topk;
-    return p >= 0 && t < g.T ? t : -1;
+    if (!g.perm) return pair;
+    const int t = pair / g.topk;
+    return pair >= 0 && t < g.T ? t : -1;
+}
+
+/* where a pair's activation quads begin, in units of 16 bytes */
+__device__ __forceinline__ uint32_t mx_units(const MxProduct &g, int pair)
+{
+    const int row = mx_row(g, pair);
+    return (uint32_t)(row < 0 ? g.T : row) * (uint32_t)(g.nQ * (MX_XQ / 16));
 }
 
 __device__ __forceinline__ const uint8_t *mx_matrix(const MxProduct &g, const uint8_t *w, int e)
@@ -354,7 +376,7 @@ __device__ __forceinline__ void mx_few_sums(const MxProduct &g, const MxFew<X, U
             const int col = 512 * Q + 8 * t.lane, blk = t.lane >> 2, cols = g.cols;
             gm_wave_sync();
             for (int r = 0; r < t.np; ++r) {
-                const int row = gm_uniform(mx_row(g, t.p0 + r));
+                const int row = gm_uniform(mx_row(g, mx_pair(g, t.p0 + r)));
                 Mx8 v = {{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}};
                 if (col < cols && row >= 0) v = mx_load8(t.row + (size_t)row * cols + col);
                 uint32_t s;
@@ -432,10 +454,7 @@ k_mx_few(const MxProduct g)
     }
     if constexpr (QUADS) {
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            const int row = mx_row(g, p0 + min(16 * n + c, np - 1));
-            t.x[n] = (uint32_t)(row < 0 ? g.T : row) * (g.nQ * (MX_XQ / 16));
-        }
+        for (int n = 0; n < NB; ++n) t.x[n] = mx_units(g, mx_pair(g, p0 + min(16 * n + c, np - 1)));
     } else {
         t.row = (const X *)g.x;
         t.lds = lds + wave * MX_QT;
@@ -503,8 +522,8 @@ struct MxWave {
     const uint8_t *w[2];               /* two pairs of row blocks: the first's first quad, */
     uint32_t at[2], sat[2];            /* this lane's codes and scales from there */
     const uint8_t *xq;                 /* the activations; in units of 16 bytes from there: */
-    uint32_t x[COPIES];                /* the units this lane copies: rows 4 (wave + WV i) .. + 3 */
-    uint32_t xs;                       /* the scales this lane copies (waves below TM / 64) */
+    int row[COPIES], rows;             /* rows 4 (wave + WV i) .. + 3: the one this lane copies a unit of, */
+    uint32_t unit[COPIES];             /* and which; the one whose scales it copies (waves below TM / 64) */
     uint32_t lds;
     const uint8_t *ldsp;
     int lane, wave, nQ, nK;
@@ -512,7 +531,8 @@ struct MxWave {
 
 /* NB blocks of 32 places */
 template <int TM, int WV, int NB>
-__device__ __forceinline__ void mx_gemm_sums(const MxWave<TM, WV> &t, mx_v16f (&acc)[2][NB])
+__device__ __forceinline__ void mx_gemm_sums(const MxProduct &g, const MxWave<TM, WV> &t,
+                                             mx_v16f (&acc)[2][NB])
 {
 #pragma unroll
     for (int r = 0; r < 2; ++r)
@@ -520,7 +540,7 @@ __device__ __forceinline__ void mx_gemm_sums(const MxWave<TM, WV> &t, mx_v16f (&
         for (int n = 0; n < NB; ++n) acc[r][n] = mx_v16f{};
     const int d = t.lane & 31, hi = t.lane >> 5;
     gm_v4u a[4][2][2];
-    uint32_t sA[2][2], sN[2][2];
+    uint32_t sA[2][2], sN[2][2], x[MxWave<TM, WV>::COPIES], xs;
     auto load = [&](int Q, auto jc) {
         constexpr int J = decltype(jc)::value;
 #pragma unroll
@@ -546,10 +566,10 @@ __device__ __forceinline__ void mx_gemm_sums(const MxWave<TM, WV> &t, mx_v16f (&
         for (int i = 0; WV * i < 8 * NB; ++i) {
             const int at = WV * i + t.wave;
             if (WV * (i + 1) <= 8 * NB || at < 8 * NB)
-                gm_dma16(from + (uint64_t)mx_here(t.x[i]) * 16, st + 1024 * at);
+                gm_dma16(from + (uint64_t)mx_here(x[i]) * 16, st + 1024 * at);
         }
         if (64 * t.wave < 32 * NB)
-            gm_dma16(from + (uint64_t)mx_here(t.xs) * 16, st + t.SCALES + 1024 * t.wave);
+            gm_dma16(from + (uint64_t)mx_here(xs) * 16, st + t.SCALES + 1024 * t.wave);
     };
     /* operands are read one block ahead of their products, over the chunks of a quad (two and three
      * ahead are no faster: 8192 rows by 8192 x 8192 in 314, 316 and 319 us) */
@@ -604,53 +624,79 @@ __device__ __forceinline__ void mx_gemm_sums(const MxWave<TM, WV> &t, mx_v16f (&
         }
         __builtin_amdgcn_sched_barrier(0);
     };
-    dma(0);
+    /* the weights are asked for before the rows of the activations are known */
     load_scales(0, sA);
     load(0, GmInt<0>{});
     load(0, GmInt<1>{});
     load(0, GmInt<2>{});
     load(0, GmInt<3>{});
+#pragma unroll
+    for (int i = 0; i < t.COPIES; ++i) x[i] = mx_units(g, t.row[i]) + t.unit[i];
+    xs = mx_units(g, t.rows) + 16;
+    dma(0);
+    gm_wait_vm<0>();
     for (int Q = 0; Q + 1 < t.nQ; ++Q) quad(Q, GmInt<1>{});
     quad(t.nQ - 1, GmInt<0>{});
 }
 
-__device__ __forceinline__ void mx_put16(float *o, const mx_v16f &v)
+/* 16 consecutive sums as units of 16 bytes at o, unit i at slot (u + i) ^ x */
+__device__ __forceinline__ void mx_put16(uint8_t *o, int u, int x, const mx_v16f &v, float)
 {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) *(k3v4f *)(o + 4 * i) = k3v4f{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+    for (int i = 0; i < 4; ++i)
+        *(k3v4f *)(o + 16 * ((u + i) ^ x)) = k3v4f{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
 }
 
-__device__ __forceinline__ void mx_put16(uint16_t *o, const mx_v16f &v)
+__device__ __forceinline__ void mx_put16(uint8_t *o, int u, int x, const mx_v16f &v, uint16_t)
 {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-        *(gm_v4u *)(o + 8 * i) = gm_v4u{k3d_bf16x2(v[8 * i], v[8 * i + 1]), k3d_bf16x2(v[8 * i + 2], v[8 * i + 3]),
-                                        k3d_bf16x2(v[8 * i + 4], v[8 * i + 5]),
-                                        k3d_bf16x2(v[8 * i + 6], v[8 * i + 7])};
+        *(gm_v4u *)(o + 16 * ((u + i) ^ x)) =
+            gm_v4u{k3d_bf16x2(v[8 * i], v[8 * i + 1]), k3d_bf16x2(v[8 * i + 2], v[8 * i + 3]),
+                   k3d_bf16x2(v[8 * i + 4], v[8 * i + 5]), k3d_bf16x2(v[8 * i + 6], v[8 * i + 7])};
 }
 
+/* The sums go out by way of LDS, a wave's own 16 KB (TM 128) at a time: a lane holds 32 or 64 bytes
+ * of one place's row, and stored as they are they reach the L2 as quarters of lines (470 MB of bf16
+ * rows cost 129 of 729 us); read back by rows, a wave stores 8 rows of 128 bytes at once. */
 template <typename Y, bool GATED, int NB, int TM, int WV>
-__device__ __forceinline__ void mx_gemm_tile(const MxProduct &g, const MxWave<TM, WV> &t, int p0, int np,
-                                             int rb0)
+__device__ __forceinline__ void mx_gemm_tile(const MxProduct &g, const MxWave<TM, WV> &t, uint8_t *lds,
+                                             int p0, int np, int rb0)
 {
     mx_v16f acc[2][NB];
-    mx_gemm_sums<TM, WV, NB>(t, acc);
-    const int d = t.lane & 31, hi = t.lane >> 5, nrb = g.N / 16;
+    mx_gemm_sums<TM, WV, NB>(g, t, acc);
+    const int d = t.lane & 31, hi = t.lane >> 5;
+    constexpr int F = GATED ? 32 : 64, UNITS = F * (int)sizeof(Y) / 16;      /* of a row */
+    constexpr int FIT = TM * 128 / (32 * UNITS * 16), PER = FIT < NB ? FIT : NB;
+    static_assert(WV * TM * 128 <= 2 * MxWave<TM, WV>::STAGE, "LDS");
+    uint8_t *mine = lds + t.wave * TM * 128;
+    __syncthreads();
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        if (32 * n + d >= np) continue;
-        Y *o = (Y *)g.y + (size_t)(p0 + 32 * n + d) * g.N;
+    for (int n0 = 0; n0 < NB; n0 += PER) {
 #pragma unroll
-        for (int r = 0; r < (GATED ? 1 : 2); ++r) {
-            const int rb = rb0 + 2 * r + hi;
-            if (rb >= nrb) continue;
-            mx_v16f v = acc[r][n];
-            if (GATED) {
+        for (int n = n0; n < n0 + PER && n < NB; ++n) {
+            const int row = 32 * (n - n0) + d;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) v[i] = k3d_act(v[i], acc[1][n][i], g.b1, g.b2);
+            for (int r = 0; r < (GATED ? 1 : 2); ++r) {
+                mx_v16f v = acc[r][n];
+                if (GATED) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[i] = k3d_act(v[i], acc[1][n][i], g.b1, g.b2);
+                }
+                mx_put16(mine + 16 * UNITS * row, (32 * r + 16 * hi) * (int)sizeof(Y) / 16, row % UNITS, v, Y());
             }
-            mx_put16(o + 16 * rb, v);
         }
+        gm_wave_sync();
+        const int u = t.lane % UNITS, f = 16 * rb0 + u * (16 / (int)sizeof(Y));
+        const int rows = min(np - 32 * n0, 32 * PER);
+        Y *o = (Y *)g.y + (size_t)(p0 + 32 * n0) * g.N + f;
+        for (int row = t.lane / UNITS; row < rows; row += 64 / UNITS)
+            if (f < g.N) {
+                const gm_v4u v = *(const gm_v4u *)(mine + 16 * (UNITS * row + (u ^ row % UNITS)));
+                if (g.stream) __builtin_nontemporal_store(v, (gm_v4u *)(o + (size_t)row * g.N));
+                else *(gm_v4u *)(o + (size_t)row * g.N) = v;
+            }
+        gm_wave_sync();
     }
 }
 
@@ -673,7 +719,6 @@ k_mx_gemm(const MxProduct g)
     t.ldsp = lds;
     const uint8_t *w1 = mx_matrix(g, g.w, e), *w3 = GATED ? mx_matrix(g, g.w3, e) : w1;
     const int rb0 = (WV * ft + t.wave) * RB;
-    const uint32_t row16 = g.nQ * (MX_XQ / 16);
     if (!w1 || !w3) {
         mx_zeros<Y, 64 * WV>(g, p0, np, 16 * WV * RB * ft, 16 * WV * RB);
         return;
@@ -688,23 +733,20 @@ k_mx_gemm(const MxProduct g)
         t.at[r] = second + 16 * row + 256 * hi;
         t.sat[r] = second + 4 * row + 64 * hi;
     }
-    auto source = [&](int r) {
-        const int row = mx_row(g, p0 + min(r, np - 1));
-        return (uint32_t)(row < 0 ? g.T : row) * row16;
-    };
     const int nb = (np + 31) / 32;
 #pragma unroll
     for (int i = 0; i < t.COPIES; ++i) {
         const int r = 4 * (WV * i + t.wave) + (t.lane >> 4);
-        t.x[i] = source(r) + ((t.lane & 15) ^ (r & 15));
+        t.row[i] = mx_pair(g, p0 + min(r, np - 1));
+        t.unit[i] = (t.lane & 15) ^ (r & 15);
     }
-    t.xs = source(64 * t.wave + t.lane) + 16;
+    t.rows = mx_pair(g, p0 + min(64 * t.wave + t.lane, np - 1));
     if constexpr (TM == 128) {
-        if (nb == 4) return mx_gemm_tile<Y, GATED, 4>(g, t, p0, np, rb0);
-        if (nb == 3) return mx_gemm_tile<Y, GATED, 3>(g, t, p0, np, rb0);
+        if (nb == 4) return mx_gemm_tile<Y, GATED, 4>(g, t, lds, p0, np, rb0);
+        if (nb == 3) return mx_gemm_tile<Y, GATED, 3>(g, t, lds, p0, np, rb0);
     }
-    if (nb == 2) return mx_gemm_tile<Y, GATED, 2>(g, t, p0, np, rb0);
-    mx_gemm_tile<Y, GATED, 1>(g, t, p0, np, rb0);
+    if (nb == 2) return mx_gemm_tile<Y, GATED, 2>(g, t, lds, p0, np, rb0);
+    mx_gemm_tile<Y, GATED, 1>(g, t, lds, p0, np, rb0);
 }
 
 /* ------------------------------------------------------------- entry points ---- */
@@ -917,6 +959,7 @@ static int mx_product(const char *who, MxProduct &g, const void *x, int xdt, int
     g.xq = (const uint8_t *)work;
     g.x = x;
     g.cols = cols;
+    g.stream = (size_t)g.P * g.N * (ydt == K3_WBF16 ? 2 : 4) > MX_STREAM;
     const bool bf = ydt == K3_WBF16, gated = g.w3 != nullptr;
     MxPlan plan = mx_plan(g, gated);
     const int64_t blocks = mx_grid(g, plan.tm, plan.rb);
@@ -974,10 +1017,10 @@ extern "C" int k3g_grouped_mxfp4(const void *x, int xdt, int rows, int cols, con
         mx_pointer(who, "off", off, 4, rows > 0) || mx_pointer(who, "perm", perm, 4, false) ||
         mx_pointer(who, "w", w, 8, rows > 0) || mx_pointer(who, "w3", w3, 8, false))
         return -1;
-    if (n_experts < 1 || n_experts > 1024 || topk < 1 || topk > K3G_MAX_TOPK || (!perm && topk != 1) ||
+    if (n_experts < 1 || n_experts > MX_MAX_EXPERTS || topk < 1 || topk > K3G_MAX_TOPK || (!perm && topk != 1) ||
         (int64_t)rows * topk > MX_MAX_PAIRS) {
-        fprintf(stderr, "%s: needs 1 to 1024 experts, 1 <= topk <= %d (1 without perm) and at most %d "
-                        "pairs (%d experts, %d x %d)\n", who, K3G_MAX_TOPK, MX_MAX_PAIRS, n_experts, rows,
+        fprintf(stderr, "%s: needs 1 to %d experts, 1 <= topk <= %d (1 without perm) and at most %d "
+                        "pairs (%d experts, %d x %d)\n", who, MX_MAX_EXPERTS, K3G_MAX_TOPK, MX_MAX_PAIRS, n_experts, rows,
                 topk);
         return -1;
     }
