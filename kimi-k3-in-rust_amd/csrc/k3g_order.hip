@@ -22,7 +22,7 @@
 #define OD_MAX_EXPERTS 1024
 #define OD_MAX_PAIRS (1 << 23)         /* a block of 256 threads each makes fewer than 2^32 */
 #define OD_MAX_WIDTH (1 << 24)
-#define OD_THREADS 512                 /* threads of a sort block */
+#define OD_THREADS 1024                /* threads of a sort block */
 #define OD_WAVES (OD_THREADS / 64)
 #define OD_CHUNKS 128                  /* chunks of a sort at most */
 
@@ -76,7 +76,7 @@ k_order_count(const int32_t *__restrict__ idx, int P, int E, int m, int32_t *__r
  * give where the chunk's first pair of it goes (counts of k_order_count; one chunk needs none),
  * and a block scan of the totals gives where the expert begins.
  * M > 0: m = M, and a thread's experts and ranks stay in registers, every load asked for before
- * the first is used (3,702 pairs in one block 11.4 -> 5.2 us). M = 0: any m; a pair's rank waits in
+ * the first is used (3,702 pairs in one block 11.4 -> 6.0 us, half of it by 16 waves for 8). M = 0: any m; a pair's rank waits in
  * its own entry of pos between the two walks. */
 template <int M>
 __global__ void __launch_bounds__(OD_THREADS)
@@ -194,7 +194,7 @@ k_order_place(const int32_t *__restrict__ idx, int P, int E, int any_m,
 
 /* 16 bytes of a row, whatever the row's alignment (rows of an odd width begin at any element;
  * global loads of 16 bytes take any address). */
-typedef uint32_t od_v4u __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t od_v4u __attribute__((ext_vector_type(4), aligned(2), may_alias));
 
 template <typename T> struct OdRow;
 template <> struct OdRow<float> {
@@ -317,7 +317,7 @@ k_unpermute(const OdGrid g, const T *__restrict__ sorted, const int32_t *__restr
     int t, v;
     if (!od_mine<T, WIDE>(g, t, v)) return;
     const int32_t *pt = pos + (size_t)t * g.k;
-    const float *wrow = wt + (size_t)t * g.k;
+    const float *wrow = wt ? wt + (size_t)t * g.k : nullptr;
     float acc[V], f[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.0f;
@@ -401,14 +401,16 @@ k_unpermute_grad(const OdGrid g, const T *__restrict__ dout, const T *__restrict
 /* ------------------------------------------------------------------ entry points ---- */
 
 /* Chunks of the sort and the multiple m of OD_THREADS pairs that each has. Up to 4096 pairs one
- * block does all; past that a chunk is 2048 or 4096 pairs, or what makes 128 chunks: every chunk
- * reads the counts of all (32,768 pairs in 64 chunks took 9.4 us, in 16 4.4). */
+ * block does all (5,600 in one block 11.0 us, in chunks 7.8); past that a chunk is 2048, 4096 or
+ * 8192 pairs, or what makes 128 chunks: every chunk reads the counts of all, so there are few.
+ * us, on 384 experts: 8 pairs 3.4, 1024 3.8, 4096 7.4, 32,768 8.1, 524,288 18.6. */
 static int sort_chunks(int P, int *m)
 {
-    int per = P <= OD_THREADS ? 1 : P <= 2 * OD_THREADS ? 2 : P <= 4 * OD_THREADS ? 4 : 8;
-    if (P > 8 * OD_THREADS) {
-        if (P <= 32 * 4 * OD_THREADS) per = 4;
-        else if (P > OD_CHUNKS * 8 * OD_THREADS)
+    int per = P <= OD_THREADS ? 1 : P <= 2 * OD_THREADS ? 2 : 4;
+    if (P > 4 * OD_THREADS) {
+        if (P <= 32 * 2 * OD_THREADS) per = 2;
+        else if (P > 32 * 4 * OD_THREADS) per = 8;
+        if (P > OD_CHUNKS * 8 * OD_THREADS)
             per = (P + OD_CHUNKS * OD_THREADS - 1) / (OD_CHUNKS * OD_THREADS);
     }
     *m = per;

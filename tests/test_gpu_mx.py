@@ -7,7 +7,7 @@ import pytest
 
 import k3moe
 import ops64
-from test_gpu_order import DT, Out, dev, floats, routing, rows_of, sort_tokens
+from test_gpu_order import DT, Out, dev, floats, graphs, routing, rows_of, sort_tokens
 
 pytestmark = pytest.mark.gpu
 
@@ -146,7 +146,8 @@ def check(got, want, tol, dt):
 
 MATS = [(1, 32, 16), (1, 7168, 2048), (2, 544, 48), (3, 128, 4096), (4, 2048, 64), (5, 160, 80), (15, 1056, 272),
         (16, 512, 256), (17, 64, 16), (33, 4128, 208), (64, 1024, 512), (65, 2592, 1040), (129, 96, 336),
-        (300, 1536, 640), (513, 576, 528)]
+        (300, 1536, 640), (513, 576, 528), (500, 160, 6144), (512, 672, 7152), (1000, 160, 6096),
+        (2000, 288, 7088)]
 
 
 @pytest.mark.parametrize("rows,cols,n", MATS)
@@ -174,18 +175,18 @@ def test_matmul_infinities(gpu):
     """A row with an infinity or a NaN is NaN, its neighbours are not."""
     print("case: k3g_matmul_mxfp4 with infinities", flush=True)
     L = k3moe.lib()
-    for rows in (3, 40):
+    for rows, n in ((3, 64), (40, 64), (500, 6144)):
         rng = np.random.default_rng(rows)
         x = rng.normal(0, 1, (rows, 1056)).astype(np.float32)
         x[1, 700], x[rows - 1, 1055] = np.inf, np.nan
-        pk, sc, w = matrix(rng, 64, 1056)
+        pk, sc, w = matrix(rng, n, 1056)
         bx, px = dev(x)
-        t = tiled(pk, sc, 64, 1056)
+        t = tiled(pk, sc, n, 1056)
         size = L.k3g_mxfp4_work_bytes(rows, 1056)
-        work, y = Out(np.uint8, size), Out(np.float32, rows * 64)
-        assert L.k3g_matmul_mxfp4(px, 0, rows, 1056, C.c_void_p(t.ptr), 64, y.ptr, 0, work.ptr, size, None) == 0
+        work, y = Out(np.uint8, size), Out(np.float32, rows * n)
+        assert L.k3g_matmul_mxfp4(px, 0, rows, 1056, C.c_void_p(t.ptr), n, y.ptr, 0, work.ptr, size, None) == 0
         k3moe.sync()
-        bad = np.isnan(y.get().reshape(rows, 64))
+        bad = np.isnan(y.get().reshape(rows, n))
         assert bad[1].all() and bad[rows - 1].all()
         bad[[1, rows - 1]] = False
         assert not bad.any()
@@ -217,7 +218,8 @@ def grouped(x, xdt, perm, topk, off, tables, n, ydt, P, caps=(2.0 ** 100, 2.0 **
 
 
 GROUPS = [(1, 8, 16, 512, 64, 0.0), (3, 2, 5, 96, 48, 0.3), (8, 8, 24, 2048, 256, 0.0), (40, 1, 3, 1056, 80, 0.2),
-          (64, 4, 7, 544, 304, 0.0), (100, 16, 40, 64, 16, 0.5), (600, 2, 3, 640, 272, 0.1), (5, 3, 1024, 32, 16, 0.0)]
+          (64, 4, 7, 544, 304, 0.0), (100, 16, 40, 64, 16, 0.5), (600, 2, 3, 640, 272, 0.1), (5, 3, 1024, 32, 16, 0.0),
+          (300, 4, 40, 1056, 1648, 0.1), (1500, 2, 24, 416, 2832, 0.0)]
 
 
 @pytest.mark.parametrize("T,k,E,cols,n,drop", GROUPS)
@@ -306,6 +308,17 @@ def test_grouped_ranges_and_pairs_out_of_range(gpu):
     assert (either[0] | either[1]).all()
 
 
+@pytest.mark.parametrize("T,E,n", [(3, 4, 32), (200, 4, 32), (400, 40, 1648)])
+def test_grouped_without_pairs(gpu, T, E, n):
+    """Every pair dropped: nothing is written."""
+    print(f"case: k3g_grouped_mxfp4 without pairs, {T} tokens", flush=True)
+    rng = np.random.default_rng(T)
+    mats = experts(rng, E, 64, n, 2)
+    x = rng.normal(0, 1, (T, 64)).astype(np.float32)
+    raw = grouped(x, "f32", np.full(2 * T, -1), 2, np.zeros(E + 1, int), [m[1] for m in mats], n, "f32", 2 * T)
+    assert np.all(raw.view(np.uint8) == 0x5A)
+
+
 @pytest.mark.parametrize("T", [2, 70])
 def test_expert_layer_in_four_bits(gpu, T):
     """A run of the operators as a program uses them: sort, gate and up of the tokens, down of the
@@ -352,3 +365,120 @@ def test_expert_layer_in_four_bits(gpu, T):
             want[perm[r] // k] += part
             size[perm[r] // k] += wt[perm[r]] * (np.abs(vals[2][e]) @ np.abs(q))
     assert np.all(np.abs(got - want) <= (inter // 32 + 16 + k + 2) * 2.0 ** -23 * size)
+
+
+@pytest.mark.parametrize("T", [3, 40, 700])
+def test_captured_and_replayed(gpu, T):
+    """Quantisation and the product inside it, gated and not, in a graph on a stream of its own, with
+    new activations before each replay, against eager calls."""
+    import torch
+    print(f"case: captured products, {T} tokens", flush=True)
+    L = k3moe.lib()
+    k, E, cols, n = 2, 6, 1056, 272
+    rng = np.random.default_rng(T)
+    idx = torch.from_numpy(routing(rng, T, k, E, 0.1)).cuda()
+    perm, off, _ = ops64.order(idx.cpu().numpy(), E)
+    P = T * k
+    full = np.full(P, -1, np.int32)
+    full[:perm.size] = perm
+    perm, off = torch.from_numpy(full).cuda(), torch.from_numpy(off.astype(np.int32)).cuda()
+    mats = experts(rng, E, cols, n, 2, 120, 123)
+    tab = [torch.from_numpy(m[1].astype(np.int64)).cuda() for m in mats]
+    x = torch.empty(T, cols, device="cuda").normal_()
+    size = L.k3g_mxfp4_work_bytes(T, cols)
+    work = [torch.empty(size, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    y = [torch.zeros(P, n, device="cuda") for _ in range(2)]
+    z = [torch.zeros(T, n, device="cuda") for _ in range(2)]
+    q = [torch.zeros(T, cols // 2 + cols // 32, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    torch.cuda.synchronize()
+
+    def run(st, i):
+        assert L.k3g_grouped_mxfp4(x.data_ptr(), 0, T, cols, perm.data_ptr(), k, off.data_ptr(), E, tab[0].data_ptr(),
+                                   tab[1].data_ptr(), 8, n, 4.0, 25.0, y[i].data_ptr(), 0, work[i].data_ptr(), size,
+                                   st) == 0
+        assert L.k3g_matmul_mxfp4(x.data_ptr(), 0, T, cols, int(mats[0][1][1]), n, z[i].data_ptr(), 0,
+                                  work[i].data_ptr(), size, st) == 0
+        assert L.k3g_quant_mxfp4(x.data_ptr(), 0, T, cols, q[i].data_ptr(), q[i].data_ptr() + T * cols // 2, st) == 0
+
+    for _ in graphs(lambda st: run(st, 0)):
+        run(None, 1)
+        torch.cuda.synchronize()
+        assert torch.equal(y[0], y[1]) and torch.equal(z[0], z[1]) and torch.equal(q[0], q[1])
+        assert float(z[0].abs().max()) > 0
+        x.normal_()
+        y[0].zero_()
+        z[0].zero_()
+        torch.cuda.synchronize()
+
+
+def test_two_products_at_once(gpu):
+    """Two calls on two streams, each with a workspace of its own, give what they give alone."""
+    import torch
+    print("case: two products at once", flush=True)
+    L = k3moe.lib()
+    rows, cols, n = 600, 2048, 1024
+    rng = np.random.default_rng(0)
+    pk, sc, _ = matrix(rng, n, cols)
+    t = tiled(pk, sc, n, cols)
+    size = L.k3g_mxfp4_work_bytes(rows, cols)
+    x = [torch.randn(rows, cols, device="cuda") for _ in range(2)]
+    y = [torch.empty(rows, n, device="cuda") for _ in range(2)]
+    alone = [torch.empty(rows, n, device="cuda") for _ in range(2)]
+    work = [torch.empty(size, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    st = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert L.k3g_matmul_mxfp4(x[i].data_ptr(), 0, rows, cols, t.ptr, n, alone[i].data_ptr(), 0, work[0].data_ptr(),
+                                  size, None) == 0
+        torch.cuda.synchronize()
+    for _ in range(20):
+        for i in range(2):
+            assert L.k3g_matmul_mxfp4(x[i].data_ptr(), 0, rows, cols, t.ptr, n, y[i].data_ptr(), 0, work[i].data_ptr(),
+                                      size, st[i].cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(y[0], alone[0]) and torch.equal(y[1], alone[1])
+
+
+@pytest.mark.parametrize("rows", [1, 4, 5, 16, 40, 130, 257, 520])
+def test_rows_do_not_meet(gpu, rows):
+    """A row's product is the same bits whatever rows lie beside it in the call."""
+    import torch
+    print(f"case: rows of one call, {rows}", flush=True)
+    L = k3moe.lib()
+    cols, n = 3616, 1616
+    rng = np.random.default_rng(rows)
+    pk, sc, _ = matrix(rng, n, cols)
+    t = tiled(pk, sc, n, cols)
+    x = torch.randn(rows, cols, device="cuda")
+    work = torch.empty(L.k3g_mxfp4_work_bytes(rows, cols), dtype=torch.uint8, device="cuda")
+    y = [torch.empty(rows, n, device="cuda") for _ in range(2)]
+    torch.cuda.synchronize()
+    for i, v in enumerate((x, x.flip(0).contiguous())):
+        assert L.k3g_matmul_mxfp4(v.data_ptr(), 0, rows, cols, t.ptr, n, y[i].data_ptr(), 0, work.data_ptr(),
+                                  work.numel(), None) == 0
+        torch.cuda.synchronize()
+    assert torch.equal(y[0], y[1].flip(0))
+
+
+def test_values_past_32_bits(gpu):
+    """More than 2^32 values quantised and read back: the last rows are the first rows' codes."""
+    import torch
+    print("case: values past 2^32", flush=True)
+    L = k3moe.lib()
+    rows, cols = 70000, 65536
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda")
+    block = torch.randn(100, cols, device="cuda").bfloat16()
+    x.view(700, 100, cols)[:] = block
+    pk = torch.empty(rows, cols // 2, dtype=torch.uint8, device="cuda")
+    sc = torch.empty(rows, cols // 32, dtype=torch.uint8, device="cuda")
+    assert L.k3g_quant_mxfp4(x.data_ptr(), 1, rows, cols, pk.data_ptr(), sc.data_ptr(), None) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(pk[:100], pk[-100:]) and torch.equal(sc[:100], sc[-100:])
+    code, scale = ops64.quant(block[:3].float().cpu().numpy())
+    assert np.array_equal(ops64.unpack(pk[-100:-97].cpu().numpy()), code)
+    assert np.array_equal(sc[-100:-97].cpu().numpy(), scale)
+    x.zero_()
+    assert L.k3g_dequant_mxfp4(pk.data_ptr(), sc.data_ptr(), rows, cols, x.data_ptr(), 1, None) == 0
+    torch.cuda.synchronize()
+    assert np.array_equal(x[-100:-97].float().cpu().numpy(), ops64.values(code, scale))
+    assert torch.equal(x[:100], x[-100:])

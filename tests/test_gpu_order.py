@@ -82,7 +82,8 @@ def sort_tokens(idx, E, want_err=0):
 
 @pytest.mark.parametrize("T,k,E", [(0, 8, 384), (1, 1, 1), (1, 16, 896), (4, 8, 384), (63, 1, 3), (9, 7, 64),
                                    (64, 8, 256), (513, 8, 1024), (511, 8, 1024), (4097, 1, 2),
-                                   (700, 6, 64), (4096, 8, 384), (5000, 64, 64), (70001, 1, 1000)])
+                                   (700, 6, 64), (4096, 8, 384), (5000, 64, 64), (70001, 1, 1000),
+                                   (1025, 1, 40), (2049, 1, 1024), (16385, 8, 300), (131073, 8, 500)])
 @pytest.mark.parametrize("kind", ["all", "dropped", "one expert", "none"])
 def test_sort(gpu, T, k, E, kind):
     print(f"case: k3g_sort_tokens {T} x {k} over {E}, {kind}", flush=True)
@@ -309,3 +310,132 @@ def test_gradients_against_differences(gpu):
         x2[t, i] += 1.0
         assert abs(there_and_back(x2, wt)[1] - base - dx[t, i]) < tol
     assert placed < P
+
+
+def graphs(capture, steps=3):
+    """Captures `capture(stream)` on a stream of its own and replays it with eager work of the
+    program and synchronizations in between; yields after each replay."""
+    import torch
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        capture(st.cuda_stream)
+    st.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st):
+        capture(st.cuda_stream)
+    other = torch.ones(1 << 16, device="cuda")
+    for _ in range(steps):
+        with torch.cuda.stream(st):
+            g.replay()
+        other = other * 1.5 + 1.0
+        st.synchronize()
+        torch.cuda.synchronize()
+        yield
+
+
+@pytest.mark.parametrize("T,k,n,E", [(3, 8, 100, 24), (900, 8, 72, 64)])
+def test_captured_and_replayed(gpu, T, k, n, E):
+    """Sort, rows out, back with weights and every gradient in one graph, on a stream that is not
+    the default one, with new routing, rows and weights before each replay."""
+    import torch
+    print(f"case: a captured run of {T} x {k}", flush=True)
+    L, P = k3moe.lib(), T * k
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(T)
+    dev_ = dict(device="cuda")
+    x, g = torch.empty(T, n, **dev_), torch.empty(T, n, **dev_)
+    idx, wt = torch.empty(T, k, dtype=torch.int32, **dev_), torch.empty(T, k, **dev_)
+
+    def fresh():
+        x.normal_(generator=gen)
+        g.normal_(generator=gen)
+        wt.uniform_(generator=gen)
+        i = torch.topk(torch.rand(T, E, generator=gen, **dev_), k, dim=1).indices.int()
+        idx.copy_(torch.where(torch.rand(T, k, generator=gen, **dev_) < 0.1, -1, i))
+        torch.cuda.synchronize()
+
+    perm, pos = torch.empty(P, dtype=torch.int32, **dev_), torch.empty(P, dtype=torch.int32, **dev_)
+    off = torch.empty(E + 1, dtype=torch.int32, **dev_)
+    nw = L.k3g_sort_bytes(T, k, E)
+    work = torch.empty(max(nw, 1), dtype=torch.uint8, **dev_)
+    s, ds = torch.zeros(P, n, **dev_), torch.zeros(P, n, **dev_)
+    out, dw, dx = torch.empty(T, n, **dev_), torch.empty(P, **dev_), torch.empty(T, n, **dev_)
+
+    def capture(st):
+        assert L.k3g_sort_tokens(idx.data_ptr(), T, k, E, perm.data_ptr(), off.data_ptr(), pos.data_ptr(), None,
+                                 work.data_ptr(), nw, st) == 0
+        assert L.k3g_permute(x.data_ptr(), 0, T, k, n, pos.data_ptr(), s.data_ptr(), st) == 0
+        assert L.k3g_unpermute(s.data_ptr(), 0, T, k, n, pos.data_ptr(), wt.data_ptr(), None, out.data_ptr(), st) == 0
+        assert L.k3g_unpermute_grad(g.data_ptr(), s.data_ptr(), 0, T, k, n, pos.data_ptr(), wt.data_ptr(),
+                                    ds.data_ptr(), dw.data_ptr(), st) == 0
+        assert L.k3g_permute_grad(ds.data_ptr(), 0, T, k, n, pos.data_ptr(), dx.data_ptr(), st) == 0
+
+    fresh()
+    for _ in graphs(capture):
+        kept = idx.cpu().numpy().reshape(-1) >= 0
+        assert np.array_equal(pos.cpu().numpy(), ops64.order(idx.cpu().numpy(), E)[2])
+        w64 = np.where(kept, wt.cpu().numpy().reshape(-1).astype(np.float64), 0.0).reshape(T, k)
+        xn, gn = x.cpu().numpy().astype(np.float64), g.cpu().numpy().astype(np.float64)
+        tol = (2 * k + 4) * 2.0 ** -24
+        assert np.all(np.abs(out.cpu().numpy() - w64.sum(1)[:, None] * xn) <= tol * w64.sum(1)[:, None] * np.abs(xn))
+        assert np.all(np.abs(dx.cpu().numpy() - w64.sum(1)[:, None] * gn) <= tol * w64.sum(1)[:, None] * np.abs(gn))
+        dots = np.where(kept.reshape(T, k), (xn * gn).sum(1)[:, None], 0.0)
+        assert np.all(np.abs(dw.cpu().numpy().reshape(T, k) - dots) <= (n + 1) * 2.0 ** -24 * np.abs(xn * gn).sum(1)[:, None])
+        fresh()
+
+
+def test_two_sorts_at_once(gpu):
+    """Two calls on two streams, each with a workspace of its own, do not meet."""
+    import torch
+    print("case: two sorts at once", flush=True)
+    L = k3moe.lib()
+    T, k, E = 6000, 8, 200
+    st = [torch.cuda.Stream(), torch.cuda.Stream()]
+    runs = []
+    for i in range(2):
+        idx = torch.from_numpy(routing(np.random.default_rng(i), T, k, E, 0.1)).cuda()
+        perm, pos = (torch.empty(T * k, dtype=torch.int32, device="cuda") for _ in range(2))
+        off = torch.empty(E + 1, dtype=torch.int32, device="cuda")
+        work = torch.empty(L.k3g_sort_bytes(T, k, E), dtype=torch.uint8, device="cuda")
+        runs.append((idx, perm, off, pos, work))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for (idx, perm, off, pos, work), s in zip(runs, st):
+            assert L.k3g_sort_tokens(idx.data_ptr(), T, k, E, perm.data_ptr(), off.data_ptr(), pos.data_ptr(), None,
+                                     work.data_ptr(), work.numel(), s.cuda_stream) == 0
+    torch.cuda.synchronize()
+    for idx, perm, off, pos, _ in runs:
+        wp, wo, wpos = ops64.order(idx.cpu().numpy(), E)
+        assert np.array_equal(off.cpu().numpy(), wo) and np.array_equal(pos.cpu().numpy(), wpos)
+        assert np.array_equal(perm.cpu().numpy()[:wp.size], wp)
+
+
+def test_rows_past_32_bits(gpu):
+    """Sorted rows of more than 2^32 elements (and 8 GB): the last ones go out and come back."""
+    import torch
+    print("case: sorted rows past 2^32 elements", flush=True)
+    T, k, n = 33000, 2, 65600
+    L, P = k3moe.lib(), T * k
+    assert P * n > 1 << 32
+    pos = torch.arange(P, dtype=torch.int32, device="cuda").flip(0).contiguous()
+    x = (torch.arange(T, device="cuda", dtype=torch.int32) % 251).to(torch.bfloat16).unsqueeze(1).expand(T, n).contiguous()
+    x[:, -1] = 3.0
+    s = torch.empty(P, n, dtype=torch.bfloat16, device="cuda")
+    wt = torch.full((P,), 0.5, device="cuda")
+    assert L.k3g_permute(x.data_ptr(), 1, T, k, n, pos.data_ptr(), s.data_ptr(), None) == 0
+    torch.cuda.synchronize()
+    for r in (0, 1, P // 2, P - 2, P - 1):
+        assert torch.equal(s[r], x[(P - 1 - r) // k])
+    out = torch.empty_like(x)
+    assert L.k3g_unpermute(s.data_ptr(), 1, T, k, n, pos.data_ptr(), wt.data_ptr(), None, out.data_ptr(), None) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(out, x)                  # two halves of the same value
+    dw = torch.empty(P, device="cuda")
+    out.fill_(1.0)
+    assert L.k3g_unpermute_grad(out.data_ptr(), s.data_ptr(), 1, T, k, n, pos.data_ptr(), wt.data_ptr(), s.data_ptr(),
+                                None, None) == 0
+    assert L.k3g_unpermute_grad(out.data_ptr(), x.data_ptr(), 1, 1, 1, n, pos[P - 1:].data_ptr(), None, None,
+                                dw.data_ptr(), None) == 0
+    torch.cuda.synchronize()
+    assert bool((s[0] == 0.5).all()) and bool((s[P - 1] == 0.5).all()) and bool((s[P // 2] == 0.5).all())
+    assert float(dw[0]) == 3.0                  # token 0's row is zeros but for its last element
