@@ -351,51 +351,73 @@ k_unpermute(const OdGrid g, const T *__restrict__ sorted, const int32_t *__restr
     od_store(out + (size_t)t * g.n, v, g.n, OdRow<T>::put(acc));
 }
 
-/* WV waves per pair (a block of four): its row of dsorted and its entry of dwt, the pairs of a
- * token on one XCD (block b runs on XCD b % 8), whose L2 then serves the token's dout. */
-template <typename T, int WV, bool STREAM>
+/* WV waves (a block of four) per JB slots of a token: their rows of dsorted and entries of dwt from
+ * one read of dout; a token's slots on one XCD (block b runs on XCD b % 8), whose L2 then serves
+ * dout to the next ones. */
+template <typename T, int WV, int JB, bool STREAM>
 __global__ void __launch_bounds__(256)
 k_unpermute_grad(const OdGrid g, const T *__restrict__ dout, const T *__restrict__ sorted,
                  const int32_t *__restrict__ pos, const float *__restrict__ wt,
                  T *__restrict__ dsorted, float *__restrict__ dwt)
 {
     constexpr int V = OdRow<T>::V, PER = 4 / WV;
-    __shared__ float part[4];
+    __shared__ float part[JB][4];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & (64 * WV - 1);
-    const int xcd = blockIdx.x & 7, s = (blockIdx.x >> 3) * PER + wave / WV;
-    const int t = 8 * (s / g.k) + xcd, j = s % g.k;
+    const int xcd = blockIdx.x & 7, s = (blockIdx.x >> 3) * PER + wave / WV, ng = (g.k + JB - 1) / JB;
+    const int t = 8 * (s / ng) + xcd, j0 = s % ng * JB;
     if (t >= g.T) return;
-    const size_t pair = (size_t)t * g.k + j;
-    const int p = pos[pair];
-    if ((unsigned)p >= (unsigned)g.P) {
-        if (dwt && lane == 0) dwt[pair] = 0.0f;
-        return;
+    const size_t pair = (size_t)t * g.k + j0;
+    int p[JB];
+    float w[JB], sum[JB];
+#pragma unroll
+    for (int i = 0; i < JB; ++i) {
+        p[i] = j0 + i < g.k ? pos[pair + i] : -1;
+        if ((unsigned)p[i] >= (unsigned)g.P) p[i] = -1;
+        w[i] = dsorted && p[i] >= 0 ? wt[pair + i] : 0.0f;
+        sum[i] = 0.0f;
     }
-    const float w = dsorted ? wt[pair] : 0.0f;
-    float sum = 0.0f;
     for (int v = lane; V * v < g.n; v += 64 * WV) {
         float go[V], f[V];
-        OdRow<T>::get(od_load(dout + (size_t)t * g.n, v, g.n), go);
+        od_v4u u[JB];
+        const od_v4u d = od_load(dout + (size_t)t * g.n, v, g.n);
         if (dwt) {
-            OdRow<T>::get(od_load<STREAM>(sorted + (size_t)p * g.n, v, g.n), f);
 #pragma unroll
-            for (int i = 0; i < V; ++i) sum += f[i] * go[i];
+            for (int i = 0; i < JB; ++i)
+                if (p[i] >= 0) u[i] = od_load<STREAM>(sorted + (size_t)p[i] * g.n, v, g.n);
         }
-        if (dsorted) {
+        OdRow<T>::get(d, go);
 #pragma unroll
-            for (int i = 0; i < V; ++i) f[i] = w * go[i];
-            od_store<STREAM>(dsorted + (size_t)p * g.n, v, g.n, OdRow<T>::put(f));
+        for (int i = 0; i < JB; ++i) {
+            if (p[i] < 0) continue;
+            if (dwt) {
+                OdRow<T>::get(u[i], f);
+#pragma unroll
+                for (int e = 0; e < V; ++e) sum[i] += f[e] * go[e];
+            }
+            if (dsorted) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) f[e] = w[i] * go[e];
+                od_store<STREAM>(dsorted + (size_t)p[i] * g.n, v, g.n, OdRow<T>::put(f));
+            }
         }
     }
     if (!dwt) return;
-    sum = k3d_wave_sum(sum);
+#pragma unroll
+    for (int i = 0; i < JB; ++i) sum[i] = k3d_wave_sum(sum[i]);
     if (WV == 1) {
-        if (lane == 0) dwt[pair] = sum;
+#pragma unroll
+        for (int i = 0; i < JB; ++i)
+            if (lane == 0 && j0 + i < g.k) dwt[pair + i] = sum[i];
         return;
     }
-    if ((threadIdx.x & 63) == 0) part[wave] = sum;
+#pragma unroll
+    for (int i = 0; i < JB; ++i)
+        if ((threadIdx.x & 63) == 0) part[i][wave] = sum[i];
     __syncthreads();
-    if (threadIdx.x == 0) dwt[pair] = part[0] + part[1] + part[2] + part[3];
+    if (threadIdx.x < JB && j0 + (int)threadIdx.x < g.k) {
+        const float *q = part[threadIdx.x];
+        dwt[pair + threadIdx.x] = q[0] + q[1] + q[2] + q[3];
+    }
 }
 
 /* ------------------------------------------------------------------ entry points ---- */
@@ -601,19 +623,20 @@ extern "C" int k3g_unpermute_grad(const void *dout, const void *sorted, int dt, 
     K3hOn on(stream);
     if (!on.ok) return -1;
     const OdGrid g = {T, topk, n, T * topk, 0};
-    /* short rows: a wave each */
-    const bool wave = n <= 128 * (16 / size);
-    const int64_t slots = (int64_t)((T + 7) / 8) * topk;
+    /* Short rows: a wave each. Four slots together where the rows are bf16 and make enough blocks all
+     * the same: us, 3,978 x 15 rows of 535 41.8 -> 35.5, 4,096 x 8 of 2048 57 -> 45, of 64 9.9 -> 7.3,
+     * of 7168 190 -> 189; fp32 rows, whose loads are twice as many, lose (4,096 x 8 of 256 14.0 ->
+     * 17.4, 2,000 x 16 of 3584 185 -> 238). */
+    const bool wave = n <= 128 * (16 / size), four = size == 2 && g.P >= 4096 && topk >= 3;
+    const int64_t slots = (int64_t)((T + 7) / 8) * (four ? (topk + 3) / 4 : topk);
     const dim3 grid((unsigned)(8 * (wave ? (slots + 3) / 4 : slots)));
     const bool big = (size_t)g.P * n * size > OD_STREAM;
-    if (dt == K3_WBF16) {
-        auto *k = big ? (wave ? k_unpermute_grad<uint16_t, 1, true> : k_unpermute_grad<uint16_t, 4, true>)
-                         : (wave ? k_unpermute_grad<uint16_t, 1, false> : k_unpermute_grad<uint16_t, 4, false>);
-        return k3h_launch(who, k, grid, dim3(256), on.st, g, (const uint16_t *)dout, (const uint16_t *)sorted,
-                          pos, wt, (uint16_t *)dsorted, dwt);
-    }
-    auto *k = big ? (wave ? k_unpermute_grad<float, 1, true> : k_unpermute_grad<float, 4, true>)
-                     : (wave ? k_unpermute_grad<float, 1, false> : k_unpermute_grad<float, 4, false>);
-    return k3h_launch(who, k, grid, dim3(256), on.st, g, (const float *)dout, (const float *)sorted, pos, wt,
-                      (float *)dsorted, dwt);
+#define OD_GRAD(T, JB)                                                                                   \
+    (big ? (wave ? k_unpermute_grad<T, 1, JB, true> : k_unpermute_grad<T, 4, JB, true>)                  \
+         : (wave ? k_unpermute_grad<T, 1, JB, false> : k_unpermute_grad<T, 4, JB, false>))
+    if (dt == K3_WBF16)
+        return k3h_launch(who, four ? OD_GRAD(uint16_t, 4) : OD_GRAD(uint16_t, 1), grid, dim3(256), on.st, g,
+                          (const uint16_t *)dout, (const uint16_t *)sorted, pos, wt, (uint16_t *)dsorted, dwt);
+    return k3h_launch(who, OD_GRAD(float, 1), grid, dim3(256), on.st, g, (const float *)dout,
+                      (const float *)sorted, pos, wt, (float *)dsorted, dwt);
 }

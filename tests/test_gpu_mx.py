@@ -253,8 +253,9 @@ def test_grouped(gpu, T, k, E, cols, n, drop, kind, dt):
             u, (_, tu) = a @ mats[1][2][e].T, bound(a, mats[1][2][e])
             g, tg = want, tol
             want = activation(g, u, *caps)
-            # |d act / d gate| <= 1.25 |up|, |act| <= |gate| |up|; the activation's own float
-            # operations, ten at most, are off by 2^-24 each, tanh and exp of them by 2^-23
+            # |d act / d gate| <= 1.25 |up|, |act| <= |gate| |up|; the activation itself, in fp32, has
+            # two tanh (5 roundings of 2^-24 each in all), a sigmoid (5) and 5 products and quotients:
+            # 20 of the 32 that 2^-19 is
             tol = 1.25 * tg * (np.abs(u) + tu) + np.abs(g) * tu + 2.0 ** -19 * np.abs(want)
         check(got[r], want, tol, dt)
 
@@ -482,3 +483,28 @@ def test_values_past_32_bits(gpu):
     torch.cuda.synchronize()
     assert np.array_equal(x[-100:-97].float().cpu().numpy(), ops64.values(code, scale))
     assert torch.equal(x[:100], x[-100:])
+
+
+@pytest.mark.parametrize("caps", [(2.0 ** 100, 2.0 ** 100), (4.0, 25.0), (0.5, 2.0 ** 100), (2.0 ** 100, 3.0)])
+def test_activation(gpu, caps):
+    """The gated epilogue over gates and ups from far below to far above the caps: one column, so a
+    row's gate and up are known exactly."""
+    print(f"case: the gated product's activation, caps {caps}", flush=True)
+    n = 16
+    # x: one code a row and scale, gate weights 1, up weights -1 to 1.5 in code steps
+    mags = np.array([0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
+    col = np.concatenate([s * mags * 2.0 ** e for e in range(-30, 4) for s in (1.0, -1.0)])
+    x = np.zeros((col.size, 32), np.float32)
+    x[:, 0] = col
+    gate, up = np.zeros((n, 32), np.uint8), np.zeros((n, 32), np.uint8)
+    gate[:, 0] = 2                                  # 1.0
+    up[:, 0] = np.arange(16)
+    one = np.full((n, 1), 127, np.uint8)
+    L = k3moe.lib()
+    bufs = [tiled(ops64.pack(c), one, n, 32) for c in (gate, up)]
+    tab = [np.array([b.ptr], np.uint64) for b in bufs]
+    for rows in (2, col.size):
+        raw = grouped(x[-rows:], "f32", np.arange(rows), 1, np.array([0, rows]), tab, n, "f32", rows, caps)
+        g, u = col[-rows:, None] * np.ones(n), col[-rows:, None] * ops64.values(up, one)[:, 0]
+        want = activation(g, u, *caps)
+        assert np.all(np.abs(raw - want) <= 2.0 ** -19 * np.abs(want) + 2.0 ** -149), np.abs(raw / want - 1).max()
