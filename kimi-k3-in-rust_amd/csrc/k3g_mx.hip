@@ -34,14 +34,10 @@ typedef int mx_v8i __attribute__((ext_vector_type(8)));
 
 /* ------------------------------------------------------------- quantisation ---- */
 
-/* 8 consecutive values of a row. STREAM: not to be kept in the caches, for values that are more than
- * the 256 MB of the last-level cache holds (MX_STREAM; 32768 x 7168 bf16 values there and back 221 ->
- * 178 us). */
+/* 16 bytes of values. STREAM: not to be kept in the caches, for values
+ * that are more than the 256 MB of the last-level cache holds (MX_STREAM; 32768 x 7168 bf16 values
+ * there and back 221 -> 178 us). */
 #define MX_STREAM ((size_t)256 << 20)
-
-struct Mx8 {
-    float f[8];
-};
 
 template <bool STREAM>
 __device__ __forceinline__ gm_v4u mx_get(const void *p)
@@ -49,104 +45,110 @@ __device__ __forceinline__ gm_v4u mx_get(const void *p)
     return STREAM ? __builtin_nontemporal_load((const gm_v4u *)p) : *(const gm_v4u *)p;
 }
 
-template <bool STREAM>
-__device__ __forceinline__ void mx_set(void *p, const gm_v4u &v)
+__device__ __forceinline__ void mx_values(const gm_v4u &u, float (&f)[4])
 {
-    if (STREAM) __builtin_nontemporal_store(v, (gm_v4u *)p);
-    else *(gm_v4u *)p = v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(u[i]);
 }
 
-template <bool STREAM = false>
-__device__ __forceinline__ Mx8 mx_load8(const float *p)
+__device__ __forceinline__ void mx_values(const gm_v4u &u, float (&f)[8])
 {
-    const gm_v4u a = mx_get<STREAM>(p), b = mx_get<STREAM>(p + 4);
-    return {{__uint_as_float(a[0]), __uint_as_float(a[1]), __uint_as_float(a[2]), __uint_as_float(a[3]),
-             __uint_as_float(b[0]), __uint_as_float(b[1]), __uint_as_float(b[2]), __uint_as_float(b[3])}};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[2 * i] = k3d_bf16lo(u[i]);
+        f[2 * i + 1] = k3d_bf16hi(u[i]);
+    }
 }
 
-template <bool STREAM = false>
-__device__ __forceinline__ Mx8 mx_load8(const uint16_t *p)
+/* This lane's V values of a block that it shares with the 32 / V lanes around it: their codes,
+ * element i in nibble i, and the block's scale byte. Magnitudes are compared as bits, so a NaN is
+ * the largest of all. x / 2^E is a multiplication by 2^-E, exact down to 2^-126. */
+template <int V>
+__device__ __forceinline__ uint32_t mx_quant(const float (&x)[V], uint32_t &scale)
 {
-    const gm_v4u a = mx_get<STREAM>(p);
-    return {{k3d_bf16lo(a[0]), k3d_bf16hi(a[0]), k3d_bf16lo(a[1]), k3d_bf16hi(a[1]), k3d_bf16lo(a[2]),
-             k3d_bf16hi(a[2]), k3d_bf16lo(a[3]), k3d_bf16hi(a[3])}};
-}
-
-/* The largest of a value over the four lanes of a quad of lanes */
-__device__ __forceinline__ uint32_t mx_quad_max(uint32_t v)
-{
-    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));
-    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));
-}
-
-/* This lane's 8 values of a block that it shares with the three other lanes of its quad: their
- * codes, element i in nibble i, and the block's scale byte. Magnitudes are compared as bits, so
- * a NaN is the largest of all. x / 2^E is a multiplication by 2^-E, exact down to 2^-126. */
-__device__ __forceinline__ uint32_t mx_quant8(const Mx8 &x, uint32_t &scale)
-{
+    static_assert(V == 4 || V == 8, "lanes of a block");
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x.f[i]) & 0x7FFFFFFFu);
-    m = mx_quad_max(m);
+    for (int i = 0; i < V; ++i) m = max(m, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+    /* of the four lanes of a quad, then, where eight lanes share a block, of its other quad */
+    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xF, 0xF, true));
+    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xF, 0xF, true));
+    if (V == 4) m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xF, 0xF, true));
     const bool finite = m < 0x7F800000u;
     const uint32_t byte = finite ? (uint32_t)max((int)(m >> 23) - 2, 0) : 127u;
     const float inv = __uint_as_float((254u - byte) << 23);
     uint32_t c = 0;
-    float v[8];
+    float v[V];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __builtin_amdgcn_fmed3f(x.f[i] * inv, -6.0f, 6.0f);
+    for (int i = 0; i < V; ++i) v[i] = __builtin_amdgcn_fmed3f(x[i] * inv, -6.0f, 6.0f);
     c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[0], v[1], 1.0f, 0);
     c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2], v[3], 1.0f, 1);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[4], v[5], 1.0f, 2);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6], v[7], 1.0f, 3);
+    if constexpr (V == 8) {
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[4], v[5], 1.0f, 2);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6], v[7], 1.0f, 3);
+    }
     scale = finite ? byte : 255u;
     return finite ? c : 0u;
 }
 
-/* Four lanes per block, 8 values a lane: loads of 16 bytes a lane and stores of 4, each row of
- * whole blocks. */
+/* A lane takes 16 bytes of values, 8 of bf16 (four lanes a block) or 4 of fp32 (eight), so loads and
+ * stores of a wave are whole lines (fp32 with 8 values a lane, every other 16 bytes at a time, 21127 x
+ * 5248 values there and back 259 -> 154 us). */
 template <typename T, bool STREAM>
 __global__ void __launch_bounds__(256)
-k_mx_quant(const T *__restrict__ x, size_t n8, uint8_t *__restrict__ packed,
+k_mx_quant(const T *__restrict__ x, size_t n, uint8_t *__restrict__ packed,
            uint8_t *__restrict__ scales)
 {
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n8; i += (size_t)gridDim.x * 256) {
+    constexpr int V = 16 / sizeof(T), LANES = 32 / V;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
+        float f[V];
+        mx_values(mx_get<STREAM>(x + V * i), f);
         uint32_t s;
-        *(uint32_t *)(packed + 4 * i) = mx_quant8(mx_load8<STREAM>(x + 8 * i), s);
-        if ((i & 3) == 0) scales[i >> 2] = (uint8_t)s;
+        const uint32_t c = mx_quant(f, s);
+        if (V == 8) *(uint32_t *)(packed + 4 * i) = c;
+        else *(uint16_t *)(packed + 2 * i) = (uint16_t)c;
+        if (i % LANES == 0) scales[i / LANES] = (uint8_t)s;
     }
-}
-
-template <bool STREAM>
-__device__ __forceinline__ void mx_store8(float *p, const float *f)
-{
-    mx_set<STREAM>(p, gm_v4u{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
-                             __float_as_uint(f[3])});
-    mx_set<STREAM>(p + 4, gm_v4u{__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]),
-                                 __float_as_uint(f[7])});
-}
-
-template <bool STREAM>
-__device__ __forceinline__ void mx_store8(uint16_t *p, const float *f)
-{
-    mx_set<STREAM>(p, gm_v4u{k3d_bf16x2(f[0], f[1]), k3d_bf16x2(f[2], f[3]), k3d_bf16x2(f[4], f[5]),
-                             k3d_bf16x2(f[6], f[7])});
 }
 
 template <typename T, bool STREAM>
 __global__ void __launch_bounds__(256)
-k_mx_dequant(const uint8_t *__restrict__ packed, const uint8_t *__restrict__ scales, size_t n8,
+k_mx_dequant(const uint8_t *__restrict__ packed, const uint8_t *__restrict__ scales, size_t n,
              T *__restrict__ out)
 {
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n8; i += (size_t)gridDim.x * 256) {
-        const uint32_t b = scales[i >> 2];
+    constexpr int V = 16 / sizeof(T), LANES = 32 / V;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
+        const uint32_t b = scales[i / LANES];
+        const uint32_t c = V == 8 ? *(const uint32_t *)(packed + 4 * i) : *(const uint16_t *)(packed + 2 * i);
         const float s = b == 255u ? __builtin_nanf("") : k3d_e8m0(b);
         float f[8];
-        k3d_fp4x8(*(const uint32_t *)(packed + 4 * i), 1.0f, f);
+        k3d_fp4x8(c, 1.0f, f);
+        gm_v4u u;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] *= s;
-        mx_store8<STREAM>(out + 8 * i, f);
+        for (int j = 0; j < 4; ++j)
+            u[j] = V == 8 ? k3d_bf16x2(f[2 * j] * s, f[2 * j + 1] * s) : __float_as_uint(f[j] * s);
+        gm_v4u *o = (gm_v4u *)(out + V * i);
+        if (STREAM) __builtin_nontemporal_store(u, o);
+        else *o = u;
     }
+}
+
+/* 8 consecutive values */
+struct Mx8 {
+    float f[8];
+};
+
+__device__ __forceinline__ Mx8 mx_load8(const float *p)
+{
+    const float4 a = *(const float4 *)p, b = *(const float4 *)(p + 4);
+    return {{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+}
+
+__device__ __forceinline__ Mx8 mx_load8(const uint16_t *p)
+{
+    Mx8 v;
+    mx_values(*(const gm_v4u *)p, v.f);
+    return v;
 }
 
 /* x as activation quads (see the top), a wave per quad, and a row of zeros behind them */
@@ -163,7 +165,7 @@ k_mx_x(const T *__restrict__ x, size_t nquads, int nQ, int cols, uint8_t *__rest
     if (col < cols && quad < nquads) v = mx_load8(x + row * cols + col);
     uint32_t s;
     uint8_t *o = xq + quad * MX_XQ;
-    *(uint32_t *)(o + 4 * lane) = mx_quant8(v, s);
+    *(uint32_t *)(o + 4 * lane) = mx_quant(v.f, s);
     const int b = lane >> 2;
     if ((lane & 3) == 0) o[256 + 4 * (b & 3) + (b >> 2)] = (uint8_t)s;
 }
@@ -418,7 +420,7 @@ __device__ __forceinline__ void mx_few_sums(const MxProduct &g, const MxFew<X, U
                 Mx8 v = {{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}};
                 if (col < cols && row >= 0) v = mx_load8(t.row + (size_t)row * cols + col);
                 uint32_t s;
-                const uint32_t code = mx_quant8(v, s);
+                const uint32_t code = mx_quant(v.f, s);
                 *(uint32_t *)(t.lds + 256 * r + 16 * (blk ^ r) + 4 * (t.lane & 3)) = code;
                 if ((t.lane & 3) == 0) t.lds[4096 + 16 * r + 4 * (blk & 3) + (blk >> 2)] = (uint8_t)s;
             }
@@ -826,13 +828,13 @@ extern "C" int k3g_quant_mxfp4(const void *x, int dt, int rows, int cols, void *
     if (!rows) return 0;
     K3hOn on(stream);
     if (!on.ok) return -1;
-    const size_t n8 = (size_t)rows * cols / 8;
-    const dim3 grid((unsigned)min((n8 + 255) / 256, (size_t)MX_MAX_BLOCKS));
-    const bool big = n8 * (dt == K3_WBF16 ? 16 : 32) > MX_STREAM;
+    const size_t n = (size_t)rows * cols / (dt == K3_WBF16 ? 8 : 4);
+    const dim3 grid((unsigned)min((n + 255) / 256, (size_t)MX_MAX_BLOCKS));
+    const bool big = 16 * n > MX_STREAM;
     if (dt == K3_WBF16)
-        return k3h_launch(who, big ? k_mx_quant<uint16_t, true> : k_mx_quant<uint16_t, false>, grid, dim3(256), on.st, (const uint16_t *)x, n8,
+        return k3h_launch(who, big ? k_mx_quant<uint16_t, true> : k_mx_quant<uint16_t, false>, grid, dim3(256), on.st, (const uint16_t *)x, n,
                           (uint8_t *)packed, (uint8_t *)scales);
-    return k3h_launch(who, big ? k_mx_quant<float, true> : k_mx_quant<float, false>, grid, dim3(256), on.st, (const float *)x, n8,
+    return k3h_launch(who, big ? k_mx_quant<float, true> : k_mx_quant<float, false>, grid, dim3(256), on.st, (const float *)x, n,
                       (uint8_t *)packed, (uint8_t *)scales);
 }
 
@@ -846,14 +848,14 @@ extern "C" int k3g_dequant_mxfp4(const void *packed, const void *scales, int row
     if (!rows) return 0;
     K3hOn on(stream);
     if (!on.ok) return -1;
-    const size_t n8 = (size_t)rows * cols / 8;
-    const dim3 grid((unsigned)min((n8 + 255) / 256, (size_t)MX_MAX_BLOCKS));
-    const bool big = n8 * (dt == K3_WBF16 ? 16 : 32) > MX_STREAM;
+    const size_t n = (size_t)rows * cols / (dt == K3_WBF16 ? 8 : 4);
+    const dim3 grid((unsigned)min((n + 255) / 256, (size_t)MX_MAX_BLOCKS));
+    const bool big = 16 * n > MX_STREAM;
     if (dt == K3_WBF16)
         return k3h_launch(who, big ? k_mx_dequant<uint16_t, true> : k_mx_dequant<uint16_t, false>, grid, dim3(256), on.st, (const uint8_t *)packed,
-                          (const uint8_t *)scales, n8, (uint16_t *)out);
+                          (const uint8_t *)scales, n, (uint16_t *)out);
     return k3h_launch(who, big ? k_mx_dequant<float, true> : k_mx_dequant<float, false>, grid, dim3(256), on.st, (const uint8_t *)packed,
-                      (const uint8_t *)scales, n8, (float *)out);
+                      (const uint8_t *)scales, n, (float *)out);
 }
 
 extern "C" size_t k3g_mxfp4_work_bytes(int rows, int cols)
