@@ -7,13 +7,21 @@
  * to nearest even, what exceeds 6 as 6. Only exponents are read, so nothing here is rounded but
  * the codes. A block with an infinity or NaN gets scale byte 255: it is NaN as a whole.
  *
- * Product: y[r][i] = sum_k q(x)[row(r)][k] W[i][k], both sides in MXFP4, on
- * v_mfma_scale_f32_16x16x128_f8f6f4 with FP4 operands, fp32 accumulation. The A operand is the
- * tiled layout's 1 KB chunk as it lies (lane L: row L % 16, block L / 16 of the 128 columns, its
+ * Product: y[r][i] = sum_k q(x)[row(r)][k] W[i][k], both sides in MXFP4, on the scaled matrix
+ * instructions with FP4 operands, fp32 accumulation: v_mfma_scale_f32_16x16x128_f8f6f4 for few rows
+ * (k_mx_few), v_mfma_scale_f32_32x32x64_f8f6f4 for many (k_mx_gemm). Of the first, the A operand is
+ * the tiled layout's 1 KB chunk as it lies (lane L: row L % 16, block L / 16 of the 128 columns, its
  * scale byte with it); the B operand is the same of 16 activation rows. A row of activations is
  * stored for that as quads of 512 columns, 272 bytes: 16 blocks of 16 bytes in column order,
  * then 16 scale bytes, block 4 j + q at 4 q + j, so lane (row, q) gets the scales of its four
- * chunks j in one dword; columns past the last are zero. */
+ * chunks j in one dword; columns past the last are zero.
+ *
+ * What bounds them, and what they reach (one MI355X; a large copy moves 4.7 TB/s, read and written):
+ * with few rows an expert the stream of the weights, 5.5 to 5.9 TB/s; with many the matrix cores, 3.0
+ * to 3.5 PFLOP/s (8192 rows by 7168 x 7168 in 238 us: 50 % busy at about 2.1 GHz; on the same data the
+ * matrix instructions alone would take 1.28 of the 1.93 us that a workgroup's 512 columns take, with
+ * the operands' reads from LDS 1.47, with the weights' loads 1.69); there and back, memory, 6.5 TB/s
+ * (32768 x 7168 bf16 values, 178 us). */
 #include <stdio.h>
 
 #include "k3g_dev.h"
@@ -34,9 +42,8 @@ typedef int mx_v8i __attribute__((ext_vector_type(8)));
 
 /* ------------------------------------------------------------- quantisation ---- */
 
-/* 16 bytes of values. STREAM: not to be kept in the caches, for values
- * that are more than the 256 MB of the last-level cache holds (MX_STREAM; 32768 x 7168 bf16 values
- * there and back 221 -> 178 us). */
+/* 16 bytes of values. STREAM: not to be kept in the caches, for values that are more than the
+ * last-level cache's 256 MB (MX_STREAM; 32768 x 7168 bf16 values there and back 221 -> 178 us). */
 #define MX_STREAM ((size_t)256 << 20)
 
 template <bool STREAM>
@@ -189,8 +196,7 @@ struct MxProduct {
 };
 
 /* Row tile `item` of up to TM places: expert, first place and count; false past the last. Every
- * wave finds it by itself: a lane takes up to 16 experts, all their ranges asked for at once (one
- * after the other they were 3 us of a workgroup's time), a wave scan of the lanes' tile counts
+ * wave finds it by itself: a lane takes up to 16 experts, all their ranges asked for at once, a wave scan of the lanes' tile counts
  * finds the lane that has it. The ranges are clamped to the places there are, whatever off holds. */
 template <int TM>
 __device__ __forceinline__ bool mx_tile(const MxProduct &g, int item, int &e, int &p0, int &np)
@@ -315,7 +321,8 @@ __device__ __forceinline__ bool mx_item(const MxProduct &g, int nft, int &ft, in
  * 4,088 by 21 27 of 66; here exp is v_exp_f32 with the rounding of its argument put back, every
  * reciprocal has a Newton step, and tanh is the fifth convergent of Lambert's continued fraction up
  * to 1 (with its roundings 2.8e-7 off at most), 1 - 2 / (1 + e^2x) past it: at most 10 units of the
- * last place in all, and a sigmoid is at least 2^-126. A cap of 2^64 or more is none. */
+ * last place in all. A sigmoid from a gate of -87 down (below 2^-125) is 0, so a gate of minus
+ * infinity without a cap is NaN, as the layer has it. A cap of 2^64 or more is none. */
 __device__ __forceinline__ float mx_rcp(float d)
 {
     const float y = __builtin_amdgcn_rcpf(d);
@@ -342,7 +349,7 @@ __device__ __forceinline__ float mx_tanh(float x)
 
 __device__ __forceinline__ float mx_act(const MxProduct &g, float gate, float up)
 {
-    const float s = mx_rcp(1.0f + mx_exp(-gate));
+    const float s = gate <= -87.0f ? 0.0f : mx_rcp(1.0f + mx_exp(-gate));
     const float a = g.b1 >= 0x1p64f ? gate : g.b1 * mx_tanh(gate * g.i1);
     const float u = g.b2 >= 0x1p64f ? up : g.b2 * mx_tanh(up * g.i2);
     return a * s * u;
@@ -898,12 +905,16 @@ static int64_t mx_grid(const MxProduct &g, int tm, int rb)
  * Up to four rows are quantised inside (1 row 5.5 against 7.2, 4 rows 7.6 and 7.7, 8 rows 10.8 and
  * 7.5).
  *
- * Experts: a few tokens meet about one row an expert, and the weights are all there is to wait for
- * (8 tokens x 8 by 384 experts of 7168 -> 2 x 2048: inside 138, before 139, k_mx_gemm 150; 1 token:
- * 22.6, 24.7, 26.1); where 16 tokens meet 8 experts quantising inside costs 16.8 against 11.9. 64
- * tokens x 2 by 8 experts of 4096 -> 2 x 1408: 4 x 4 by 16 rows 15.1, k_mx_gemm 19.5; 256: 25.6, by
- * 32 24.9, k_mx_gemm by 64 27.6; 1024: 53.9, k_mx_gemm by 64 40.5, by 128 51.9; 4096 x 8 by 384 of
- * 2048 -> 7168: k_mx_gemm by 64 815, by 128 741. */
+ * Experts: a few tokens meet about one row an expert, and the weights are all there is to wait for.
+ * us, bf16: quantised inside, before by 16 places, by 32, k_mx_gemm by 64, by 128:
+ *   1 token x 8 by 384 of 7168 -> 2 x 2048     21.9  23.9  24.0  24.7  24.9
+ *   8 tokens x 8                               133   131   131   141   141
+ *   16 x 8 by 8 of 4096 -> 2 x 1408            27.7  14.4  14.9  15.9  16.0
+ *   64 x 2                                     28.2  16.3  16.0  16.2  16.4
+ *   256 x 2                                    58.1  25.8  24.1  22.2  30.7
+ *   1024 x 2                                   202   62.9  52.8  33.4  35.1
+ *   4096 x 8 by 384 of 2048 -> 7168            4021  1854  1452  750   680
+ *   4096 x 8 by 384 of 7168 -> 2 x 2048        9186  2648  2224  1291  1221 */
 static MxPlan mx_plan(const MxProduct &g, bool gated)
 {
     static const struct { int tm, rb, wv; float us; } tiles[] = {
@@ -1068,8 +1079,9 @@ extern "C" int k3g_grouped_mxfp4(const void *x, int xdt, int rows, int cols, con
         fprintf(stderr, "%s: w_step is a multiple of 8 bytes (%d)\n", who, w_step);
         return -1;
     }
-    if (w3 && !(b1 > 0.0f && b2 > 0.0f)) {
-        fprintf(stderr, "%s: the activation's caps are positive (%g, %g)\n", who, b1, b2);
+    /* below, a cap's reciprocal may be infinite */
+    if (w3 && !(b1 >= 0x1p-100f && b2 >= 0x1p-100f)) {
+        fprintf(stderr, "%s: the activation's caps are 2^-100 or more (%g, %g)\n", who, b1, b2);
         return -1;
     }
     if (!rows) return 0;

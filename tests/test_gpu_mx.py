@@ -508,3 +508,25 @@ def test_activation(gpu, caps):
         g, u = col[-rows:, None] * np.ones(n), col[-rows:, None] * ops64.values(up, one)[:, 0]
         want = activation(g, u, *caps)
         assert np.all(np.abs(raw - want) <= 2.0 ** -19 * np.abs(want) + 2.0 ** -149), np.abs(raw / want - 1).max()
+
+
+@pytest.mark.parametrize("caps", [(2.0 ** 100, 2.0 ** 100), (4.0, 25.0), (2.0 ** -100, 2.0 ** -100)])
+def test_activation_far(gpu, caps):
+    """Gates and ups far from zero: from a gate of -87 down the sigmoid is 0 whatever up is, so the
+    result is off by all of the formula's; nothing becomes NaN."""
+    print(f"case: the gated product's activation, large gates, caps {caps}", flush=True)
+    mags = np.array([0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
+    col = np.concatenate([[0.0]] + [s * mags * 2.0 ** e for e in range(4, 60) for s in (1.0, -1.0)])
+    x = np.zeros((col.size, 32), np.float32)
+    x[:, 0] = col
+    code = np.zeros((2, 16, 32), np.uint8)
+    code[0, :, 0], code[1, :, 0] = 2, np.arange(16)
+    one = np.full((16, 1), 127, np.uint8)
+    bufs = [tiled(ops64.pack(c), one, 16, 32) for c in code]
+    tab = [np.array([b.ptr], np.uint64) for b in bufs]
+    raw = grouped(x, "f32", np.arange(col.size), 1, np.array([0, col.size]), tab, 16, "f32", col.size, caps)
+    g, u = col[:, None] * np.ones(16), col[:, None] * ops64.values(code[1], one)[:, 0]
+    with np.errstate(over="ignore"):
+        want = activation(g, u, *caps)
+    tol = np.where(g <= -87, 1.0, 2.0 ** -19) * np.abs(want) + 2.0 ** -149
+    assert np.all(np.abs(raw - want) <= tol), np.argwhere(~(np.abs(raw - want) <= tol))[:4]

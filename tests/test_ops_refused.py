@@ -110,6 +110,7 @@ GR = dict(x=A, xdt=BF16, rows=4, cols=64, perm=A, topk=2, off=A, n_experts=8, w=
     (dict(n_experts=0), "experts"), (dict(n_experts=1025), "experts"), (dict(topk=0), "topk"), (dict(topk=65), "topk"),
     (dict(perm=None), "topk"), (dict(off=None), "missing"), (dict(w=None), "missing"), (dict(w3=A + 4), "aligned"),
     (dict(w_step=4), "w_step"), (dict(w_step=12), "w_step"), (dict(b1=0.0), "caps"), (dict(b2=float("nan")), "caps"),
+    (dict(b1=1e-35), "caps"),
     (dict(rows=1 << 22, topk=4), "pairs"), (dict(n=40), "features"), (dict(cols=100), "columns"),
     (dict(work_bytes=0), "workspace"),
 ])
