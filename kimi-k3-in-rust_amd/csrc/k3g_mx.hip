@@ -35,8 +35,8 @@
 #define MX_MAX_COLS (1 << 20)
 #define MX_MAX_PAIRS (1 << 23)
 #define MX_MAX_EXPERTS 1024
-#define MX_MAX_QUADS (1 << 26)       /* activation quads of a call: k_mx_x has 64 threads each */
-#define MX_MAX_BLOCKS (1 << 23)      /* a launch has fewer than 2^32 threads */
+#define MX_MAX_QUADS (1 << 26)       /* activation quads of a call: 32 bits for 17 units of 16 bytes each */
+#define MX_MAX_BLOCKS (1 << 23)      /* a launch has fewer than 2^32 threads: past 2^31 they loop */
 
 typedef int mx_v8i __attribute__((ext_vector_type(8)));
 
@@ -163,18 +163,19 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 k_mx_x(const T *__restrict__ x, size_t nquads, int nQ, int cols, uint8_t *__restrict__ xq)
 {
-    const size_t quad = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (quad >= nquads + nQ) return;
     const int lane = threadIdx.x & 63;
-    const size_t row = quad / nQ;
-    const int col = 512 * (int)(quad - row * nQ) + 8 * lane;
-    Mx8 v = {{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}};
-    if (col < cols && quad < nquads) v = mx_load8(x + row * cols + col);
-    uint32_t s;
-    uint8_t *o = xq + quad * MX_XQ;
-    *(uint32_t *)(o + 4 * lane) = mx_quant(v.f, s);
-    const int b = lane >> 2;
-    if ((lane & 3) == 0) o[256 + 4 * (b & 3) + (b >> 2)] = (uint8_t)s;
+    for (size_t quad = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6); quad < nquads + nQ;
+         quad += (size_t)gridDim.x * 4) {
+        const size_t row = quad / nQ;
+        const int col = 512 * (int)(quad - row * nQ) + 8 * lane;
+        Mx8 v = {{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}};
+        if (col < cols && quad < nquads) v = mx_load8(x + row * cols + col);
+        uint32_t s;
+        uint8_t *o = xq + quad * MX_XQ;
+        *(uint32_t *)(o + 4 * lane) = mx_quant(v.f, s);
+        const int b = lane >> 2;
+        if ((lane & 3) == 0) o[256 + 4 * (b & 3) + (b >> 2)] = (uint8_t)s;
+    }
 }
 
 /* ------------------------------------------------------------------ product ---- */
@@ -1023,7 +1024,7 @@ static int mx_product(const char *who, MxProduct &g, const void *x, int xdt, int
         return xdt == K3_WBF16 ? mx_launch_values<uint16_t>(who, g, plan, bf, gated, on.st)
                                : mx_launch_values<float>(who, g, plan, bf, gated, on.st);
     const size_t nquads = (size_t)g.T * g.nQ;
-    const dim3 xgrid((unsigned)((nquads + g.nQ + 3) / 4));
+    const dim3 xgrid((unsigned)min((nquads + g.nQ + 3) / 4, (size_t)MX_MAX_BLOCKS));
     if (xdt == K3_WBF16 ? k3h_launch(who, k_mx_x<uint16_t>, xgrid, dim3(256), on.st, (const uint16_t *)x,
                                      nquads, g.nQ, cols, (uint8_t *)work)
                         : k3h_launch(who, k_mx_x<float>, xgrid, dim3(256), on.st, (const float *)x, nquads,
