@@ -37,7 +37,8 @@ struct K3hOn {
 static inline bool k3h_misaligned(const void *p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) != 0; }
 
 /* One launch and its own status (not an earlier call's error, which hipGetLastError would
- * give): 0, or -1 with a message. */
+ * give): 0, or -1 with a message. The runtime keeps a failed launch as its last error, which a later
+ * call that asks for it would take for its own: it is read here. */
 template <typename... A>
 static inline int k3h_launch(const char *who, void (*kernel)(A...), dim3 grid, dim3 block, hipStream_t st,
                              A... a)
@@ -45,6 +46,7 @@ static inline int k3h_launch(const char *who, void (*kernel)(A...), dim3 grid, d
     void *args[] = {(void *)&a...};
     const hipError_t e = hipLaunchKernel((const void *)kernel, grid, block, args, 0, st);
     if (e == hipSuccess) return 0;
+    (void)hipGetLastError();
     fprintf(stderr, "%s: launch failed: %s\n", who, hipGetErrorString(e));
     return -1;
 }
