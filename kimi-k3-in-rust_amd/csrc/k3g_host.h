@@ -18,12 +18,10 @@ struct K3hOn {
         hipDevice_t on;
         int cur;
         if (hipStreamGetDevice(st, &on) != hipSuccess || hipGetDevice(&cur) != hipSuccess) {
-            (void)hipGetLastError();
-            fprintf(stderr, "k3moe: the stream's device cannot be told\n");
-            ok = false;
+            refuse("told");
         } else if (on != cur) {
-            ok = hipSetDevice(on) == hipSuccess;
-            back = cur;
+            if (hipSetDevice(on) == hipSuccess) back = cur;
+            else refuse("made the current one");
         }
     }
     ~K3hOn()
@@ -32,6 +30,14 @@ struct K3hOn {
     }
     K3hOn(const K3hOn &) = delete;
     K3hOn &operator=(const K3hOn &) = delete;
+
+private:
+    void refuse(const char *what)
+    {
+        (void)hipGetLastError();
+        fprintf(stderr, "k3moe: the stream's device cannot be %s\n", what);
+        ok = false;
+    }
 };
 
 static inline bool k3h_misaligned(const void *p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) != 0; }

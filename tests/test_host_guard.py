@@ -29,3 +29,8 @@ def audit(tmp_path_factory):
 def test_every_case_holds(audit):
     lines = audit.stdout.split("\n")[:-1]
     assert lines and all(l.startswith("ok ") for l in lines), audit.stdout
+
+
+def test_every_refusal_has_its_message(audit):
+    for cause in ("told:", "current:"):
+        assert f"{cause}k3moe: " in audit.stderr, audit.stderr
