@@ -577,9 +577,10 @@ int  k3g_matmul_mxfp4(const void *x, int xdt, int rows, int cols, const void *w,
  * its tiled matrix, expert e's lies e * w_step bytes on (8 for an array of pointers,
  * sizeof(K3ExpertQ) for &experts[0].p1 of a layer's table). With w3 (NULL for none) each expert
  * has a second such matrix and y[r] = act(q(x) W_e^T, q(x) W3_e^T), the layer's activation with
- * caps b1, b2 (2^-100 and above; from 2^64 on uncapped, SwiGLU) in fp32, within 10 units in the last
- * place; a sigmoid from a gate of -87 down is 0. An expert that has pairs but a NULL matrix gives rows
- * of zeros. Matrices are aligned to 16 bytes. rows * topk <= 2^23. */
+ * caps b1, b2 (2^-100 and above; from 2^64 on uncapped, SwiGLU) in fp32, within 2^-19 of its value
+ * while gate / b1, up / b2 and the products on the way stay in fp32's normal range; a sigmoid from a
+ * gate of -87 down is 0 (times an infinite up: NaN). An expert that has pairs but a NULL matrix gives
+ * rows of zeros. Matrices are aligned to 16 bytes. rows * topk <= 2^23. */
 int  k3g_grouped_mxfp4(const void *x, int xdt, int rows, int cols, const int32_t *perm,
                        int topk, const int32_t *off, int n_experts, const void *const *w,
                        const void *const *w3, int w_step, int n, float b1, float b2, void *y,
