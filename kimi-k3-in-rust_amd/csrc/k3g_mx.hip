@@ -197,8 +197,9 @@ struct MxProduct {
 };
 
 /* Row tile `item` of up to TM places: expert, first place and count; false past the last. Every
- * wave finds it by itself: a lane takes up to 16 experts, all their ranges asked for at once, a wave scan of the lanes' tile counts
- * finds the lane that has it. The ranges are clamped to the places there are, whatever off holds. */
+ * wave finds it by itself: a lane takes up to 16 experts, all their ranges asked for at once, a wave
+ * scan of the lanes' tile counts finds the lane that has it. The ranges are clamped to the places
+ * there are, whatever off holds. */
 template <int TM>
 __device__ __forceinline__ bool mx_tile(const MxProduct &g, int item, int &e, int &p0, int &np)
 {
@@ -326,8 +327,8 @@ __device__ __forceinline__ bool mx_item(const MxProduct &g, int nft, int &ft, in
  * each quotient by a cap 2 (its reciprocal is rounded too; tanh does not enlarge it), the four
  * products 4, together 23 of the 32 that 2^-19 is; 13.5 is the most that has been found. Below
  * the normal range a product loses what fp32 loses. A sigmoid from a gate of -87 down (below 2^-125)
- * is 0, so a gate of minus infinity without a cap, or an infinite up with such a gate, is NaN, as
- * the layer has it. A cap of 2^64 or more is none. */
+ * is 0 (the layer's from -89 down), so an infinite up beside it gives NaN, and a gate of minus
+ * infinity without a cap does, as the layer's. A cap of 2^64 or more is none. */
 __device__ __forceinline__ float mx_rcp(float d)
 {
     const float y = __builtin_amdgcn_rcpf(d);
@@ -844,10 +845,10 @@ extern "C" int k3g_quant_mxfp4(const void *x, int dt, int rows, int cols, void *
     const dim3 grid((unsigned)min((n + 255) / 256, (size_t)MX_MAX_BLOCKS));
     const bool big = 16 * n > MX_STREAM;
     if (dt == K3_WBF16)
-        return k3h_launch(who, big ? k_mx_quant<uint16_t, true> : k_mx_quant<uint16_t, false>, grid, dim3(256), on.st, (const uint16_t *)x, n,
-                          (uint8_t *)packed, (uint8_t *)scales);
-    return k3h_launch(who, big ? k_mx_quant<float, true> : k_mx_quant<float, false>, grid, dim3(256), on.st, (const float *)x, n,
-                      (uint8_t *)packed, (uint8_t *)scales);
+        return k3h_launch(who, big ? k_mx_quant<uint16_t, true> : k_mx_quant<uint16_t, false>, grid,
+                          dim3(256), on.st, (const uint16_t *)x, n, (uint8_t *)packed, (uint8_t *)scales);
+    return k3h_launch(who, big ? k_mx_quant<float, true> : k_mx_quant<float, false>, grid, dim3(256),
+                      on.st, (const float *)x, n, (uint8_t *)packed, (uint8_t *)scales);
 }
 
 extern "C" int k3g_dequant_mxfp4(const void *packed, const void *scales, int rows, int cols, void *out,
@@ -864,10 +865,11 @@ extern "C" int k3g_dequant_mxfp4(const void *packed, const void *scales, int row
     const dim3 grid((unsigned)min((n + 255) / 256, (size_t)MX_MAX_BLOCKS));
     const bool big = 16 * n > MX_STREAM;
     if (dt == K3_WBF16)
-        return k3h_launch(who, big ? k_mx_dequant<uint16_t, true> : k_mx_dequant<uint16_t, false>, grid, dim3(256), on.st, (const uint8_t *)packed,
-                          (const uint8_t *)scales, n, (uint16_t *)out);
-    return k3h_launch(who, big ? k_mx_dequant<float, true> : k_mx_dequant<float, false>, grid, dim3(256), on.st, (const uint8_t *)packed,
-                      (const uint8_t *)scales, n, (float *)out);
+        return k3h_launch(who, big ? k_mx_dequant<uint16_t, true> : k_mx_dequant<uint16_t, false>, grid,
+                          dim3(256), on.st, (const uint8_t *)packed, (const uint8_t *)scales, n,
+                          (uint16_t *)out);
+    return k3h_launch(who, big ? k_mx_dequant<float, true> : k_mx_dequant<float, false>, grid, dim3(256),
+                      on.st, (const uint8_t *)packed, (const uint8_t *)scales, n, (float *)out);
 }
 
 extern "C" size_t k3g_mxfp4_work_bytes(int rows, int cols)
@@ -899,7 +901,8 @@ static int64_t mx_grid(const MxProduct &g, int tm, int rb)
 /* One matrix: a CU's workgroups take turns on what bounds them (its matrix cores, the data that
  * its L1 returns), so a call lasts as long as the CU with the most, ceil(workgroups / 256) times the
  * time of one. That time, in us at 7168 columns beside about 6 of quantisation and launch, is `us`:
- * the tile with the smallest product is taken. Whole calls, us, bf16, tiles in the table's order:
+ * the tile with the smallest product is taken. Only 7168 columns were measured; the rule does not look
+ * at them. Whole calls, us, bf16, tiles in the table's order:
  *   16 rows by 3584            23.4  .     23.3  .     14.3  10.9  12.4  9.5   8.5
  *   64 rows                    28.9  .     28.6  .     20.2  14.4  11.7  12.9  16.6
  *   256 rows                   33.7  30.7  26.6  23.0  19.5  21.8  26.2  30.2  42.6
@@ -911,6 +914,9 @@ static int64_t mx_grid(const MxProduct &g, int tm, int rb)
  * 7.5).
  *
  * Experts: a few tokens meet about one row an expert, and the weights are all there is to wait for.
+ * From 17 rows of x on the rule counts workgroups before it looks at the rows an expert: many experts
+ * of about one row then run by 64 places too, where the second line has the forms by 16 and 32 7 %
+ * ahead. Nothing between 8 and 4096 tokens by 384 experts was measured.
  * us, bf16: quantised inside, before by 16 places, by 32, k_mx_gemm by 64, by 128:
  *   1 token x 8 by 384 of 7168 -> 2 x 2048     21.9  23.9  24.0  24.7  24.9
  *   8 tokens x 8                               133   131   131   141   141
