@@ -586,6 +586,89 @@ int  k3g_grouped_mxfp4(const void *x, int xdt, int rows, int cols, const int32_t
                        const void *const *w3, int w_step, int n, float b1, float b2, void *y,
                        int ydt, void *work, size_t work_bytes, void *stream);
 
+/* ------------------------------------- products with weights of one's own -- */
+/* What a caller trains or serves unquantised: products by fp32 or bf16 matrices in plain rows, one
+ * matrix or an expert's each for the sorted rows, with what follows them, and their gradients. As
+ * above: device pointers, no context, no allocation, no workspace, the stream's device; rows
+ * contiguous, at any address that their elements may have; nothing is atomic, so results do not
+ * depend on the launch. No reference counterpart (the engine's products are k3_matmul's, on the
+ * CPU). Rows from 0 to 2^23, n and cols from 1 to 2^20, any of them odd.
+ *
+ * Types (K3_WF32, K3_WBF16): of the rows (xdt, dydt), of the matrices (wdt) and of what is written
+ * (ydt, dxdt, dwdt), each free. Products of bf16 values are exact in the matrix cores; an fp32
+ * operand enters them as three bf16 pieces that together are its 24 bits (values below 2^-110 lose
+ * bits, as subnormals do), the products of two fp32 operands without the last three pairs of pieces
+ * (below 2^-21 of a product, of either sign, 2^-26 as a rule: less than its rounding to fp32). Sums are fp32, what follows a product is computed on them, and each result is rounded
+ * once, to nearest even. An infinity among fp32 values may give NaN where an infinite result would
+ * be right; rows without one are not touched by it. */
+enum { K3G_ACT_NONE = 0, K3G_ACT_RELU = 1, K3G_ACT_SILU = 2, K3G_ACT_GELU = 3, K3G_ACT_GELU_TANH = 4,
+       K3G_ACT_SITU = 5 };
+
+/* y = act(z) + residual with z = x W^T + bias. K3G_ACT_SITU takes two products, z and z3 = x W3^T +
+ * bias3, and is the layer's gated activation with caps b1, b2 (2^-100 and above; from 2^64 on
+ * uncapped, SwiGLU), to which k3g_grouped_mxfp4's limits apply; GELU is z Phi(z), GELU_TANH its tanh
+ * form. Zero it before filling it; NULL stands for one of zeros. */
+typedef struct {
+    int act;
+    float b1, b2;
+    const float *bias, *bias3;      /* [n] (grouped: [n_experts][n]), or NULL */
+    const void *residual;           /* [rows][n], ydt, may be y itself; or NULL */
+    void *z, *z3;                   /* [rows][n], ydt: z and z3 are written here, for a way back; or NULL */
+} K3gEpilogue;
+
+/* What follows the product on the way back: g = dy W (+ dy3 W3) + add; dx = g, or, with z given (the
+ * values before the activation that made the rows, as K3gEpilogue kept them), dx = g act'(z), and
+ * for K3G_ACT_SITU dz3, the other one's gradient. */
+typedef struct {
+    const void *add;                /* [rows][cols], dxdt, may be dx itself; or NULL */
+    int act;
+    float b1, b2;
+    const void *z, *z3;             /* [rows][cols], dxdt; z3 for K3G_ACT_SITU only */
+    void *dz3;                      /* [rows][cols], dxdt; K3G_ACT_SITU only */
+} K3gBack;
+
+/* y [rows][n] from x [rows][cols], w [n][cols] and, for K3G_ACT_SITU only, w3 [n][cols]. */
+int  k3g_matmul(const void *x, int xdt, int rows, int cols, const void *w, const void *w3, int wdt,
+                int n, const K3gEpilogue *ep, void *y, int ydt, void *stream);
+/* dx [rows][cols] from dy [rows][n] and w, and from dy3 and w3 too, or neither. */
+int  k3g_matmul_grad_x(const void *dy, const void *dy3, int dydt, int rows, int n, const void *w,
+                       const void *w3, int wdt, int cols, const K3gBack *back, void *dx, int dxdt,
+                       void *stream);
+/* dw [n][cols] = dy^T x, or += with accumulate, and dbias [n] (or NULL) the sums of dy's columns,
+ * accumulated as dw is. Without rows they are zeros, or stay. */
+int  k3g_matmul_grad_w(const void *dy, int dydt, const void *x, int xdt, int rows, int n, int cols,
+                       int accumulate, void *dw, int dwdt, float *dbias, void *stream);
+
+/* The same for the sorted rows of n_experts (1 to 1024) experts: place r of expert e, off[e] <= r <
+ * off[e + 1] with off as k3g_sort_tokens writes it, by that expert's matrices. x is the tokens' rows,
+ * place r's being perm[r] / topk (rows * topk <= 2^23), or without perm (NULL, topk 1) the sorted
+ * rows. y, z, z3, residual and bias of a place are its own; places from off[n_experts] on are left as
+ * they were. w: the device address of expert 0's pointer to its matrix, expert e's lies e * w_step
+ * bytes on; a NULL matrix is one of zeros (either of two: the expert's rows are zeros, no bias or
+ * residual added). */
+int  k3g_grouped(const void *x, int xdt, int rows, int cols, const int32_t *perm, int topk,
+                 const int32_t *off, int n_experts, const void *const *w, const void *const *w3,
+                 int w_step, int wdt, int n, const K3gEpilogue *ep, void *y, int ydt, void *stream);
+/* dx [rows][cols] of the sorted rows (rows: places; k3g_permute_grad takes them to the tokens). An
+ * expert with a NULL matrix (either of two) has gradients of zero. */
+int  k3g_grouped_grad_x(const void *dy, const void *dy3, int dydt, int rows, int n,
+                        const int32_t *off, int n_experts, const void *const *w,
+                        const void *const *w3, int w_step, int wdt, int cols, const K3gBack *back,
+                        void *dx, int dxdt, void *stream);
+/* dw: the device address of expert 0's pointer to its gradient [n][cols], expert e's dw_step bytes
+ * on; NULL for an expert whose gradients are not wanted (dbias has none for it either). dbias [n_experts][n] or NULL. dy: the sorted
+ * rows' [places][n]; x, rows, perm, topk as in k3g_grouped. */
+int  k3g_grouped_grad_w(const void *dy, int dydt, const void *x, int xdt, int rows, int n, int cols,
+                        const int32_t *perm, int topk, const int32_t *off, int n_experts,
+                        int accumulate, void *const *dw, int dw_step, int dwdt, float *dbias,
+                        void *stream);
+
+/* Through the activation alone: dz = dh act'(z) and, for K3G_ACT_SITU, dz3, of [rows][n] values (n
+ * from 1 to 2^24, rows from 0 to 2^26) of type dt. dz may be dh or z itself, dz3 too, but not both
+ * the same. */
+int  k3g_act_grad(const void *dh, int dt, int rows, int n, int act, float b1, float b2, const void *z,
+                  const void *z3, void *dz, void *dz3, void *stream);
+
 /* Synchronise the stream and report any error a kernel raised on the device
  * (an exhausted bounded wait, a bad expert index). Returns 0 when clean. */
 int  k3g_sync(K3gCtx *ctx, void *stream);

@@ -1,0 +1,115 @@
+/* k3g_act.h - the activations in fp32, for products that do not give the engine's bits, and their
+ * derivatives. */
+#pragma once
+
+#include "k3g_dev.h"
+#include "../../include/k3moe.h"
+
+/* The layer's activation (k3d_act's formula) in fp32. k3d_act gives the engine's bits by way of
+ * double exp and tanh, which cost a gated product of 25,305 pairs by 9 experts 80 of 261 us, one of
+ * 4,088 by 21 27 of 66; here exp is v_exp_f32 with the rounding of its argument put back, every
+ * reciprocal has a Newton step, and tanh is the fifth convergent of Lambert's continued fraction up
+ * to 1, 1 - 2 / (1 + e^2x) past it. How far off, in units of 2^-24 of the value (every 7th float
+ * tried, v_exp_f32 and v_rcp_f32 up to a unit in the last place off): the sigmoid 5.3, each tanh 4.9,
+ * each quotient by a cap 2 (its reciprocal is rounded too; tanh does not enlarge it), the four
+ * products 4, together 23 of the 32 that 2^-19 is; 13.5 is the most that has been found. Below
+ * the normal range a product loses what fp32 loses. A sigmoid from a gate of -87 down (below 2^-125)
+ * is 0 (the layer's from -89 down), so an infinite up beside it gives NaN, and a gate of minus
+ * infinity without a cap does, as the layer's. A cap of 2^64 or more is none. */
+__device__ __forceinline__ float ka_rcp(float d)
+{
+    const float y = __builtin_amdgcn_rcpf(d);
+    return fmaf(fmaf(-d, y, 1.0f), y, y);
+}
+
+/* e^x for |x| < 87; 2^-126 or 2^126 past that */
+__device__ __forceinline__ float ka_exp(float x)
+{
+    const float L = 1.44269502f, LO = 1.92596303e-8f;          /* log2 e = L + LO */
+    const float t = __builtin_amdgcn_fmed3f(x * L, -126.0f, 126.0f);
+    const float r = fabsf(x) < 87.0f ? fmaf(x, LO, fmaf(x, L, -t)) * 0.693147182f : 0.0f;
+    const float e = __builtin_amdgcn_exp2f(t);
+    return fmaf(e, r, e);
+}
+
+__device__ __forceinline__ float ka_tanh(float x)
+{
+    const float q = x * x, a = fabsf(x);
+    const float low = x * fmaf(q, q + 105.0f, 945.0f) * ka_rcp(fmaf(q, fmaf(q, 15.0f, 420.0f), 945.0f));
+    const float high = copysignf(fmaf(-2.0f, ka_rcp(1.0f + ka_exp(2.0f * a)), 1.0f), x);
+    return a > 1.0f ? high : low;               /* NaN: low */
+}
+
+__device__ __forceinline__ float ka_sigmoid(float v)
+{
+    return v <= -87.0f ? 0.0f : ka_rcp(1.0f + ka_exp(-v));
+}
+
+/* caps b1, b2 and their reciprocals */
+__device__ __forceinline__ float ka_situ(float gate, float up, float b1, float b2, float i1, float i2)
+{
+    const float s = ka_sigmoid(gate);
+    const float a = b1 >= 0x1p64f ? gate : b1 * ka_tanh(gate * i1);
+    const float u = b2 >= 0x1p64f ? up : b2 * ka_tanh(up * i2);
+    return a * s * u;
+}
+
+/* ---- the activations of k3g_matmul (K3G_ACT_*) and their derivatives ----
+ *
+ * Written so that nothing cancels but where the function itself does: gelu by erfc (1 + erf loses
+ * every bit left of -6), its tanh form as z sigmoid(2 t), 1 - sigmoid(z) as sigmoid(-z) and
+ * 1 - tanh^2 as 4 e / (1 + e)^2 with e = exp(-2 |x|). */
+__device__ __forceinline__ float ka_act(int act, float z)
+{
+    const float K = 1.59576912f, C = 0.044715f;         /* sqrt(8 / pi) */
+    switch (act) {
+    case K3G_ACT_RELU: return z < 0.0f ? 0.0f : z;
+    case K3G_ACT_SILU: return z * ka_sigmoid(z);
+    case K3G_ACT_GELU: return 0.5f * z * erfcf(z * -0.707106781f);
+    case K3G_ACT_GELU_TANH: return z * ka_sigmoid(K * fmaf(C * z, z * z, z));
+    default: return z;
+    }
+}
+
+/* d act / dz; past |z| = 64 the gelus' are 0 or 1, and their polynomials stay finite */
+__device__ __forceinline__ float ka_slope(int act, float z)
+{
+    const float K = 1.59576912f, C = 0.044715f;
+    switch (act) {
+    case K3G_ACT_RELU: return z > 0.0f ? 1.0f : z <= 0.0f ? 0.0f : z;
+    case K3G_ACT_SILU: return ka_sigmoid(z) * fmaf(z, ka_sigmoid(-z), 1.0f);
+    case K3G_ACT_GELU: {
+        const float c = __builtin_amdgcn_fmed3f(z, -64.0f, 64.0f);
+        return fmaf(0.5f, erfcf(z * -0.707106781f), c * 0.398942280f * ka_exp(-0.5f * c * c));
+    }
+    case K3G_ACT_GELU_TANH: {
+        const float c = __builtin_amdgcn_fmed3f(z, -64.0f, 64.0f), v = K * fmaf(C * c, c * c, c);
+        const float d = ka_sigmoid(v) * fmaf(c * ka_sigmoid(-v), K * fmaf(3.0f * C, c * c, 1.0f), 1.0f);
+        return z != z ? z : d;
+    }
+    default: return 1.0f;
+    }
+}
+
+/* b tanh(x / b) and its derivative; b from 2^64 on: x and 1 */
+__device__ __forceinline__ float ka_cap(float x, float b, float i, float &slope)
+{
+    if (b >= 0x1p64f) {
+        slope = 1.0f;
+        return x;
+    }
+    const float t = x * i, e = ka_exp(-2.0f * fabsf(t)), r = ka_rcp(1.0f + e);
+    slope = 4.0f * e * r * r;
+    return b * ka_tanh(t);
+}
+
+/* the derivatives of ka_situ by gate and by up */
+__device__ __forceinline__ void ka_situ_slopes(float gate, float up, float b1, float b2, float i1, float i2,
+                                               float &dgate, float &dup)
+{
+    const float s = ka_sigmoid(gate);
+    float da, du;
+    const float a = ka_cap(gate, b1, i1, da), u = ka_cap(up, b2, i2, du);
+    dgate = s * fmaf(a, ka_sigmoid(-gate), da) * u;
+    dup = a * s * du;
+}

@@ -24,8 +24,10 @@
  * (32768 x 7168 bf16 values, 178 us). */
 #include <stdio.h>
 
+#include "k3g_act.h"
 #include "k3g_dev.h"
 #include "k3g_gemm.h"
+#include "k3g_groups.h"
 #include "k3g_host.h"
 #include "k3g_kernels.h"
 
@@ -34,7 +36,7 @@
 #define MX_MAX_ROWS (1 << 26)
 #define MX_MAX_COLS (1 << 20)
 #define MX_MAX_PAIRS (1 << 23)
-#define MX_MAX_EXPERTS 1024
+#define MX_MAX_EXPERTS GM_MAX_EXPERTS
 #define MX_MAX_QUADS (1 << 26)       /* activation quads of a call: 32 bits for 17 units of 16 bytes each */
 #define MX_MAX_BLOCKS (1 << 23)      /* a launch has fewer than 2^32 threads: past 2^31 they loop */
 
@@ -196,59 +198,6 @@ struct MxProduct {
     bool stream;                     /* y is more than the last-level cache holds */
 };
 
-/* Row tile `item` of up to TM places: expert, first place and count; false past the last. Every
- * wave finds it by itself: a lane takes up to 16 experts, all their ranges asked for at once, a wave
- * scan of the lanes' tile counts finds the lane that has it. The ranges are clamped to the places
- * there are, whatever off holds. */
-template <int TM>
-__device__ __forceinline__ bool mx_tile(const MxProduct &g, int item, int &e, int &p0, int &np)
-{
-    if (!g.off) {
-        e = 0;
-        p0 = item * TM;
-        np = min(TM, g.P - p0);
-        return np > 0;
-    }
-    const int lane = threadIdx.x & 63;
-    constexpr int MOST = MX_MAX_EXPERTS / 64;
-    const int per = (g.E + 63) >> 6, e0 = lane * per;
-    int at[MOST + 1], n = 0;
-#pragma unroll
-    for (int i = 0; i <= MOST; ++i)
-        if (i <= per) at[i] = g.off[min(e0 + i, g.E)];
-#pragma unroll
-    for (int i = 0; i < MOST; ++i) {
-        if (i >= per) continue;
-        at[i] = min(max(at[i], 0), g.P);
-        n += (min(max(at[i + 1], at[i]), g.P) - at[i] + TM - 1) / TM;
-    }
-    int inc = n;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(inc, d, K3G_WAVE);
-        if (lane >= d) inc += o;
-    }
-    const uint64_t past = __ballot(inc > item);
-    if (!past) return false;
-    int left = item - (inc - n), fe = 0, fp = 0, fn = 0;
-#pragma unroll
-    for (int i = 0; i < MOST; ++i) {
-        if (i >= per) continue;
-        const int rows = min(max(at[i + 1], at[i]), g.P) - at[i], t = (rows + TM - 1) / TM;
-        if (left >= 0 && left < t) {
-            fe = e0 + i;
-            fp = at[i] + left * TM;
-            fn = min(TM, rows - left * TM);
-        }
-        left -= t;
-    }
-    const int L = __ffsll((unsigned long long)past) - 1;
-    e = __builtin_amdgcn_readlane(fe, L);
-    p0 = __builtin_amdgcn_readlane(fp, L);
-    np = __builtin_amdgcn_readlane(fn, L);
-    return true;
-}
-
 /* What perm says of a place (the place itself without one), and the activation row that is: -1
  * (zeros) for no pair of these tokens. */
 __device__ __forceinline__ int mx_pair(const MxProduct &g, int place) { return g.perm ? g.perm[place] : place; }
@@ -296,69 +245,15 @@ __device__ __forceinline__ uint32_t mx_here(uint32_t v)
     return v;
 }
 
-/* Workgroup b runs on XCD b % 8. One matrix: each XCD takes an eighth of the (feature tile, row
- * tile) pairs in bands of 8 row tiles, so the 64 that run on it at a time are about 8 x 8 and read
- * a sixteenth of what they would alone from past its L2. Experts: the feature tiles are dealt to the
- * XCDs one by one, each with two row tiles one after the other, so an expert's second row tile
- * finds its weights in that L2, and a few experts still fill every XCD. */
 template <int TM>
 __device__ __forceinline__ bool mx_item(const MxProduct &g, int nft, int &ft, int &e, int &p0, int &np)
 {
-    const int xcd = blockIdx.x & 7, s = blockIdx.x >> 3;
-    if (!g.off) {
-        const int tiles = (g.P + TM - 1) / TM, items = tiles * nft, per = (items + 7) / 8;
-        const int i = xcd * per + s;
-        if (s >= per || i >= items) return false;
-        const int band = i / (8 * nft), in = i - band * 8 * nft, wide = min(8, tiles - 8 * band);
-        ft = in / wide;
-        return mx_tile<TM>(g, 8 * band + in - ft * wide, e, p0, np);
-    }
-    const int i = 8 * (s >> 1) + xcd, pair = i / nft;
-    ft = i - pair * nft;
-    return mx_tile<TM>(g, 2 * pair + (s & 1), e, p0, np);
-}
-
-/* The layer's activation (k3d_act's formula) in fp32. k3d_act gives the engine's bits by way of
- * double exp and tanh, which cost a gated product of 25,305 pairs by 9 experts 80 of 261 us, one of
- * 4,088 by 21 27 of 66; here exp is v_exp_f32 with the rounding of its argument put back, every
- * reciprocal has a Newton step, and tanh is the fifth convergent of Lambert's continued fraction up
- * to 1, 1 - 2 / (1 + e^2x) past it. How far off, in units of 2^-24 of the value (every 7th float
- * tried, v_exp_f32 and v_rcp_f32 up to a unit in the last place off): the sigmoid 5.3, each tanh 4.9,
- * each quotient by a cap 2 (its reciprocal is rounded too; tanh does not enlarge it), the four
- * products 4, together 23 of the 32 that 2^-19 is; 13.5 is the most that has been found. Below
- * the normal range a product loses what fp32 loses. A sigmoid from a gate of -87 down (below 2^-125)
- * is 0 (the layer's from -89 down), so an infinite up beside it gives NaN, and a gate of minus
- * infinity without a cap does, as the layer's. A cap of 2^64 or more is none. */
-__device__ __forceinline__ float mx_rcp(float d)
-{
-    const float y = __builtin_amdgcn_rcpf(d);
-    return fmaf(fmaf(-d, y, 1.0f), y, y);
-}
-
-/* e^x for |x| < 87; 2^-126 or 2^126 past that */
-__device__ __forceinline__ float mx_exp(float x)
-{
-    const float L = 1.44269502f, LO = 1.92596303e-8f;          /* log2 e = L + LO */
-    const float t = __builtin_amdgcn_fmed3f(x * L, -126.0f, 126.0f);
-    const float r = fabsf(x) < 87.0f ? fmaf(x, LO, fmaf(x, L, -t)) * 0.693147182f : 0.0f;
-    const float e = __builtin_amdgcn_exp2f(t);
-    return fmaf(e, r, e);
-}
-
-__device__ __forceinline__ float mx_tanh(float x)
-{
-    const float q = x * x, a = fabsf(x);
-    const float low = x * fmaf(q, q + 105.0f, 945.0f) * mx_rcp(fmaf(q, fmaf(q, 15.0f, 420.0f), 945.0f));
-    const float high = copysignf(fmaf(-2.0f, mx_rcp(1.0f + mx_exp(2.0f * a)), 1.0f), x);
-    return a > 1.0f ? high : low;               /* NaN: low */
+    return gm_row_item<TM>(g.off, g.E, g.P, nft, ft, e, p0, np);
 }
 
 __device__ __forceinline__ float mx_act(const MxProduct &g, float gate, float up)
 {
-    const float s = gate <= -87.0f ? 0.0f : mx_rcp(1.0f + mx_exp(-gate));
-    const float a = g.b1 >= 0x1p64f ? gate : g.b1 * mx_tanh(gate * g.i1);
-    const float u = g.b2 >= 0x1p64f ? up : g.b2 * mx_tanh(up * g.i2);
-    return a * s * u;
+    return ka_situ(gate, up, g.b1, g.b2, g.i1, g.i2);
 }
 
 /* np rows of zeros from p0 on, features n0 .. n0 + n (an expert without a matrix) */
@@ -889,13 +784,10 @@ struct MxPlan {
     unsigned blocks;
 };
 
-/* workgroups of tiles of tm rows by rb row blocks, as many as mx_item may be asked for */
+/* workgroups of tiles of tm rows by rb row blocks */
 static int64_t mx_grid(const MxProduct &g, int tm, int rb)
 {
-    const int64_t nft = (g.N / 16 + rb - 1) / rb;
-    if (!g.off) return ((g.P + tm - 1) / tm * nft + 7) / 8 * 8;
-    const int64_t tiles = g.P / tm + min(g.E, g.P);
-    return ((tiles + 1) / 2 * nft + 7) / 8 * 16;
+    return gm_row_items(g.off != nullptr, g.E, g.P, tm, (g.N / 16 + rb - 1) / rb);
 }
 
 /* One matrix: a CU's workgroups take turns on what bounds them (its matrix cores, the data that

@@ -148,6 +148,20 @@ class K3gLayer(C.Structure):
     ]
 
 
+class K3gEpilogue(C.Structure):
+    """include/k3moe.h K3gEpilogue"""
+    _fields_ = [("act", C.c_int), ("b1", C.c_float), ("b2", C.c_float),
+                ("bias", C.c_void_p), ("bias3", C.c_void_p), ("residual", C.c_void_p),
+                ("z", C.c_void_p), ("z3", C.c_void_p)]
+
+
+class K3gBack(C.Structure):
+    """include/k3moe.h K3gBack"""
+    _fields_ = [("add", C.c_void_p), ("act", C.c_int), ("b1", C.c_float), ("b2", C.c_float),
+                ("z", C.c_void_p), ("z3", C.c_void_p), ("dz3", C.c_void_p)]
+
+
+K3G_ACT_NONE, K3G_ACT_RELU, K3G_ACT_SILU, K3G_ACT_GELU, K3G_ACT_GELU_TANH, K3G_ACT_SITU = range(6)
 K3G_EXPERT_MXFP4, K3G_EXPERT_F32, K3G_EXPERT_MXFP4_TILED = 0, 1, 2
 K3_WF32, K3_WBF16, K3_WI8 = 0, 1, 2
 SWIGLU_CAP = float(2.0 ** 100)   # the engine's SwiGLU setting of the SiTU caps
@@ -243,6 +257,21 @@ def lib() -> C.CDLL:
         L.k3g_grouped_mxfp4.argtypes = [vp, i, i, i, vp, i, vp, i, vp, vp, i, i, f, f, vp, i, vp,
                                         sz, vp]
         L.k3g_grouped_mxfp4.restype = i
+        ep, back = C.POINTER(K3gEpilogue), C.POINTER(K3gBack)
+        L.k3g_matmul.argtypes = [vp, i, i, i, vp, vp, i, i, ep, vp, i, vp]
+        L.k3g_matmul.restype = i
+        L.k3g_matmul_grad_x.argtypes = [vp, vp, i, i, i, vp, vp, i, i, back, vp, i, vp]
+        L.k3g_matmul_grad_x.restype = i
+        L.k3g_matmul_grad_w.argtypes = [vp, i, vp, i, i, i, i, i, vp, i, vp, vp]
+        L.k3g_matmul_grad_w.restype = i
+        L.k3g_grouped.argtypes = [vp, i, i, i, vp, i, vp, i, vp, vp, i, i, i, ep, vp, i, vp]
+        L.k3g_grouped.restype = i
+        L.k3g_grouped_grad_x.argtypes = [vp, vp, i, i, i, vp, i, vp, vp, i, i, i, back, vp, i, vp]
+        L.k3g_grouped_grad_x.restype = i
+        L.k3g_grouped_grad_w.argtypes = [vp, i, vp, i, i, i, i, vp, i, vp, i, i, vp, i, i, vp, vp]
+        L.k3g_grouped_grad_w.restype = i
+        L.k3g_act_grad.argtypes = [vp, i, i, i, i, f, f, vp, vp, vp, vp, vp]
+        L.k3g_act_grad.restype = i
         L.k3g_sync.argtypes = [vp, vp]
         L.k3g_sync.restype = i
         L.k3s_byte.argtypes = [u64, u64, u64]
