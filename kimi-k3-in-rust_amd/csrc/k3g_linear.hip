@@ -11,7 +11,10 @@
  * and, of the third, dy with contiguous b. The matrix instruction's accumulator then holds four
  * consecutive a of one b a lane.
  */
+#include <math.h>
 #include <stdio.h>
+
+#include <utility>
 
 #include "k3g_act.h"
 #include "k3g_dev.h"
@@ -30,7 +33,7 @@ struct LnArgs {
     const uint8_t *b, *b3;           /* the rows: x, dy and dy3, dy */
     const int32_t *perm;             /* place -> pair, or NULL: place r is row r */
     uint32_t magic;                  /* ceil(2^32 / topk), 0 for a topk of 1 */
-    int pairs;
+    int T, pairs;                    /* rows of x, and their pairs */
     const int32_t *off;              /* [E + 1] places of each expert, or NULL: one, all places */
     int E, P;                        /* P places at most */
     int64_t step, dstep;             /* bytes from one expert's pointer to the next, of a and of y (grad_w) */
@@ -43,6 +46,7 @@ struct LnArgs {
     uint8_t *z, *z3, *dz3;
     int accumulate;
     float *dbias;
+    bool stream;                     /* results are more than the last-level cache holds */
 };
 
 /* ------------------------------------------------------------ values in memory ---- */
@@ -56,30 +60,47 @@ typedef gm_v2u ln_any8 __attribute__((aligned(2)));
 #define LN_G(T) T
 #endif
 
-__device__ __forceinline__ k3v4f ln_get4(const float *p, int n)
+/* four values as they lie, n of them there */
+template <typename T> struct LnRaw;
+template <> struct LnRaw<float> { gm_v4u v; };
+template <> struct LnRaw<uint16_t> { gm_v2u v; };
+
+__device__ __forceinline__ LnRaw<float> ln_raw4(const float *p, int n)
 {
-    const LN_G(float) *g = (const LN_G(float) *)p;
-    if (n >= 4) {
-        const gm_v4u v = *(const LN_G(ln_any16) *)g;
-        return __builtin_bit_cast(k3v4f, v);
-    }
-    return k3v4f{g[0], n > 1 ? g[1] : 0.0f, n > 2 ? g[2] : 0.0f, 0.0f};
+    const LN_G(uint32_t) *g = (const LN_G(uint32_t) *)p;
+    if (n >= 4) return {*(const LN_G(ln_any16) *)g};
+    return {gm_v4u{g[0], n > 1 ? g[1] : 0u, n > 2 ? g[2] : 0u, 0u}};
 }
 
-__device__ __forceinline__ k3v4f ln_get4(const uint16_t *p, int n)
+__device__ __forceinline__ LnRaw<uint16_t> ln_raw4(const uint16_t *p, int n)
 {
     const LN_G(uint16_t) *g = (const LN_G(uint16_t) *)p;
-    gm_v2u v;
-    if (n >= 4) v = *(const LN_G(ln_any8) *)g;
-    else v = gm_v2u{g[0] | (n > 1 ? (uint32_t)g[1] << 16 : 0u), n > 2 ? g[2] : 0u};
-    return k3v4f{k3d_bf16lo(v.x), k3d_bf16hi(v.x), k3d_bf16lo(v.y), k3d_bf16hi(v.y)};
+    if (n >= 4) return {*(const LN_G(ln_any8) *)g};
+    return {gm_v2u{g[0] | (n > 1 ? (uint32_t)g[1] << 16 : 0u), n > 2 ? g[2] : 0u}};
 }
 
-__device__ __forceinline__ void ln_put4(float *p, int n, const k3v4f &v)
+__device__ __forceinline__ k3v4f ln_values(const LnRaw<float> &r) { return __builtin_bit_cast(k3v4f, r.v); }
+__device__ __forceinline__ k3v4f ln_values(const LnRaw<uint16_t> &r)
+{
+    return k3v4f{k3d_bf16lo(r.v.x), k3d_bf16hi(r.v.x), k3d_bf16lo(r.v.y), k3d_bf16hi(r.v.y)};
+}
+
+template <typename T>
+__device__ __forceinline__ k3v4f ln_get4(const T *p, int n) { return ln_values(ln_raw4(p, n)); }
+
+/* n of four values. stream: past the caches, for results that are more than the last-level cache's
+ * 256 MB (LN_STREAM; gradients of 64 matrices 1408 x 2048 in fp32, 738 MB: 365 -> 268 us). Smaller
+ * ones stay for whoever reads them next: rows of 4096 x 7168 in bf16 are 138 us either way, and what
+ * reads them then 20 us, or 33 where they went past. */
+#define LN_STREAM ((size_t)256 << 20)
+
+__device__ __forceinline__ void ln_put4(float *p, int n, const k3v4f &v, bool stream)
 {
     LN_G(float) *g = (LN_G(float) *)p;
     if (n >= 4) {
-        *(LN_G(ln_any16) *)g = __builtin_bit_cast(gm_v4u, v);
+        const gm_v4u u = __builtin_bit_cast(gm_v4u, v);
+        if (stream) __builtin_nontemporal_store(u, (LN_G(ln_any16) *)g);
+        else *(LN_G(ln_any16) *)g = u;
         return;
     }
     g[0] = v[0];
@@ -87,12 +108,13 @@ __device__ __forceinline__ void ln_put4(float *p, int n, const k3v4f &v)
     if (n > 2) g[2] = v[2];
 }
 
-__device__ __forceinline__ void ln_put4(uint16_t *p, int n, const k3v4f &v)
+__device__ __forceinline__ void ln_put4(uint16_t *p, int n, const k3v4f &v, bool stream)
 {
     LN_G(uint16_t) *g = (LN_G(uint16_t) *)p;
     const gm_v2u u = {k3d_bf16x2(v[0], v[1]), k3d_bf16x2(v[2], v[3])};
     if (n >= 4) {
-        *(LN_G(ln_any8) *)g = u;
+        if (stream) __builtin_nontemporal_store(u, (LN_G(ln_any8) *)g);
+        else *(LN_G(ln_any8) *)g = u;
         return;
     }
     g[0] = (uint16_t)u.x;
@@ -186,69 +208,107 @@ __device__ __forceinline__ const uint8_t *ln_matrix(const LnArgs &g, const uint8
 
 /* ------------------------------------------------------------------- epilogue ---- */
 
-/* What follows four consecutive sums v (and u, of the second matrix) of output row `row`, from
- * column a on: n of them are stored. */
-template <int MODE, bool GATED, typename Y>
-__device__ __forceinline__ void ln_finish(const LnArgs &g, Y *out, int e, size_t row, int a, k3v4f v, k3v4f u)
+/* What the epilogue reads of an output's four values: what is added to them, and the values before
+ * the activation. */
+template <int MODE, typename Y>
+struct LnRead {
+    LnRaw<Y> add, z[MODE == LN_GRAD_X ? 2 : 1];
+};
+
+template <int MODE, typename Y>
+__device__ __forceinline__ void ln_ask(const LnArgs &g, const Y *out, size_t at, int n, LnRead<MODE, Y> &r)
 {
-    const int n = min(4, g.NA - a);
-    const size_t at = row * g.NA + a;
+    const Y *add = MODE == LN_GRAD_W ? (g.accumulate ? out : nullptr) : (const Y *)g.add;
+    if (add) r.add = ln_raw4(add + at, n);
+    if (MODE == LN_GRAD_X && g.z) r.z[0] = ln_raw4((const Y *)g.z + at, n);
+    if (MODE == LN_GRAD_X && g.dz3) r.z[MODE == LN_GRAD_X] = ln_raw4((const Y *)g.z3 + at, n);
+}
+
+/* What follows four consecutive sums v (and u, of the second matrix; b and b3 their biases): n of
+ * them are stored at `at`. */
+template <int MODE, bool GATED, typename Y>
+__device__ __forceinline__ void ln_finish(const LnArgs &g, Y *out, size_t at, int n, k3v4f v, k3v4f u, const k3v4f &b,
+                                          const k3v4f &b3, const LnRead<MODE, Y> &r)
+{
     if constexpr (MODE == LN_FWD) {
-        if (g.bias) v += ln_get4(g.bias + (size_t)e * g.NA + a, n);
-        if (GATED && g.bias3) u += ln_get4(g.bias3 + (size_t)e * g.NA + a, n);
-        if (g.z) ln_put4((Y *)g.z + at, n, v);
-        if (GATED && g.z3) ln_put4((Y *)g.z3 + at, n, u);
+        v += b;
+        if (g.z) ln_put4((Y *)g.z + at, n, v, g.stream);
+        if (GATED) {
+            u += b3;
+            if (g.z3) ln_put4((Y *)g.z3 + at, n, u, g.stream);
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             v[i] = GATED ? ka_situ(v[i], u[i], g.b1, g.b2, g.i1, g.i2) : ka_act(g.act, v[i]);
-        if (g.add) v += ln_get4((const Y *)g.add + at, n);
+        if (g.add) v += ln_values(r.add);
     } else if constexpr (MODE == LN_GRAD_X) {
-        if (g.add) v += ln_get4((const Y *)g.add + at, n);
-        if (g.z) {
-            const k3v4f z = ln_get4((const Y *)g.z + at, n);
-            if (g.dz3) {
-                const k3v4f z3 = ln_get4((const Y *)g.z3 + at, n);
+        if (g.add) v += ln_values(r.add);
+        if (g.dz3) {
+            const k3v4f z = ln_values(r.z[0]), z3 = ln_values(r.z[1]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float dg, du;
-                    ka_situ_slopes(z[i], z3[i], g.b1, g.b2, g.i1, g.i2, dg, du);
-                    u[i] = v[i] * du;
-                    v[i] *= dg;
-                }
-                ln_put4((Y *)g.dz3 + at, n, u);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] *= ka_slope(g.act, z[i]);
+            for (int i = 0; i < 4; ++i) {
+                float dg, du;
+                ka_situ_slopes(z[i], z3[i], g.b1, g.b2, g.i1, g.i2, dg, du);
+                u[i] = v[i] * du;
+                v[i] *= dg;
             }
+            ln_put4((Y *)g.dz3 + at, n, u, g.stream);
+        } else if (g.z) {
+            const k3v4f z = ln_values(r.z[0]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] *= ka_slope(g.act, z[i]);
         }
     } else {
-        if (g.accumulate) v += ln_get4(out + at, n);
+        if (g.accumulate) v += ln_values(r.add);
     }
-    ln_put4(out + at, n, v);
+    ln_put4(out + at, n, v, g.stream);
 }
 
 /* A wave's sums (MA x MB blocks of 16 a x 16 b) out by way of LDS (16 x (16 MA + 4) floats of its
  * own), so that it reads and writes whole pieces of rows: rows row0 + 0 .. rows - 1, columns col0 on.
- * GATED: the blocks are the two matrices' in turn. */
+ * GATED: the blocks are the two matrices' in turn. Everything that 16 rows read from memory is asked
+ * for in one or two goes, the first before their sums go to LDS (one piece of a row at a time, a residual of 4096 x 7168
+ * took 50 of 248 us). */
 template <int MODE, bool GATED, typename Y, int MA, int MB>
 __device__ __forceinline__ void ln_out(const LnArgs &g, float *lds, const k3v4f (&acc)[MA][MB], Y *out, int e,
                                        size_t row0, int rows, int col0)
 {
-    constexpr int PITCH = 16 * MA + 4, LANES = (GATED ? 2 : 4) * MA, STEP = 64 / LANES;
+    constexpr int PITCH = 16 * MA + 4, LANES = (GATED ? 2 : 4) * MA, STEP = 64 / LANES, PASSES = 16 / STEP;
+    constexpr int CHUNK = MODE == LN_GRAD_X && PASSES > 4 ? 4 : PASSES;       /* as registers allow */
     const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
-    const int f = 4 * (lane % LANES), from = GATED ? 32 * (f >> 4) + (f & 15) : f;
-#pragma unroll
+    const int f = 4 * (lane % LANES), from = GATED ? 32 * (f >> 4) + (f & 15) : f, a = col0 + f, n = min(4, g.NA - a);
+    k3v4f b = {0.f, 0.f, 0.f, 0.f}, b3 = b;
+    if (n <= 0) rows = 0;
+    if (MODE == LN_FWD && g.bias && n > 0) b = ln_get4(g.bias + (size_t)e * g.NA + a, n);
+    if (MODE == LN_FWD && GATED && g.bias3 && n > 0) b3 = ln_get4(g.bias3 + (size_t)e * g.NA + a, n);
+#pragma unroll 1
     for (int j = 0; j < MB; ++j) {
-        gm_wave_sync();
+        const int r0 = 16 * j + lane / LANES;
+        const size_t at = (row0 + r0) * g.NA + a;
 #pragma unroll
-        for (int i = 0; i < MA; ++i) *(k3v4f *)(lds + c * PITCH + 16 * i + 4 * q) = acc[i][j];
-        gm_wave_sync();
-#pragma unroll 2
-        for (int r = lane / LANES; r < 16; r += STEP) {
-            if (16 * j + r >= rows || col0 + f >= g.NA) continue;
-            const float *o = lds + r * PITCH + from;
-            const k3v4f v = *(const k3v4f *)o, u = GATED ? *(const k3v4f *)(o + 16) : k3v4f{0.f, 0.f, 0.f, 0.f};
-            ln_finish<MODE, GATED, Y>(g, out, e, row0 + 16 * j + r, col0 + f, v, u);
+        for (int p0 = 0; p0 < PASSES; p0 += CHUNK) {
+            LnRead<MODE, Y> read[CHUNK];
+#pragma unroll
+            for (int p = 0; p < CHUNK; ++p)
+                if (r0 + STEP * (p0 + p) < rows)
+                    ln_ask<MODE, Y>(g, out, at + (size_t)(STEP * (p0 + p)) * g.NA, n, read[p]);
+            if (!p0) {
+                gm_wave_sync();
+#pragma unroll
+                for (int k = 0; k < MB; ++k) {
+                    if (k != j) continue;      /* what follows is in the code once, not MB times */
+#pragma unroll
+                    for (int i = 0; i < MA; ++i) *(k3v4f *)(lds + c * PITCH + 16 * i + 4 * q) = acc[i][k];
+                }
+                gm_wave_sync();
+            }
+#pragma unroll
+            for (int p = 0; p < CHUNK; ++p) {
+                if (r0 + STEP * (p0 + p) >= rows) continue;
+                const float *o = lds + (lane / LANES + STEP * (p0 + p)) * PITCH + from;
+                const k3v4f v = *(const k3v4f *)o, u = GATED ? *(const k3v4f *)(o + 16) : k3v4f{0.f, 0.f, 0.f, 0.f};
+                ln_finish<MODE, GATED, Y>(g, out, at + (size_t)(STEP * (p0 + p)) * g.NA, n, v, u, b, b3, read[p]);
+            }
         }
     }
 }
@@ -489,12 +549,367 @@ k_ln_any(const LnArgs g)
                                  t.a0 + FA / 2 * wa);
 }
 
+/* ---- bf16 rows and matrices whose widths are multiples of 8: BA x BB outputs by four waves, a
+ * quarter each, 64 k at a time. The tiles come to LDS by DMA, two stages; an operand's fragments of
+ * the next 32 k are read while the products of these 32 run, across the stages too, so a step has one
+ * barrier, in its middle: before it every wave has read the last of this stage (into which the
+ * copies for the step after the next then go) and its own copies of the next stage have arrived.
+ *
+ * Rows of contiguous k are 128 bytes of LDS, unit u of row r at slot u ^ (r % 8); rows k of
+ * contiguous a or b as in the tiles of 32 k above, 64 of them. */
+/* The 1 KB copies of an operand's stage by WV waves, WV i + wave the one of this wave: which row (TR: k) of the
+ * tile this lane copies 16 bytes of, and which unit of it */
+template <bool TR, int B, int WV>
+__device__ __forceinline__ int ln_copy_row(int i, int lane, int wave)
+{
+    constexpr int UNITS = TR ? B / 8 : 8;
+    return (64 / UNITS) * (WV * i + wave) + lane / UNITS;
+}
+
+template <bool TR, int B, int WV>
+__device__ __forceinline__ int ln_copy_unit(int i, int lane, int wave)
+{
+    if (!TR) return (lane & 7) ^ (lane >> 3);
+    return (lane % (B / 8)) ^ (2 * ln_swap(ln_copy_row<TR, B, WV>(i, lane, wave)));
+}
+
+/* block i's operand of k 32 kh .. 32 kh + 31 */
+template <bool TR, int B>
+__device__ __forceinline__ k3v8bf ln_frag(const uint8_t *tile, int kh, int i)
+{
+    const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+    if constexpr (TR) {
+        const int k = 32 * kh + 8 * q + (c >> 2), at = 32 * i + 8 * (c & 3);
+        const gm_v2u lo = ln_read_tr(tile + 2 * B * k + (at ^ (32 * ln_swap(k))));
+        const gm_v2u hi = ln_read_tr(tile + 2 * B * (k + 4) + (at ^ (32 * ln_swap(k + 4))));
+        return __builtin_bit_cast(k3v8bf, gm_v4u{lo.x, lo.y, hi.x, hi.y});
+    } else {
+        return __builtin_bit_cast(k3v8bf, *(const gm_v4u *)(tile + 128 * (16 * i + c) + 16 * ((4 * kh + q) ^ (c & 7))));
+    }
+}
+
+/* f(0) ... f(N - 1), each with its number as a constant */
+template <typename F, int... I>
+__device__ __forceinline__ void ln_each(F f, std::integer_sequence<int, I...>)
+{
+    (f(GmInt<I>{}), ...);
+}
+
+/* A copy in two instructions with whatever stands between them: where in LDS it goes, then the 64
+ * lanes x 16 bytes from base + at. M0 is not put back: nothing else in these kernels uses it (the
+ * compiler keeps no value in it, and of the instructions that read it none is here). */
+template <int MORE>
+__device__ __forceinline__ void ln_dma_at(uint32_t lds)
+{
+    asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0" : : "s"(lds), "i"(MORE) : "scc", "memory");
+}
+__device__ __forceinline__ void ln_dma(const uint8_t *base, uint32_t at)
+{
+    asm volatile("global_load_lds_dwordx4 %0, %1" : : "v"(at), "s"(base) : "memory");
+}
+
+/* acc += A B in place. BIG: sums of 128 accumulation registers a lane; the compiler, given the
+ * builtin, moves a third of them about in every step, so the instruction stands here. Its operands
+ * come from LDS as they are (a vector instruction that writes one needs two wait states before it: the
+ * compiler puts none in front of assembly), and whoever reads the sums waits first: ln_settle. */
+template <bool BIG>
+__device__ __forceinline__ void ln_mfma(const k3v8bf &a, const k3v8bf &b, k3v4f &acc)
+{
+    if constexpr (BIG)
+        asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+    else acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0);
+}
+
+/* the same with sums in general registers and an operand that is made in registers */
+template <bool BIG>
+__device__ __forceinline__ void ln_mfma_v(const k3v8bf &a, const k3v8bf &b, k3v4f &acc)
+{
+    if constexpr (BIG)
+        asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(acc) : "v"(a), "v"(b));
+    else acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0);
+}
+
+/* every product under way has written its sums */
+template <bool BIG, int N>
+__device__ __forceinline__ void ln_settle(k3v4f (&acc)[N])
+{
+    if constexpr (BIG) {
+        asm volatile("s_nop 15\n\ts_nop 15" : : : "memory");
+#pragma unroll
+        for (int i = 0; i < N; ++i) asm volatile("" : "+a"(acc[i]));
+    }
+}
+
+/* What is issued after which of the N = MA MB products of 32 k (in the order of A's blocks): reads
+ * of the next fragments (a block i of A, in place, after its last product; MA + j: block j of B, to
+ * the other half) and copies. An instruction of a wave takes four cycles to issue, a product sixteen:
+ * one of these after a product at a time leaves the matrix cores busy, several in a row do not. */
+template <int MA, int MB, int C>
+struct LnPlan {
+    static constexpr int N = MA * MB, BAR = MB * (MA / 4 > 1 ? MA / 4 : 1) - 1;
+    static constexpr int ALL = (2 * N - 1 - BAR) / C, STRIDE = ALL < 4 ? ALL : 4;
+    static constexpr int FIRST = (N - 2 - BAR) / STRIDE + 1 < C ? (N - 2 - BAR) / STRIDE + 1 : C;
+    signed char read[N][2], copy[N];
+    constexpr void put(int slot, int what)
+    {
+        while (slot < N - 1 && read[slot][0] >= 0) ++slot;
+        read[slot][read[slot][0] >= 0] = (signed char)what;
+    }
+    /* bar: the second half, whose reads and copies come after product BAR */
+    constexpr LnPlan(bool bar) : read(), copy()
+    {
+        for (int i = 0; i < N; ++i) read[i][0] = read[i][1] = copy[i] = -1;
+        const int from = bar ? BAR + 1 : 0, room = N - from;
+        for (int i = 0; i < MA; ++i) {
+            const int done = MB * i + MB - 1;
+            if (done >= from) put(done, i);
+        }
+        for (int j = 0; j < MB; ++j) put(from + j * room / (2 * MB), MA + j);
+        for (int i = 0; i < MA; ++i)
+            if (MB * i + MB - 1 < from) put(from + room / 2 + 2 * i, i);
+        for (int c = 0; c < C; ++c)
+            if ((c < FIRST) == bar) copy[bar ? from + c * STRIDE : (c - FIRST) * STRIDE + STRIDE / 2] = (signed char)c;
+    }
+};
+
+template <int MODE, bool GATED, typename Y, int BA, int BB, int WV>
+__global__ void __launch_bounds__(64 * WV, BA + BB > 256 && WV == 4 ? 1 : 2)
+k_ln_tile(const LnArgs g)
+{
+    constexpr bool TA = MODE != LN_FWD, TB = MODE == LN_GRAD_W;
+    constexpr int MA = BA / 32, MB = BB / (8 * WV), STAGE = 128 * (BA + BB), FA = GATED ? BA / 2 : BA;
+    constexpr int CA = BA / (8 * WV), CB = BB / (8 * WV);           /* a wave's copies of a stage */
+    constexpr bool BIG = MA * MB > 16;
+    static_assert(WV * 16 * (16 * MA + 4) * 4 <= 2 * STAGE, "the sums' way out");
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE];
+    LnTile t;
+    if (!ln_tile<MODE, FA, BB>(g, t)) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = gm_uniform(tid >> 6), wa = wave & 1, wb = wave >> 1;
+    const uint8_t *m1 = g.a, *m3 = g.a3;
+    Y *out = (Y *)g.y;
+    if constexpr (MODE == LN_GRAD_W) {
+        if (g.off) out = (Y *)gm_uniform_ptr(*(uint8_t *const *)(g.y + (size_t)t.e * g.dstep));
+        if (!out || (g.accumulate && !t.np)) return;
+    } else {
+        m1 = ln_matrix(g, g.a, t.e);
+        if (g.a3) m3 = ln_matrix(g, g.a3, t.e);
+        if (!m1 || (g.a3 && !m3)) {
+            ln_zeros<MODE, GATED, Y, 64 * WV>(g, out, t.p0, t.np, t.a0, FA);
+            return;
+        }
+    }
+    const int K = MODE == LN_GRAD_W ? t.np : g.K, nk = (K + 63) / 64;
+    const int steps = MODE == LN_GRAD_X && g.a3 ? 2 * nk : nk;
+    /* a matrix comes by the caller's table, and the host has not seen its address: one that is not
+     * aligned for DMA is copied by DMA from the 16 bytes around, and then (fix) by registers */
+    const bool aligned = ((((uintptr_t)m1) | (uintptr_t)m3) & 15) == 0;
+    const bool gather = MODE == LN_GRAD_W && g.perm;
+    const uint32_t ldsp = (uint32_t)(uintptr_t)(k3lds)lds + 1024 * wave;
+
+    /* What this lane copies: at oa, ob from bases that move on by a stage's k, and no further than the
+     * end of the operand, so all reads are of memory that is there. Whatever of it is not of these
+     * rows, columns or k gives outputs that are not stored, or is set to zero once it has arrived
+     * (fix). Forward with two matrices, their blocks of 16 rows alternate in A, and all that a wave
+     * copies is of one. */
+    const size_t a0 = MODE == LN_FWD ? (size_t)t.a0 * K : (size_t)t.a0;
+    const uint8_t *sa = MODE == LN_GRAD_W ? g.a : GATED && wave & 2 ? m3 : m1, *sb = g.b;
+    const uint8_t *ea = sa + 2 * (size_t)g.NA * (MODE == LN_GRAD_W ? g.T : g.K);
+    const uint8_t *eb = sb + 2 * (size_t)(MODE == LN_FWD ? g.T : g.P) * (MODE == LN_GRAD_W ? g.NB : g.K);
+    sa += 2 * (MODE == LN_GRAD_W && !gather ? a0 + (size_t)t.p0 * g.NA : a0);
+    if (MODE == LN_GRAD_W) sb += 2 * ((size_t)t.p0 * g.NB + t.b0);
+    else if (MODE != LN_FWD || !g.perm) sb += 2 * (size_t)t.p0 * K;
+    uint32_t oa[CA], ob[CB], bad = 0;          /* bit i of bad: row i of B is of no pair */
+#pragma unroll
+    for (int i = 0; i < CA; ++i) {
+        const uint32_t r = ln_copy_row<TA, BA, WV>(i, lane, wave), u = ln_copy_unit<TA, BA, WV>(i, lane, wave);
+        if (MODE == LN_FWD) oa[i] = 2 * (GATED ? 16 * (r >> 5) + (r & 15) : r) * K + 16 * u;
+        else oa[i] = 2 * (gather ? 0 : r) * g.NA + 16 * u;
+    }
+#pragma unroll
+    for (int i = 0; i < CB; ++i) {
+        const uint32_t r = ln_copy_row<TB, BB, WV>(i, lane, wave), u = ln_copy_unit<TB, BB, WV>(i, lane, wave);
+        ob[i] = 2 * r * (MODE == LN_GRAD_W ? g.NB : K) + 16 * u;
+        if (MODE == LN_FWD && g.perm) {
+            const int row = ln_row(g, t.p0 + min((int)r, t.np - 1));
+            if (row < 0) bad |= 1u << i;
+            ob[i] = 2 * (uint32_t)max(row, 0) * K + 16 * u;
+        }
+    }
+    const bool any_bad = MODE == LN_FWD && __any(bad != 0);
+    /* the gathered rows of step s, asked for a step ahead of their copies; which of them are none, and
+     * which of the copies under way are */
+    int rows[MODE == LN_GRAD_W ? CA : 1];
+    uint32_t none = 0, flying = 0;
+    auto look = [&](int s) {
+        if constexpr (MODE == LN_GRAD_W) {
+            none = 0;
+#pragma unroll
+            for (int i = 0; i < CA; ++i) {
+                const int k = 64 * s + ln_copy_row<TA, BA, WV>(i, lane, wave);
+                rows[i] = k < K ? ln_row(g, t.p0 + k) : -1;
+                if (rows[i] < 0) none |= 1u << i;
+            }
+        }
+    };
+    auto left = [&](int s) { return K - 64 * (MODE == LN_GRAD_X && s >= nk ? s - nk : s); };
+    uint32_t la = 0, lb = 0, lodd = 0;
+    const uint8_t *odd = sa;                   /* a matrix that is not aligned: its base and limit of the last copies */
+    /* before the copies of step s */
+    auto turn = [&](int s) {
+        if (MODE == LN_GRAD_X && s == nk && s < steps) {
+            sa = m3 + 2 * a0;
+            ea = m3 + 2 * (size_t)g.NA * g.K;
+            sb = g.b3 + 2 * (size_t)t.p0 * K;
+            eb = g.b3 + 2 * (size_t)g.P * g.K;
+        }
+        /* a step past the last is copied all the same, one unit over and over, and not read */
+        if (s >= steps) {
+            sa = ea - 16;
+            sb = eb - 16;
+        }
+        la = (uint32_t)min((size_t)(ea - sa) - 16, (size_t)0xFFFFFFF0u);
+        lb = (uint32_t)min((size_t)(eb - sb) - 16, (size_t)0xFFFFFFF0u);
+    };
+    auto at_a = [&](int i) {
+        if (MODE == LN_GRAD_W && gather) return (uint32_t)max(rows[MODE == LN_GRAD_W ? i : 0], 0) * (2u * g.NA) + oa[i];
+        return oa[i];
+    };
+    auto copy_a = [&](int i) { ln_dma(MODE == LN_GRAD_W ? sa : (const uint8_t *)((uintptr_t)sa & ~(uintptr_t)15), min(at_a(i), la)); };
+    auto copy_b = [&](int i) { ln_dma(sb, min(ob[i], lb)); };
+    auto moved = [&]() {
+        odd = sa;
+        lodd = la;
+        if (!gather) sa += TA ? (size_t)128 * g.NA : (size_t)128;
+        sb += TB ? (size_t)128 * g.NB : (size_t)128;
+        flying = none;
+    };
+    auto copy_to = [&](auto c_, uint32_t to) {
+        constexpr int C = decltype(c_)::value;
+        ln_dma_at<(C < CA ? 0 : 128 * BA) + 1024 * WV * (C < CA ? C : C - CA)>(to);
+        if constexpr (C < CA) copy_a(C);
+        else copy_b(C - CA);
+    };
+    auto copies = [&](int s) {
+        const uint32_t to = ldsp + (s & 1) * STAGE;
+        turn(s);
+        ln_each([&](auto c_) { copy_to(c_, to); }, std::make_integer_sequence<int, CA + CB>{});
+        moved();
+    };
+    /* what this wave's copies of step s brought that does not count, and what DMA could not bring */
+    auto fix = [&](int s) {
+        const int k = left(s);
+        if (s >= steps || (k >= 64 && aligned && !any_bad && !(gather && __any(flying != 0)))) return;
+        uint8_t *to = lds + (s & 1) * STAGE + 1024 * wave + 16 * lane;
+#pragma unroll
+        for (int i = 0; i < CA; ++i) {
+            const int r = ln_copy_row<TA, BA, WV>(i, lane, wave), u = ln_copy_unit<TA, BA, WV>(i, lane, wave);
+            gm_v4u *o = (gm_v4u *)(to + 1024 * WV * i);
+            if (gather ? flying >> i & 1 : (TA ? r : 8 * u) >= k) *o = gm_v4u{0, 0, 0, 0};
+            else if (!aligned) *o = *(const LN_G(ln_any16) *)(odd + min(oa[i], lodd));
+        }
+#pragma unroll
+        for (int i = 0; i < CB; ++i) {
+            const int r = ln_copy_row<TB, BB, WV>(i, lane, wave), u = ln_copy_unit<TB, BB, WV>(i, lane, wave);
+            if ((TB ? r : 8 * u) >= k || (bad >> i & 1)) *(gm_v4u *)(to + 128 * BA + 1024 * WV * i) = gm_v4u{0, 0, 0, 0};
+        }
+        /* no load is pending behind this: the compiler would wait for it, and so for all copies, below */
+        gm_wait_vm<0>();
+    };
+
+    k3v4f acc[MA][MB], sums[MB];
+#pragma unroll
+    for (int j = 0; j < MB; ++j) {
+        sums[j] = k3v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < MA; ++i) acc[i][j] = k3v4f{0.f, 0.f, 0.f, 0.f};
+    }
+    const bool bias = MODE == LN_GRAD_W && g.dbias && t.a0 == 0 && wa == 0;
+    const k3v8bf one = __builtin_bit_cast(k3v8bf, gm_v4u{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u});
+    k3v8bf fa[MA], fb[2][MB];
+    auto read_a = [&](int s, int kh, int i) { fa[i] = ln_frag<TA, BA>(lds + (s & 1) * STAGE, kh, MA * wa + i); };
+    auto read_b = [&](int s, int kh, int j) {
+        fb[kh][j] = ln_frag<TB, BB>(lds + (s & 1) * STAGE + 128 * BA, kh, MB * wb + j);
+    };
+    constexpr int PLAN1 = LnPlan<MA, MB, CA + CB>::FIRST;
+    /* the products of half kh of step s and what goes on meanwhile: reads of the next half (of the next
+     * step after the barrier that the second half has), and copies: of step s + 2 after that barrier,
+     * of step s + 1 the rest in the first half */
+    auto half = [&](auto kh_, int s) {
+        constexpr int KH = decltype(kh_)::value;
+        static constexpr LnPlan<MA, MB, CA + CB> plan(KH == 1);
+        const uint32_t to = ldsp + ((s + 1 + KH) & 1) * STAGE;
+        if (KH == 1) turn(s + 2);
+        ln_each([&](auto m_) {
+            constexpr int M = decltype(m_)::value, I = M / MB, J = M % MB, C = plan.copy[M];
+            constexpr int R0 = plan.read[M][0], R1 = plan.read[M][1];
+            ln_mfma<BIG>(fa[I], fb[KH][J], acc[I][J]);
+            if constexpr (C >= 0) copy_to(GmInt<C>{}, to);
+            if constexpr (KH == 1 && M == plan.BAR) {
+                __builtin_amdgcn_s_waitcnt(0x0070);            /* vmcnt(0) lgkmcnt(0) */
+                fix(s + 1);
+                __syncthreads();
+            }
+            if constexpr (R0 >= MA) read_b(s + KH, 1 - KH, R0 - MA);
+            else if constexpr (R0 >= 0) read_a(s + KH, 1 - KH, R0);
+            if constexpr (R1 >= MA) read_b(s + KH, 1 - KH, R1 - MA);
+            else if constexpr (R1 >= 0) read_a(s + KH, 1 - KH, R1);
+            __builtin_amdgcn_sched_barrier(0);
+        }, std::make_integer_sequence<int, MA * MB>{});
+        if (bias) {
+#pragma unroll
+            for (int j = 0; j < MB; ++j) ln_mfma_v<BIG>(one, fb[KH][j], sums[j]);
+        }
+        if (KH == 0) moved();
+    };
+    if (steps) {
+        if (gather) look(0);
+        copies(0);
+        gm_wait_vm<0>();
+        fix(0);
+        __syncthreads();
+        if (gather) look(1);
+        turn(1);
+        ln_each([&](auto c_) { copy_to(c_, ldsp + STAGE); }, std::make_integer_sequence<int, PLAN1>{});
+#pragma unroll
+        for (int i = 0; i < MA; ++i) read_a(0, 0, i);
+#pragma unroll
+        for (int j = 0; j < MB; ++j) read_b(0, 0, j);
+        if (BIG) asm volatile("s_nop 7" : : : "memory");       /* the sums' zeros */
+        for (int s = 0; s < steps; ++s) {
+            half(GmInt<0>{}, s);
+            if (gather) look(s + 2);
+            half(GmInt<1>{}, s);
+        }
+        gm_wait_vm<0>();
+#pragma unroll
+        for (int i = 0; i < MA; ++i) ln_settle<BIG>(acc[i]);
+        if (MODE == LN_GRAD_W && BIG) {
+#pragma unroll
+            for (int j = 0; j < MB; ++j) asm volatile("" : "+v"(sums[j]));
+        }
+    }
+    __syncthreads();
+    if (bias && lane < 16) {
+#pragma unroll
+        for (int j = 0; j < MB; ++j) {
+            const int b = t.b0 + 16 * MB * wb + 16 * j + lane;
+            if (b >= g.NB) continue;
+            float *o = g.dbias + (size_t)t.e * g.NB + b;
+            *o = g.accumulate ? *o + sums[j][0] : sums[j][0];
+        }
+    }
+    const int valid = MODE == LN_GRAD_W ? g.NB - t.b0 : t.np;
+    ln_out<MODE, GATED, Y, MA, MB>(g, (float *)lds + wave * 16 * (16 * MA + 4), acc, out, t.e,
+                                   (size_t)(MODE == LN_GRAD_W ? t.b0 : t.p0) + 16 * MB * wb, valid - 16 * MB * wb,
+                                   t.a0 + FA / 2 * wa);
+}
+
 /* ---------------------------------------------------- through the activation alone ---- */
 
 template <typename T>
 __global__ void __launch_bounds__(256)
 k_ln_act_grad(const T *dh, const T *z, const T *z3, T *dz, T *dz3, size_t n, int act, float b1, float b2, float i1,
-              float i2)
+              float i2, bool stream)
 {
     for (size_t i = 4 * ((size_t)blockIdx.x * 256 + threadIdx.x); i < n; i += 4 * (size_t)gridDim.x * 256) {
         const int m = (int)min(n - i, (size_t)4);
@@ -510,12 +925,12 @@ k_ln_act_grad(const T *dh, const T *z, const T *z3, T *dz, T *dz3, size_t n, int
                 d3[j] = d[j] * du;
                 d[j] *= dg;
             }
-            ln_put4(dz3 + i, m, d3);
+            ln_put4(dz3 + i, m, d3, stream);
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j) d[j] *= ka_slope(act, v[j]);
         }
-        ln_put4(dz + i, m, d);
+        ln_put4(dz + i, m, d, stream);
     }
 }
 
@@ -590,24 +1005,76 @@ static int ln_groups(const char *who, LnArgs &g, int rows, const int32_t *perm, 
     /* pair / topk is the upper half of pair * ceil(2^32 / topk) for pairs below 2^32 / topk */
     g.perm = perm;
     g.magic = topk > 1 ? (uint32_t)((((uint64_t)1 << 32) + topk - 1) / topk) : 0;
+    g.T = rows;
     g.pairs = g.P = rows * topk;
     g.off = off;
     g.E = E;
     return 0;
 }
 
-template <int MODE, bool GATED, typename TA, typename TB, typename Y>
-static int ln_run(const char *who, const LnArgs &g, hipStream_t st)
+/* workgroups of tiles of fa outputs by fb */
+template <int MODE>
+static int64_t ln_grid(const LnArgs &g, int fa, int fb)
 {
-    const int64_t na = (g.NA + (GATED ? 63 : 127)) / (GATED ? 64 : 128);
-    const int64_t blocks = MODE == LN_GRAD_W ? 8 * (int64_t)g.E * ((na * ((g.NB + 127) / 128) + 7) / 8)
-                                             : gm_row_items(g.off != nullptr, g.E, g.P, 128, na);
-    if (blocks * 256 > UINT32_MAX) {
+    const int64_t na = (g.NA + fa - 1) / fa;
+    if (MODE != LN_GRAD_W) return gm_row_items(g.off != nullptr, g.E, g.P, fb, na);
+    return 8 * (int64_t)g.E * ((na * ((g.NB + fb - 1) / fb) + 7) / 8);
+}
+
+template <int MODE>
+static int ln_launch(const char *who, void (*kernel)(LnArgs), const LnArgs &g, int fa, int fb, int threads,
+                     hipStream_t st)
+{
+    const int64_t blocks = ln_grid<MODE>(g, fa, fb);
+    if (blocks * threads > UINT32_MAX) {
         fprintf(stderr, "%s: %d rows by %d columns (%d experts) are more than a launch takes\n", who,
                 MODE == LN_GRAD_W ? g.NB : g.P, g.NA, g.E);
         return -1;
     }
-    return k3h_launch(who, k_ln_any<MODE, GATED, TA, TB, Y>, dim3((unsigned)blocks), dim3(256), st, (LnArgs)g);
+    return k3h_launch(who, kernel, dim3((unsigned)blocks), dim3(threads), st, (LnArgs)g);
+}
+
+/* bf16 operands whose rows are whole units of 16 bytes */
+template <int MODE>
+static bool ln_tiles(const LnArgs &g)
+{
+    if (g.NA % 8 && MODE != LN_FWD) return false;
+    if (MODE == LN_GRAD_W ? g.NB % 8 : g.K % 8) return false;
+    return !k3h_misaligned(g.b, 16) && !k3h_misaligned(g.b3, 16) && !(MODE == LN_GRAD_W && k3h_misaligned(g.a, 16));
+}
+
+/* about how many tiles of fa outputs by fb there are: of an expert's rows, half a tile more than they fill */
+template <int MODE>
+static double ln_count(const LnArgs &g, int fa, int fb)
+{
+    const double na = (g.NA + fa - 1) / fa;
+    if (MODE == LN_GRAD_W) return na * ((g.NB + fb - 1) / fb) * g.E;
+    if (!g.off) return na * ((g.P + fb - 1) / fb);
+    const int met = g.E < g.P ? g.E : g.P;
+    const double mean = (double)g.P / met;
+    return na * met * (mean < fb / 2 ? 1.0 : mean / fb + 0.5);
+}
+
+/* 256 x 256 tiles (one a CU) or 128 x 128 (two at a time)? */
+template <int MODE>
+static bool ln_wide(const LnArgs &g, bool gated)
+{
+    const double wide = 10.0 * ceil(ln_count<MODE>(g, gated ? 128 : 256, 256) / 256);
+    const double small = fmax(3.0 * ceil(ln_count<MODE>(g, gated ? 64 : 128, 128) / 256), 4.2);
+    return wide < small;
+}
+
+template <int MODE, bool GATED, typename TA, typename TB, typename Y>
+static int ln_run(const char *who, const LnArgs &g, hipStream_t st)
+{
+    if constexpr (sizeof(TA) == 2 && sizeof(TB) == 2) {
+        if (ln_tiles<MODE>(g)) {
+            if (ln_wide<MODE>(g, GATED))
+                return ln_launch<MODE>(who, k_ln_tile<MODE, GATED, Y, 256, 256, 8>, g, GATED ? 128 : 256, 256, 512, st);
+            return ln_launch<MODE>(who, k_ln_tile<MODE, GATED, Y, 128, 128, 4>, g, GATED ? 64 : 128, 128, 256, st);
+        }
+    }
+    return ln_launch<MODE>(who, k_ln_any<MODE, GATED, TA, TB, Y>, g, GATED ? 64 : 128, 128, 256, st);
 }
 
 template <int MODE, bool GATED, typename TA, typename TB>
@@ -618,10 +1085,11 @@ static int ln_run_y(const char *who, const LnArgs &g, int ydt, hipStream_t st)
 }
 
 template <int MODE, bool GATED>
-static int ln_product(const char *who, const LnArgs &g, int adt, int bdt, int ydt, void *stream)
+static int ln_product(const char *who, LnArgs &g, int adt, int bdt, int ydt, void *stream)
 {
     K3hOn on(stream);
     if (!on.ok) return -1;
+    g.stream = (size_t)(MODE == LN_GRAD_W ? (size_t)g.E * g.NB : g.P) * g.NA * ln_size(ydt) > LN_STREAM;
     if (adt == K3_WBF16)
         return bdt == K3_WBF16 ? ln_run_y<MODE, GATED, uint16_t, uint16_t>(who, g, ydt, on.st)
                                : ln_run_y<MODE, GATED, uint16_t, float>(who, g, ydt, on.st);
@@ -668,7 +1136,7 @@ extern "C" int k3g_matmul(const void *x, int xdt, int rows, int cols, const void
                           const K3gEpilogue *ep, void *y, int ydt, void *stream)
 {
     LnArgs g = {};
-    g.pairs = g.P = rows;
+    g.T = g.pairs = g.P = rows;
     g.E = 1;
     return ln_forward("k3g_matmul", g, x, xdt, rows, cols, w, w3, wdt, ln_size(wdt), n, ep, y, ydt, stream);
 }
@@ -775,7 +1243,7 @@ extern "C" int k3g_matmul_grad_w(const void *dy, int dydt, const void *x, int xd
                                  int accumulate, void *dw, int dwdt, float *dbias, void *stream)
 {
     LnArgs g = {};
-    g.pairs = g.P = rows;
+    g.T = g.pairs = g.P = rows;
     g.E = 1;
     return ln_back_w("k3g_matmul_grad_w", g, dy, dydt, x, xdt, rows, n, cols, accumulate, dw, dwdt, ln_size(dwdt),
                      dbias, stream);
@@ -823,10 +1291,12 @@ extern "C" int k3g_act_grad(const void *dh, int dt, int rows, int n, int act, fl
     const size_t count = (size_t)rows * n;
     const dim3 grid((unsigned)min((count + 1023) / 1024, (size_t)1 << 16));
     const float i1 = 1.0f / b1, i2 = 1.0f / b2;
+    const bool stream = count * ln_size(dt) > LN_STREAM;
     if (dt == K3_WBF16)
         return k3h_launch(who, k_ln_act_grad<uint16_t>, grid, dim3(256), on.st, (const uint16_t *)dh,
                           (const uint16_t *)z, (const uint16_t *)z3, (uint16_t *)dz, (uint16_t *)dz3, count, act, b1, b2,
-                          i1, i2);
+                          i1, i2, stream);
     return k3h_launch(who, k_ln_act_grad<float>, grid, dim3(256), on.st, (const float *)dh, (const float *)z,
-                      (const float *)z3, (float *)dz, (float *)dz3, count, act, b1, b2, i1, i2);
+                      (const float *)z3, (float *)dz, (float *)dz3, count, act, b1, b2, i1, i2,
+                      stream);
 }
