@@ -1291,12 +1291,12 @@ extern "C" int k3g_act_grad(const void *dh, int dt, int rows, int n, int act, fl
     const size_t count = (size_t)rows * n;
     const dim3 grid((unsigned)min((count + 1023) / 1024, (size_t)1 << 16));
     const float i1 = 1.0f / b1, i2 = 1.0f / b2;
-    const bool stream = count * ln_size(dt) > LN_STREAM;
+    const bool big = count * ln_size(dt) > LN_STREAM;
     if (dt == K3_WBF16)
         return k3h_launch(who, k_ln_act_grad<uint16_t>, grid, dim3(256), on.st, (const uint16_t *)dh,
                           (const uint16_t *)z, (const uint16_t *)z3, (uint16_t *)dz, (uint16_t *)dz3, count, act, b1, b2,
-                          i1, i2, stream);
+                          i1, i2, big);
     return k3h_launch(who, k_ln_act_grad<float>, grid, dim3(256), on.st, (const float *)dh, (const float *)z,
                       (const float *)z3, (float *)dz, (float *)dz3, count, act, b1, b2, i1, i2,
-                      stream);
+                      big);
 }
