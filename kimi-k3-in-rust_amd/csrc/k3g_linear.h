@@ -1,0 +1,435 @@
+/* k3g_linear.h - what the kernels of the products with weights of one's own share: their arguments,
+ * values in memory, pieces, rows and experts, tiles, and what follows a product. */
+#pragma once
+
+#include <stdio.h>
+
+#include "k3g_act.h"
+#include "k3g_dev.h"
+#include "k3g_gemm.h"
+#include "k3g_groups.h"
+#include "k3g_host.h"
+#include "k3g_kernels.h"
+
+enum { LN_FWD, LN_GRAD_X, LN_GRAD_W };
+
+struct LnArgs {
+    const uint8_t *a, *a3;           /* the matrices (off NULL) or the first expert's pointers; grad_w: x */
+    const uint8_t *b, *b3;           /* the rows: x, dy and dy3, dy */
+    const int32_t *perm;             /* place -> pair, or NULL: place r is row r */
+    uint32_t magic;                  /* ceil(2^32 / topk), 0 for a topk of 1 */
+    int T, pairs;                    /* rows of x, and their pairs */
+    const int32_t *off;              /* [E + 1] places of each expert, or NULL: one, all places */
+    int E, P;                        /* P places at most */
+    int64_t step, dstep;             /* bytes from one expert's pointer to the next, of a and of y (grad_w) */
+    int NA, NB, K;                   /* extents of a, of b (grad_w), of k (not grad_w) */
+    uint8_t *y;                      /* the output; grad_w with off: the first expert's pointer to it */
+    int act;
+    float b1, b2, i1, i2;            /* caps and their reciprocals */
+    const float *bias, *bias3;
+    const uint8_t *add;              /* the residual, or what grad_x adds */
+    uint8_t *z, *z3, *dz3;
+    int accumulate;
+    float *dbias;
+    bool stream;                     /* results are more than the last-level cache holds */
+};
+
+/* ------------------------------------------------------------ values in memory ---- */
+
+/* 16 bytes at any address that two have */
+typedef gm_v4u ln_any16 __attribute__((aligned(2)));
+typedef gm_v2u ln_any8 __attribute__((aligned(2)));
+#ifdef __HIP_DEVICE_COMPILE__
+#define LN_G(T) __attribute__((address_space(1))) T
+#else
+#define LN_G(T) T
+#endif
+
+/* four values as they lie, n of them there */
+template <typename T> struct LnRaw;
+template <> struct LnRaw<float> { gm_v4u v; };
+template <> struct LnRaw<uint16_t> { gm_v2u v; };
+
+__device__ __forceinline__ LnRaw<float> ln_raw4(const float *p, int n)
+{
+    const LN_G(uint32_t) *g = (const LN_G(uint32_t) *)p;
+    if (n >= 4) return {*(const LN_G(ln_any16) *)g};
+    return {gm_v4u{g[0], n > 1 ? g[1] : 0u, n > 2 ? g[2] : 0u, 0u}};
+}
+
+__device__ __forceinline__ LnRaw<uint16_t> ln_raw4(const uint16_t *p, int n)
+{
+    const LN_G(uint16_t) *g = (const LN_G(uint16_t) *)p;
+    if (n >= 4) return {*(const LN_G(ln_any8) *)g};
+    return {gm_v2u{g[0] | (n > 1 ? (uint32_t)g[1] << 16 : 0u), n > 2 ? g[2] : 0u}};
+}
+
+__device__ __forceinline__ k3v4f ln_values(const LnRaw<float> &r) { return __builtin_bit_cast(k3v4f, r.v); }
+__device__ __forceinline__ k3v4f ln_values(const LnRaw<uint16_t> &r)
+{
+    return k3v4f{k3d_bf16lo(r.v.x), k3d_bf16hi(r.v.x), k3d_bf16lo(r.v.y), k3d_bf16hi(r.v.y)};
+}
+
+template <typename T>
+__device__ __forceinline__ k3v4f ln_get4(const T *p, int n) { return ln_values(ln_raw4(p, n)); }
+
+/* n of four values. stream: past the caches, for results that are more than the last-level cache's
+ * 256 MB (LN_STREAM; gradients of 64 matrices 1408 x 2048 in fp32, 738 MB: 365 -> 268 us). Smaller
+ * ones stay for whoever reads them next: rows of 4096 x 7168 in bf16 are 138 us either way, and what
+ * reads them then 20 us, or 33 where they went past. */
+#define LN_STREAM ((size_t)256 << 20)
+
+__device__ __forceinline__ void ln_put4(float *p, int n, const k3v4f &v, bool stream)
+{
+    LN_G(float) *g = (LN_G(float) *)p;
+    if (n >= 4) {
+        const gm_v4u u = __builtin_bit_cast(gm_v4u, v);
+        if (stream) __builtin_nontemporal_store(u, (LN_G(ln_any16) *)g);
+        else *(LN_G(ln_any16) *)g = u;
+        return;
+    }
+    g[0] = v[0];
+    if (n > 1) g[1] = v[1];
+    if (n > 2) g[2] = v[2];
+}
+
+__device__ __forceinline__ void ln_put4(uint16_t *p, int n, const k3v4f &v, bool stream)
+{
+    LN_G(uint16_t) *g = (LN_G(uint16_t) *)p;
+    const gm_v2u u = {k3d_bf16x2(v[0], v[1]), k3d_bf16x2(v[2], v[3])};
+    if (n >= 4) {
+        if (stream) __builtin_nontemporal_store(u, (LN_G(ln_any8) *)g);
+        else *(LN_G(ln_any8) *)g = u;
+        return;
+    }
+    g[0] = (uint16_t)u.x;
+    if (n > 1) g[1] = (uint16_t)(u.x >> 16);
+    if (n > 2) g[2] = (uint16_t)u.y;
+}
+
+/* A unit: 8 consecutive values as they lie */
+template <typename T>
+struct LnUnit {
+    gm_v4u v[sizeof(T) / 2];
+};
+
+template <typename T>
+__device__ __forceinline__ LnUnit<T> ln_whole(const T *p)
+{
+    LnUnit<T> u;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u.v[i] = ((const LN_G(ln_any16) *)p)[i];
+    return u;
+}
+
+/* n of them, zeros behind and for n <= 0 */
+template <typename T>
+__device__ __forceinline__ LnUnit<T> ln_unit(const T *p, int n)
+{
+    LnUnit<T> u;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u.v[i] = gm_v4u{0, 0, 0, 0};
+    if (n >= 8) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) u.v[i] = ((const LN_G(ln_any16) *)p)[i];
+    } else if (n > 0) {
+        const LN_G(T) *g = (const LN_G(T) *)p;
+#pragma unroll
+        for (int i = 0; i < 7; ++i) {
+            if (i >= n) continue;
+            if constexpr (sizeof(T) == 4) u.v[i >> 2][i & 3] = __float_as_uint(g[i]);
+            else u.v[0][i >> 1] |= (uint32_t)g[i] << (16 * (i & 1));
+        }
+    }
+    return u;
+}
+
+/* Its bf16 pieces: one of bf16 values; of fp32 values three, 8 bits each, their sum exact as long as
+ * the last is a normal number. The first is truncated, so none of a finite value is infinite, the
+ * second rounded to nearest, so the last has either sign and the pairs of pieces that a product of
+ * two fp32 values leaves out have no bias. An infinity is its first piece alone. */
+template <typename T> constexpr int ln_pieces = sizeof(T) == 4 ? 3 : 1;
+
+__device__ __forceinline__ void ln_split(const LnUnit<uint16_t> &u, gm_v4u (&p)[1]) { p[0] = u.v[0]; }
+
+__device__ __forceinline__ void ln_split(const LnUnit<float> &u, gm_v4u (&p)[3])
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t h[2];
+        float r[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int e = 2 * i + j;
+            h[j] = u.v[e >> 2][e & 3];
+            const float x = __uint_as_float(h[j]);
+            r[j] = fabsf(x) == __builtin_inff() ? 0.0f : x - __uint_as_float(h[j] & 0xFFFF0000u);
+        }
+        p[0][i] = __builtin_amdgcn_perm(h[1], h[0], 0x07060302u);
+        p[1][i] = k3d_bf16x2(r[0], r[1]);
+        p[2][i] = __builtin_amdgcn_perm(__float_as_uint(r[1] - k3d_bf16hi(p[1][i])),
+                                        __float_as_uint(r[0] - k3d_bf16lo(p[1][i])), 0x07060302u);
+    }
+}
+
+/* acc += A B: every pair of pieces but, of two fp32 operands, the three below 2^-23 of the product */
+template <int PA, int PB>
+__device__ __forceinline__ void ln_mma(const k3v8bf (&a)[PA], const k3v8bf (&b)[PB], k3v4f &acc)
+{
+#pragma unroll
+    for (int i = PA - 1; i >= 0; --i)
+#pragma unroll
+        for (int j = PB - 1; j >= 0; --j)
+            if (i + j <= 2) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], acc, 0, 0, 0);
+}
+
+/* ------------------------------------------------------------- rows and experts ---- */
+
+/* the row of x that a place takes; -1 (zeros) for no pair of these tokens */
+__device__ __forceinline__ int ln_row(const LnArgs &g, int place)
+{
+    if (!g.perm) return place;
+    const uint32_t pair = (uint32_t)g.perm[place];
+    if (pair >= (uint32_t)g.pairs) return -1;
+    return (int)(g.magic ? __umulhi(pair, g.magic) : pair);
+}
+
+__device__ __forceinline__ const uint8_t *ln_matrix(const LnArgs &g, const uint8_t *w, int e)
+{
+    if (!g.off) return w;
+    return gm_uniform_ptr(*(const uint8_t *const *)(w + (size_t)e * g.step));
+}
+
+/* ------------------------------------------------------------------- epilogue ---- */
+
+/* What the epilogue reads of an output's four values: what is added to them, and the values before
+ * the activation. */
+template <int MODE, typename Y>
+struct LnRead {
+    LnRaw<Y> add, z[MODE == LN_GRAD_X ? 2 : 1];
+};
+
+template <int MODE, typename Y>
+__device__ __forceinline__ void ln_ask(const LnArgs &g, const Y *out, size_t at, int n, LnRead<MODE, Y> &r)
+{
+    const Y *add = MODE == LN_GRAD_W ? (g.accumulate ? out : nullptr) : (const Y *)g.add;
+    if (add) r.add = ln_raw4(add + at, n);
+    if (MODE == LN_GRAD_X && g.z) r.z[0] = ln_raw4((const Y *)g.z + at, n);
+    if (MODE == LN_GRAD_X && g.dz3) r.z[MODE == LN_GRAD_X] = ln_raw4((const Y *)g.z3 + at, n);
+}
+
+/* What follows four consecutive sums v (and u, of the second matrix; b and b3 their biases): n of
+ * them are stored at `at`. */
+template <int MODE, bool GATED, typename Y>
+__device__ __forceinline__ void ln_finish(const LnArgs &g, Y *out, size_t at, int n, k3v4f v, k3v4f u, const k3v4f &b,
+                                          const k3v4f &b3, const LnRead<MODE, Y> &r)
+{
+    if constexpr (MODE == LN_FWD) {
+        v += b;
+        if (g.z) ln_put4((Y *)g.z + at, n, v, g.stream);
+        if (GATED) {
+            u += b3;
+            if (g.z3) ln_put4((Y *)g.z3 + at, n, u, g.stream);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            v[i] = GATED ? ka_situ(v[i], u[i], g.b1, g.b2, g.i1, g.i2) : ka_act(g.act, v[i]);
+        if (g.add) v += ln_values(r.add);
+    } else if constexpr (MODE == LN_GRAD_X) {
+        if (g.add) v += ln_values(r.add);
+        if (g.dz3) {
+            const k3v4f z = ln_values(r.z[0]), z3 = ln_values(r.z[1]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float dg, du;
+                ka_situ_slopes(z[i], z3[i], g.b1, g.b2, g.i1, g.i2, dg, du);
+                u[i] = v[i] * du;
+                v[i] *= dg;
+            }
+            ln_put4((Y *)g.dz3 + at, n, u, g.stream);
+        } else if (g.z) {
+            const k3v4f z = ln_values(r.z[0]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] *= ka_slope(g.act, z[i]);
+        }
+    } else {
+        if (g.accumulate) v += ln_values(r.add);
+    }
+    ln_put4(out + at, n, v, g.stream);
+}
+
+/* A wave's sums (MA x MB blocks of 16 a x 16 b) out by way of LDS (16 x (16 MA + 4) floats of its
+ * own), so that it reads and writes whole pieces of rows: rows row0 + 0 .. rows - 1, columns col0 on.
+ * GATED: the blocks are the two matrices' in turn. Everything that 16 rows read from memory is asked
+ * for in one or two goes, the first before their sums go to LDS (one piece of a row at a time, a residual of 4096 x 7168
+ * took 50 of 248 us). */
+template <int MODE, bool GATED, typename Y, int MA, int MB>
+__device__ __forceinline__ void ln_out(const LnArgs &g, float *lds, const k3v4f (&acc)[MA][MB], Y *out, int e,
+                                       size_t row0, int rows, int col0)
+{
+    constexpr int PITCH = 16 * MA + 4, LANES = (GATED ? 2 : 4) * MA, STEP = 64 / LANES, PASSES = 16 / STEP;
+    constexpr int CHUNK = MODE == LN_GRAD_X && PASSES > 4 ? 4 : PASSES;       /* as registers allow */
+    const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+    const int f = 4 * (lane % LANES), from = GATED ? 32 * (f >> 4) + (f & 15) : f, a = col0 + f, n = min(4, g.NA - a);
+    k3v4f b = {0.f, 0.f, 0.f, 0.f}, b3 = b;
+    if (n <= 0) rows = 0;
+    if (MODE == LN_FWD && g.bias && n > 0) b = ln_get4(g.bias + (size_t)e * g.NA + a, n);
+    if (MODE == LN_FWD && GATED && g.bias3 && n > 0) b3 = ln_get4(g.bias3 + (size_t)e * g.NA + a, n);
+#pragma unroll 1
+    for (int j = 0; j < MB; ++j) {
+        const int r0 = 16 * j + lane / LANES;
+        const size_t at = (row0 + r0) * g.NA + a;
+#pragma unroll
+        for (int p0 = 0; p0 < PASSES; p0 += CHUNK) {
+            LnRead<MODE, Y> read[CHUNK];
+#pragma unroll
+            for (int p = 0; p < CHUNK; ++p)
+                if (r0 + STEP * (p0 + p) < rows)
+                    ln_ask<MODE, Y>(g, out, at + (size_t)(STEP * (p0 + p)) * g.NA, n, read[p]);
+            if (!p0) {
+                gm_wave_sync();
+#pragma unroll
+                for (int k = 0; k < MB; ++k) {
+                    if (k != j) continue;      /* what follows is in the code once, not MB times */
+#pragma unroll
+                    for (int i = 0; i < MA; ++i) *(k3v4f *)(lds + c * PITCH + 16 * i + 4 * q) = acc[i][k];
+                }
+                gm_wave_sync();
+            }
+#pragma unroll
+            for (int p = 0; p < CHUNK; ++p) {
+                if (r0 + STEP * (p0 + p) >= rows) continue;
+                const float *o = lds + (lane / LANES + STEP * (p0 + p)) * PITCH + from;
+                const k3v4f v = *(const k3v4f *)o, u = GATED ? *(const k3v4f *)(o + 16) : k3v4f{0.f, 0.f, 0.f, 0.f};
+                ln_finish<MODE, GATED, Y>(g, out, at + (size_t)(STEP * (p0 + p)) * g.NA, n, v, u, b, b3, read[p]);
+            }
+        }
+    }
+}
+
+/* rows x n zeros of an output (an expert without a matrix) */
+template <int MODE, bool GATED, typename Y, int THREADS>
+__device__ __forceinline__ void ln_zeros(const LnArgs &g, Y *out, size_t row0, int rows, int col0, int n)
+{
+    n = min(n, g.NA - col0);
+    for (int i = threadIdx.x; i < rows * n; i += THREADS) {
+        const size_t at = (row0 + i / n) * g.NA + col0 + i % n;
+        out[at] = (Y)0;
+        if (MODE == LN_FWD && g.z) ((Y *)g.z)[at] = (Y)0;
+        if (MODE == LN_FWD && GATED && g.z3) ((Y *)g.z3)[at] = (Y)0;
+        if (MODE == LN_GRAD_X && g.dz3) ((Y *)g.dz3)[at] = (Y)0;
+    }
+}
+
+/* ---- which tile a workgroup takes: rows p0 .. p0 + np of expert e, a from a0, b from b0 (grad_w) ---- */
+struct LnTile {
+    int e, p0, np, a0, b0;
+};
+
+/* grad_w: every expert's tiles are shared out among the XCDs, an eighth in a row each, the first
+ * eighth to another XCD for every expert; so a popular expert's do not lie on one, and an XCD's
+ * neighbours read the same rows. */
+template <int MODE, int TA, int TB>
+__device__ __forceinline__ bool ln_tile(const LnArgs &g, LnTile &t)
+{
+    if constexpr (MODE == LN_GRAD_W) {
+        const int na = (g.NA + TA - 1) / TA, nb = (g.NB + TB - 1) / TB, tiles = na * nb, per = (tiles + 7) / 8;
+        const int s = blockIdx.x >> 3;
+        t.e = s / per;
+        const int i = ((blockIdx.x + t.e) & 7) * per + s - t.e * per;
+        if (i >= tiles) return false;
+        t.b0 = i / na * TB;
+        t.a0 = i % na * TA;
+        t.p0 = 0;
+        t.np = g.P;
+        if (g.off) {
+            t.p0 = min(max(g.off[t.e], 0), g.P);
+            t.np = min(max(g.off[t.e + 1], t.p0), g.P) - t.p0;
+        }
+        return true;
+    } else {
+        int ft;
+        if (!gm_row_item<TB>(g.off, g.E, g.P, (g.NA + TA - 1) / TA, ft, t.e, t.p0, t.np)) return false;
+        t.a0 = ft * TA;
+        t.b0 = 0;
+        return true;
+    }
+}
+
+/* ------------------------------------------------------------------- LDS tiles ----
+ *
+ * An operand's tile of 32 k, bf16: contiguous k: rows of 64 bytes, 16-byte unit u of row r at slot
+ * u ^ (r / 2 % 4); contiguous a (or b): 32 rows k of 128 values, 256 bytes, the 32-byte piece c at
+ * slot c ^ (k % 4 + 4 (k / 8 % 2)), which the transposing read takes four rows k of at once. */
+__device__ __forceinline__ int ln_krow(int row, int u) { return 64 * row + 16 * (u ^ ((row >> 1) & 3)); }
+__device__ __forceinline__ int ln_swap(int k) { return (k & 3) | ((k >> 1) & 4); }
+
+typedef short ln_v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) ln_v4s *ln_l4s;
+
+__device__ __forceinline__ gm_v2u ln_read_tr(const uint8_t *p)
+{
+#ifdef __HIP_DEVICE_COMPILE__
+    return __builtin_bit_cast(gm_v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ln_l4s)p));
+#else
+    return gm_v2u{};
+#endif
+}
+
+/* block i's operand from a tile whose rows are k: lane (c, q) gets k = 8 q .. 8 q + 7 of index 16 i + c */
+__device__ __forceinline__ k3v8bf ln_frag_t(const uint8_t *tile, int i)
+{
+    const int lane = threadIdx.x & 63, k = 8 * (lane >> 4) + ((lane & 15) >> 2), at = 32 * i + 8 * (lane & 3);
+    const gm_v2u lo = ln_read_tr(tile + 256 * k + (at ^ (32 * ln_swap(k))));
+    const gm_v2u hi = ln_read_tr(tile + 256 * (k + 4) + (at ^ (32 * ln_swap(k + 4))));
+    return __builtin_bit_cast(k3v8bf, gm_v4u{lo.x, lo.y, hi.x, hi.y});
+}
+
+__device__ __forceinline__ k3v8bf ln_frag_k(const uint8_t *tile, int i)
+{
+    const int lane = threadIdx.x & 63;
+    return __builtin_bit_cast(k3v8bf, *(const gm_v4u *)(tile + ln_krow(16 * i + (lane & 15), lane >> 4)));
+}
+
+/* ------------------------------------------------------------------- launches ---- */
+
+/* workgroups of tiles of fa outputs by fb */
+template <int MODE>
+static inline int64_t ln_grid(const LnArgs &g, int fa, int fb)
+{
+    const int64_t na = (g.NA + fa - 1) / fa;
+    if (MODE != LN_GRAD_W) return gm_row_items(g.off != nullptr, g.E, g.P, fb, na);
+    return 8 * (int64_t)g.E * ((na * ((g.NB + fb - 1) / fb) + 7) / 8);
+}
+
+template <int MODE>
+static inline int ln_launch(const char *who, void (*kernel)(LnArgs), const LnArgs &g, int fa, int fb, int threads,
+                     hipStream_t st)
+{
+    const int64_t blocks = ln_grid<MODE>(g, fa, fb);
+    if (blocks * threads > UINT32_MAX) {
+        fprintf(stderr, "%s: %d rows by %d columns (%d experts) are more than a launch takes\n", who,
+                MODE == LN_GRAD_W ? g.NB : g.P, g.NA, g.E);
+        return -1;
+    }
+    return k3h_launch(who, kernel, dim3((unsigned)blocks), dim3(threads), st, (LnArgs)g);
+}
+
+/* about how many tiles of fa outputs by fb there are: of an expert's rows, half a tile more than they fill */
+template <int MODE>
+static inline double ln_count(const LnArgs &g, int fa, int fb)
+{
+    const double na = (g.NA + fa - 1) / fa;
+    if (MODE == LN_GRAD_W) return na * ((g.NB + fb - 1) / fb) * g.E;
+    if (!g.off) return na * ((g.P + fb - 1) / fb);
+    const int met = g.E < g.P ? g.E : g.P;
+    const double mean = (double)g.P / met;
+    return na * met * (mean < fb / 2 ? 1.0 : mean / fb + 0.5);
+}
+
+/* The kernels by what they take; each returns 0, or -1 with a message. */
+int ln_run_any(const char *who, const LnArgs &g, int mode, bool gated, int adt, int bdt, int ydt, hipStream_t st);
+bool ln_tile_takes(const LnArgs &g, int mode, bool gated, int adt, int bdt);
+int ln_run_tile(const char *who, const LnArgs &g, int mode, bool gated, int ydt, hipStream_t st);
+bool ln_few_takes(const LnArgs &g, int mode);
+int ln_run_few(const char *who, const LnArgs &g, bool gated, int adt, int bdt, int ydt, hipStream_t st);

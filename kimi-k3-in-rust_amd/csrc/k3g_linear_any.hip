@@ -1,0 +1,275 @@
+/* k3g_linear_any.hip - products of any types and widths and their gradients (k3g_linear.hip has the
+ * formulas). */
+#include "k3g_linear.h"
+
+/* B x B outputs by four waves, a quarter each: 128 x 128 with 32 k at a time, or, where that makes too
+ * few workgroups, 64 x 64 with 64, by G = 2 such groups of waves that take the steps in turn and add
+ * up their sums at the end. A thread's two units of each operand come to registers two of its steps
+ * ahead, and are split into their pieces on the way to LDS, once a workgroup.
+ *
+ * LDS: a plane of 8 KB for each piece. 128 x 32: as in k3g_linear.h. 64 x 64: rows of 128 bytes, of
+ * contiguous k unit u of row r at slot u ^ (r % 8); rows k with the 32-byte piece c at slot
+ * c ^ (k / 2 % 2 + 2 (k / 8 % 2)). Either way a read meets every bank once. */
+#define LN_PLANE 8192
+
+/* where unit u of row r (TR: k) lies */
+template <bool TR, int B>
+__device__ __forceinline__ int ln_any_at(int r, int u)
+{
+    if constexpr (B == 128) return TR ? 256 * r + ((16 * u) ^ (32 * ln_swap(r))) : ln_krow(r, u);
+    return 128 * r + (TR ? (16 * u) ^ (32 * (((r >> 1) & 1) | ((r >> 2) & 2))) : 16 * (u ^ (r & 7)));
+}
+
+/* block i's operand of k 32 h .. 32 h + 31 */
+template <bool TR, int B>
+__device__ __forceinline__ k3v8bf ln_any_frag(const uint8_t *plane, int h, int i)
+{
+    if constexpr (B == 128) return TR ? ln_frag_t(plane, i) : ln_frag_k(plane, i);
+    const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+    if constexpr (TR) {
+        const int k = 32 * h + 8 * q + (c >> 2), u = 2 * i + ((c & 3) >> 1), in = 8 * (c & 1);
+        const gm_v2u lo = ln_read_tr(plane + ln_any_at<true, B>(k, u) + in);
+        const gm_v2u hi = ln_read_tr(plane + ln_any_at<true, B>(k + 4, u) + in);
+        return __builtin_bit_cast(k3v8bf, gm_v4u{lo.x, lo.y, hi.x, hi.y});
+    }
+    return __builtin_bit_cast(k3v8bf, *(const gm_v4u *)(plane + ln_any_at<false, B>(16 * i + c, 4 * h + q)));
+}
+
+template <int MODE, bool GATED, typename TA, typename TB, typename Y, int B, int G>
+__global__ void __launch_bounds__(256 * G, 2)
+k_ln_any(const LnArgs g)
+{
+    constexpr bool RA = MODE != LN_FWD, RB = MODE == LN_GRAD_W;        /* rows k */
+    constexpr int PA = ln_pieces<TA>, PB = ln_pieces<TB>, M = B / 32, BK = 4096 / B, H = BK / 32;
+    constexpr int STAGE = (PA + PB) * LN_PLANE, OUT = 4 * 16 * (16 * M + 4) * 4, JOIN = G > 1 ? 256 * (M * M + M) * 16 : 0;
+    constexpr int BYTES = G * STAGE > OUT ? G * STAGE : OUT;
+    __shared__ __attribute__((aligned(16))) uint8_t lds_all[BYTES > JOIN ? BYTES : JOIN];
+    constexpr int FA = GATED ? B / 2 : B;              /* outputs a of a tile */
+    LnTile t;
+    if (!ln_tile<MODE, FA, B>(g, t)) return;
+    const int tid = threadIdx.x & 255, group = G > 1 ? gm_uniform(threadIdx.x >> 8) : 0;
+    const int lane = tid & 63, wave = gm_uniform(tid >> 6), wa = wave & 1, wb = wave >> 1;
+    uint8_t *lds = lds_all + group * STAGE;
+    const TA *a1 = (const TA *)g.a, *a3 = (const TA *)g.a3;
+    Y *out = (Y *)g.y;
+    if constexpr (MODE == LN_GRAD_W) {
+        if (g.off) out = (Y *)gm_uniform_ptr(*(uint8_t *const *)(g.y + (size_t)t.e * g.dstep));
+        if (!out || (g.accumulate && !t.np)) return;
+    } else {
+        a1 = (const TA *)ln_matrix(g, g.a, t.e);
+        if (g.a3) a3 = (const TA *)ln_matrix(g, g.a3, t.e);
+        if (!a1 || (g.a3 && !a3)) {
+            ln_zeros<MODE, GATED, Y, 256 * G>(g, out, t.p0, t.np, t.a0, FA);
+            return;
+        }
+    }
+    const int K = MODE == LN_GRAD_W ? t.np : g.K, nk = (K + BK - 1) / BK;
+    const int steps = MODE == LN_GRAD_X && g.a3 ? 2 * nk : nk;
+    const bool gather = MODE == LN_GRAD_W && g.perm;
+    /* unit j of this thread: row (or k) and unit of the tile, what it reads next, how many values of it
+     * there are whatever k (0: none) */
+    constexpr int UA = (RA ? B : BK) / 8, UB = (RB ? B : BK) / 8;      /* units of a row */
+    int ra[2], ua[2], rb[2], ub[2], na[2], nb[2], xr[2];
+    const TA *pa[2];
+    const TB *pb[2];
+    auto begin = [&](const TA *m1, const TA *m3, const TB *rows) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int id = tid + 256 * j;
+            ra[j] = id / UA;
+            ua[j] = id % UA;
+            rb[j] = id / UB;
+            ub[j] = id % UB;
+            if constexpr (MODE == LN_FWD) {
+                const int blk = ra[j] >> 4, f = t.a0 + (GATED ? 16 * (blk >> 1) + (ra[j] & 15) : ra[j]);
+                na[j] = f < g.NA ? 8 : 0;
+                pa[j] = (GATED && (blk & 1) ? m3 : m1) + (size_t)min(f, g.NA - 1) * K + 8 * ua[j];
+            } else {
+                const int col = t.a0 + 8 * ua[j];
+                na[j] = min(max(g.NA - col, 0), 8);
+                pa[j] = m1 + (size_t)(MODE == LN_GRAD_X ? ra[j] : gather ? 0 : t.p0 + ra[j]) * g.NA + col;
+            }
+            if constexpr (MODE == LN_GRAD_W) {
+                const int col = t.b0 + 8 * ub[j];
+                nb[j] = min(max(g.NB - col, 0), 8);
+                pb[j] = rows + (size_t)(t.p0 + rb[j]) * g.NB + col;
+            } else {
+                const int row = rb[j] >= t.np ? -1 : MODE == LN_FWD ? ln_row(g, t.p0 + rb[j]) : t.p0 + rb[j];
+                nb[j] = row < 0 ? 0 : 8;
+                pb[j] = rows + (size_t)max(row, 0) * K + 8 * ub[j];
+            }
+        }
+    };
+    /* the gathered rows of step s, asked for a step ahead of what reads them */
+    auto look = [&](int s) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int k = BK * s + ra[j];
+            xr[j] = k < K ? ln_row(g, t.p0 + k) : -1;
+        }
+    };
+    LnUnit<TA> va[2][2];
+    LnUnit<TB> vb[2][2];
+    bool inside = false;                       /* every unit of this wave has its 8 values, k apart */
+    auto fetch = [&](int s, int d) {
+        const bool second = MODE == LN_GRAD_X && s >= nk;
+        if (s < G || (second && s < nk + G)) {
+            begin(second ? a3 : a1, a3, (const TB *)(second ? g.b3 : g.b));
+            inside = __all(na[0] == 8 && na[1] == 8 && nb[0] == 8 && nb[1] == 8);
+        }
+        const int k0 = BK * (second ? s - nk : s), left = s < steps ? K - k0 : 0;
+        if (gather && s < G) look(s);
+        const size_t ka = (size_t)k0 * (RA ? g.NA : 1), kb = (size_t)k0 * (RB ? g.NB : 1);
+        if (inside && left >= BK && !gather) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                va[d][j] = ln_whole(pa[j] + ka);
+                vb[d][j] = ln_whole(pb[j] + kb);
+            }
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const TA *p = pa[j] + (gather ? (size_t)max(xr[j], 0) * g.NA : ka);
+            int n = na[j];
+            if (!RA) n = min(n, left - 8 * ua[j]);
+            else if (gather ? xr[j] < 0 : ra[j] >= left) n = 0;
+            va[d][j] = ln_unit(n > 0 ? p : pa[j], n);
+            n = nb[j];
+            if (!RB) n = min(n, left - 8 * ub[j]);
+            else if (rb[j] >= left) n = 0;
+            vb[d][j] = ln_unit(n > 0 ? pb[j] + kb : pb[j], n);
+        }
+        if (gather) look(s + G);
+    };
+    k3v4f acc[M][M], sums[M];
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+        sums[i] = k3v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < M; ++j) acc[i][j] = k3v4f{0.f, 0.f, 0.f, 0.f};
+    }
+    const bool bias = MODE == LN_GRAD_W && g.dbias && t.a0 == 0 && wa == 0;
+    if (steps) {
+        fetch(group, 0);
+        fetch(group + G, 1);
+    }
+    for (int s0 = 0; s0 < steps; s0 += 2 * G)
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+            if (s0 + G * d >= steps) break;
+            const int s = s0 + G * d + group;              /* past the last: zeros */
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                gm_v4u qa[PA], qb[PB];
+                ln_split(va[d][j], qa);
+                ln_split(vb[d][j], qb);
+                const int oa = ln_any_at<RA, B>(ra[j], ua[j]), ob = ln_any_at<RB, B>(rb[j], ub[j]);
+#pragma unroll
+                for (int i = 0; i < PA; ++i) *(gm_v4u *)(lds + i * LN_PLANE + oa) = qa[i];
+#pragma unroll
+                for (int i = 0; i < PB; ++i) *(gm_v4u *)(lds + (PA + i) * LN_PLANE + ob) = qb[i];
+            }
+            __syncthreads();
+            if (s0 + G * (d + 2) < steps) fetch(s + 2 * G, d);
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                k3v8bf fb[M][PB];
+#pragma unroll
+                for (int j = 0; j < M; ++j)
+#pragma unroll
+                    for (int i = 0; i < PB; ++i) fb[j][i] = ln_any_frag<RB, B>(lds + (PA + i) * LN_PLANE, h, M * wb + j);
+#pragma unroll
+                for (int i = 0; i < M; ++i) {
+                    k3v8bf fa[PA];
+#pragma unroll
+                    for (int p = 0; p < PA; ++p) fa[p] = ln_any_frag<RA, B>(lds + p * LN_PLANE, h, M * wa + i);
+#pragma unroll
+                    for (int j = 0; j < M; ++j) ln_mma<PA, PB>(fa, fb[j], acc[i][j]);
+                }
+                if (bias) {
+                    k3v8bf one[1];
+                    one[0] = __builtin_bit_cast(k3v8bf, gm_v4u{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u});
+#pragma unroll
+                    for (int j = 0; j < M; ++j) ln_mma<1, PB>(one, fb[j], sums[j]);
+                }
+            }
+        }
+    __syncthreads();
+    if constexpr (G > 1) {
+        /* the second group's sums to the first */
+        k3v4f *join = (k3v4f *)lds_all + tid;
+        if (group) {
+#pragma unroll
+            for (int i = 0; i < M; ++i) {
+                join[256 * (M * M + i)] = sums[i];
+#pragma unroll
+                for (int j = 0; j < M; ++j) join[256 * (M * i + j)] = acc[i][j];
+            }
+        }
+        __syncthreads();
+        if (!group) {
+#pragma unroll
+            for (int i = 0; i < M; ++i) {
+                sums[i] += join[256 * (M * M + i)];
+#pragma unroll
+                for (int j = 0; j < M; ++j) acc[i][j] += join[256 * (M * i + j)];
+            }
+        }
+        __syncthreads();
+        if (group) return;
+    }
+    if (bias && lane < 16) {
+        /* every row of the product with ones is the sums; lane c holds those of index c */
+#pragma unroll
+        for (int j = 0; j < M; ++j) {
+            const int b = t.b0 + B / 2 * wb + 16 * j + lane;
+            if (b >= g.NB) continue;
+            float *o = g.dbias + (size_t)t.e * g.NB + b;
+            *o = g.accumulate ? *o + sums[j][0] : sums[j][0];
+        }
+    }
+    const int valid = MODE == LN_GRAD_W ? g.NB - t.b0 : t.np;
+    ln_out<MODE, GATED, Y, M, M>(g, (float *)lds_all + wave * 16 * (16 * M + 4), acc, out, t.e,
+                                 (size_t)(MODE == LN_GRAD_W ? t.b0 : t.p0) + B / 2 * wb, valid - B / 2 * wb,
+                                 t.a0 + FA / 2 * wa);
+}
+
+/* Which tile: 64 x 64 where 128 x 128 would make less than a workgroup a CU, or experts have too few
+ * rows to fill them; two groups of waves where those make no more than that either. us, fp32 rows and
+ * (forward, second gradient) fp32 matrices, tiles of 128, of 64 with one group, with two:
+ *   617 rows, 709 -> 1411, gradient of the rows      57   30   20
+ *   the same, of the matrix                          72   36   35
+ *   617 x 6 pairs by 64 experts, 1411 -> 2 x 709     269  221  337 */
+template <int MODE, bool GATED, typename TA, typename TB>
+static int ln_any_y(const char *who, const LnArgs &g, int ydt, hipStream_t st)
+{
+    const int met = g.off ? (g.E < g.P ? g.E : g.P) : 1;
+    const bool short_rows = MODE != LN_GRAD_W && g.off && g.P / met <= 64;
+    if (!short_rows && ln_count<MODE>(g, GATED ? 64 : 128, 128) >= 256)
+        return ln_launch<MODE>(who, ydt == K3_WBF16 ? k_ln_any<MODE, GATED, TA, TB, uint16_t, 128, 1>
+                                                    : k_ln_any<MODE, GATED, TA, TB, float, 128, 1>, g, GATED ? 64 : 128, 128, 256, st);
+    if (ln_count<MODE>(g, GATED ? 32 : 64, 64) > 256)
+        return ln_launch<MODE>(who, ydt == K3_WBF16 ? k_ln_any<MODE, GATED, TA, TB, uint16_t, 64, 1>
+                                                    : k_ln_any<MODE, GATED, TA, TB, float, 64, 1>, g, GATED ? 32 : 64, 64, 256, st);
+    return ln_launch<MODE>(who, ydt == K3_WBF16 ? k_ln_any<MODE, GATED, TA, TB, uint16_t, 64, 2>
+                                                : k_ln_any<MODE, GATED, TA, TB, float, 64, 2>, g, GATED ? 32 : 64, 64, 512, st);
+}
+
+template <int MODE, bool GATED>
+static int ln_any_m(const char *who, const LnArgs &g, int adt, int bdt, int ydt, hipStream_t st)
+{
+    if (adt == K3_WBF16)
+        return bdt == K3_WBF16 ? ln_any_y<MODE, GATED, uint16_t, uint16_t>(who, g, ydt, st)
+                               : ln_any_y<MODE, GATED, uint16_t, float>(who, g, ydt, st);
+    return bdt == K3_WBF16 ? ln_any_y<MODE, GATED, float, uint16_t>(who, g, ydt, st)
+                           : ln_any_y<MODE, GATED, float, float>(who, g, ydt, st);
+}
+
+int ln_run_any(const char *who, const LnArgs &g, int mode, bool gated, int adt, int bdt, int ydt, hipStream_t st)
+{
+    if (mode == LN_GRAD_X) return ln_any_m<LN_GRAD_X, false>(who, g, adt, bdt, ydt, st);
+    if (mode == LN_GRAD_W) return ln_any_m<LN_GRAD_W, false>(who, g, adt, bdt, ydt, st);
+    return gated ? ln_any_m<LN_FWD, true>(who, g, adt, bdt, ydt, st) : ln_any_m<LN_FWD, false>(who, g, adt, bdt, ydt, st);
+}

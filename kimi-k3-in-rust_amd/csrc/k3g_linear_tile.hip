@@ -1,0 +1,456 @@
+/* k3g_linear_tile.hip - products of bf16 rows by bf16 matrices whose widths are multiples of 8, and
+ * their gradients (k3g_linear.hip has the formulas): tiles of many rows. */
+#include <math.h>
+
+#include <utility>
+
+#include "k3g_linear.h"
+
+/* ---- bf16 rows and matrices whose widths are multiples of 8: BA x BB outputs by four waves, a
+ * quarter each, 64 k at a time. The tiles come to LDS by DMA, NS stages; an operand's fragments of
+ * the next 32 k are read while the products of these 32 run, across the stages too, so a step has one
+ * barrier, in its middle: before it every wave has read the last of this stage (into which the
+ * copies for step NS after this one then go) and its own copies of the next stage have arrived.
+ *
+ * Rows of contiguous k are 128 bytes of LDS, unit u of row r at slot u ^ (r % 8); rows k of
+ * contiguous a or b as in the tiles of 32 k above, 64 of them. */
+/* The 1 KB copies of an operand's stage by WV waves, WV i + wave the one of this wave: which row (TR: k) of the
+ * tile this lane copies 16 bytes of, and which unit of it */
+template <bool TR, int B, int WV>
+__device__ __forceinline__ int ln_copy_row(int i, int lane, int wave)
+{
+    constexpr int UNITS = TR ? B / 8 : 8;
+    return (64 / UNITS) * (WV * i + wave) + lane / UNITS;
+}
+
+template <bool TR, int B, int WV>
+__device__ __forceinline__ int ln_copy_unit(int i, int lane, int wave)
+{
+    if (!TR) return (lane & 7) ^ (lane >> 3);
+    return (lane % (B / 8)) ^ (2 * ln_swap(ln_copy_row<TR, B, WV>(i, lane, wave)));
+}
+
+/* block i's operand of k 32 kh .. 32 kh + 31 */
+template <bool TR, int B>
+__device__ __forceinline__ k3v8bf ln_frag(const uint8_t *tile, int kh, int i)
+{
+    const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+    if constexpr (TR) {
+        const int k = 32 * kh + 8 * q + (c >> 2), at = 32 * i + 8 * (c & 3);
+        const gm_v2u lo = ln_read_tr(tile + 2 * B * k + (at ^ (32 * ln_swap(k))));
+        const gm_v2u hi = ln_read_tr(tile + 2 * B * (k + 4) + (at ^ (32 * ln_swap(k + 4))));
+        return __builtin_bit_cast(k3v8bf, gm_v4u{lo.x, lo.y, hi.x, hi.y});
+    } else {
+        return __builtin_bit_cast(k3v8bf, *(const gm_v4u *)(tile + 128 * (16 * i + c) + 16 * ((4 * kh + q) ^ (c & 7))));
+    }
+}
+
+/* f(0) ... f(N - 1), each with its number as a constant */
+template <typename F, int... I>
+__device__ __forceinline__ void ln_each(F f, std::integer_sequence<int, I...>)
+{
+    (f(GmInt<I>{}), ...);
+}
+
+/* A copy in two instructions with whatever stands between them: where in LDS it goes, then the 64
+ * lanes x 16 bytes from base + at. M0 is not put back: nothing else in these kernels uses it (the
+ * compiler keeps no value in it, and of the instructions that read it none is here). */
+template <int MORE>
+__device__ __forceinline__ void ln_dma_at(uint32_t lds)
+{
+    asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0" : : "s"(lds), "i"(MORE) : "scc", "memory");
+}
+__device__ __forceinline__ void ln_dma(const uint8_t *base, uint32_t at)
+{
+    asm volatile("global_load_lds_dwordx4 %0, %1" : : "v"(at), "s"(base) : "memory");
+}
+
+/* acc += A B in place. BIG: sums of 128 accumulation registers a lane; the compiler, given the
+ * builtin, moves a third of them about in every step, so the instruction stands here. Its operands
+ * come from LDS as they are (a vector instruction that writes one needs two wait states before it: the
+ * compiler puts none in front of assembly), and whoever reads the sums waits first: ln_settle. */
+template <bool BIG>
+__device__ __forceinline__ void ln_mfma(const k3v8bf &a, const k3v8bf &b, k3v4f &acc)
+{
+    if constexpr (BIG)
+        asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+    else acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0);
+}
+
+/* the same with sums in general registers and an operand that is made in registers */
+template <bool BIG>
+__device__ __forceinline__ void ln_mfma_v(const k3v8bf &a, const k3v8bf &b, k3v4f &acc)
+{
+    if constexpr (BIG)
+        asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(acc) : "v"(a), "v"(b));
+    else acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0);
+}
+
+/* at most N copies under way, and every read of LDS back */
+template <int N>
+__device__ __forceinline__ void ln_wait()
+{
+    __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14);
+}
+
+/* every product under way has written its sums */
+template <bool BIG, int N>
+__device__ __forceinline__ void ln_settle(k3v4f (&acc)[N])
+{
+    if constexpr (BIG) {
+        asm volatile("s_nop 15\n\ts_nop 15" : : : "memory");
+#pragma unroll
+        for (int i = 0; i < N; ++i) asm volatile("" : "+a"(acc[i]));
+    }
+}
+
+/* What is issued after which of the N = MA MB products of 32 k (in the order of A's blocks): reads
+ * of the next fragments (a block i of A, in place, after its last product; MA + j: block j of B, to
+ * the other half) and copies. An instruction of a wave takes four cycles to issue, a product sixteen:
+ * one of these after a product at a time leaves the matrix cores busy, several in a row do not. */
+template <int MA, int MB, int C>
+struct LnPlan {
+    static constexpr int N = MA * MB, BAR = MB * (MA / 4 > 1 ? MA / 4 : 1) - 1;
+    static constexpr int ALL = (2 * N - 1 - BAR) / C, STRIDE = ALL < 4 ? ALL : 4;
+    static constexpr int FIRST = (N - 2 - BAR) / STRIDE + 1 < C ? (N - 2 - BAR) / STRIDE + 1 : C;
+    signed char read[N][2], copy[N];
+    constexpr void put(int slot, int what)
+    {
+        while (slot < N - 1 && read[slot][0] >= 0) ++slot;
+        read[slot][read[slot][0] >= 0] = (signed char)what;
+    }
+    /* bar: the second half, whose reads and copies come after product BAR */
+    constexpr LnPlan(bool bar) : read(), copy()
+    {
+        for (int i = 0; i < N; ++i) read[i][0] = read[i][1] = copy[i] = -1;
+        const int from = bar ? BAR + 1 : 0, room = N - from;
+        for (int i = 0; i < MA; ++i) {
+            const int done = MB * i + MB - 1;
+            if (done >= from) put(done, i);
+        }
+        for (int j = 0; j < MB; ++j) put(from + j * room / (2 * MB), MA + j);
+        for (int i = 0; i < MA; ++i)
+            if (MB * i + MB - 1 < from) put(from + room / 2 + 2 * i, i);
+        for (int c = 0; c < C; ++c)
+            if ((c < FIRST) == bar) copy[bar ? from + c * STRIDE : (c - FIRST) * STRIDE + STRIDE / 2] = (signed char)c;
+    }
+};
+
+template <int MODE, bool GATED, typename Y, int BA, int BB, int WV, int NS>
+__global__ void __launch_bounds__(64 * WV, 2)
+k_ln_tile(const LnArgs g)
+{
+    constexpr bool TA = MODE != LN_FWD, TB = MODE == LN_GRAD_W;
+    constexpr int MA = BA / 32, MB = BB / (8 * WV), STAGE = 128 * (BA + BB), FA = GATED ? BA / 2 : BA;
+    constexpr int CA = BA / (8 * WV), CB = BB / (8 * WV);           /* a wave's copies of a stage */
+    constexpr bool BIG = MA * MB > 16;
+    static_assert(WV * 16 * (16 * MA + 4) * 4 <= NS * STAGE, "the sums' way out");
+    static_assert(NS == 2 || MODE != LN_GRAD_W, "gathered rows are looked up one step ahead");
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[NS * STAGE];
+    LnTile t;
+    if (!ln_tile<MODE, FA, BB>(g, t)) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = gm_uniform(tid >> 6), wa = wave & 1, wb = wave >> 1;
+    const uint8_t *m1 = g.a, *m3 = g.a3;
+    Y *out = (Y *)g.y;
+    if constexpr (MODE == LN_GRAD_W) {
+        if (g.off) out = (Y *)gm_uniform_ptr(*(uint8_t *const *)(g.y + (size_t)t.e * g.dstep));
+        if (!out || (g.accumulate && !t.np)) return;
+    } else {
+        m1 = ln_matrix(g, g.a, t.e);
+        if (g.a3) m3 = ln_matrix(g, g.a3, t.e);
+        if (!m1 || (g.a3 && !m3)) {
+            ln_zeros<MODE, GATED, Y, 64 * WV>(g, out, t.p0, t.np, t.a0, FA);
+            return;
+        }
+    }
+    const int K = MODE == LN_GRAD_W ? t.np : g.K, nk = (K + 63) / 64;
+    const int steps = MODE == LN_GRAD_X && g.a3 ? 2 * nk : nk;
+    /* a matrix comes by the caller's table, and the host has not seen its address: one that is not
+     * aligned for DMA is copied by DMA from the 16 bytes around, and then (fix) by registers */
+    const bool aligned = ((((uintptr_t)m1) | (uintptr_t)m3) & 15) == 0;
+    const bool gather = MODE == LN_GRAD_W && g.perm;
+    const uint32_t ldsp = (uint32_t)(uintptr_t)(k3lds)lds + 1024 * wave;
+
+    /* What this lane copies: at oa, ob from bases that move on by a stage's k, and no further than the
+     * end of the operand, so all reads are of memory that is there. Whatever of it is not of these
+     * rows, columns or k gives outputs that are not stored, or is set to zero once it has arrived
+     * (fix). Forward with two matrices, their blocks of 16 rows alternate in A, and all that a wave
+     * copies is of one. */
+    const size_t a0 = MODE == LN_FWD ? (size_t)t.a0 * K : (size_t)t.a0;
+    const uint8_t *sa = MODE == LN_GRAD_W ? g.a : GATED && wave & 2 ? m3 : m1, *sb = g.b;
+    const uint8_t *ea = sa + 2 * (size_t)g.NA * (MODE == LN_GRAD_W ? g.T : g.K);
+    const uint8_t *eb = sb + 2 * (size_t)(MODE == LN_FWD ? g.T : g.P) * (MODE == LN_GRAD_W ? g.NB : g.K);
+    sa += 2 * (MODE == LN_GRAD_W && !gather ? a0 + (size_t)t.p0 * g.NA : a0);
+    if (MODE == LN_GRAD_W) sb += 2 * ((size_t)t.p0 * g.NB + t.b0);
+    else if (MODE != LN_FWD || !g.perm) sb += 2 * (size_t)t.p0 * K;
+    uint32_t oa[CA], ob[CB], bad = 0;          /* bit i of bad: row i of B is of no pair */
+#pragma unroll
+    for (int i = 0; i < CA; ++i) {
+        const uint32_t r = ln_copy_row<TA, BA, WV>(i, lane, wave), u = ln_copy_unit<TA, BA, WV>(i, lane, wave);
+        if (MODE == LN_FWD) oa[i] = 2 * (GATED ? 16 * (r >> 5) + (r & 15) : r) * K + 16 * u;
+        else oa[i] = 2 * (gather ? 0 : r) * g.NA + 16 * u;
+    }
+#pragma unroll
+    for (int i = 0; i < CB; ++i) {
+        const uint32_t r = ln_copy_row<TB, BB, WV>(i, lane, wave), u = ln_copy_unit<TB, BB, WV>(i, lane, wave);
+        ob[i] = 2 * r * (MODE == LN_GRAD_W ? g.NB : K) + 16 * u;
+        if (MODE == LN_FWD && g.perm) {
+            const int row = ln_row(g, t.p0 + min((int)r, t.np - 1));
+            if (row < 0) bad |= 1u << i;
+            ob[i] = 2 * (uint32_t)max(row, 0) * K + 16 * u;
+        }
+    }
+    const bool any_bad = MODE == LN_FWD && __any(bad != 0);
+    /* the gathered rows of step s, asked for a step ahead of their copies; which of them are none, and
+     * which of the copies under way are */
+    int rows[MODE == LN_GRAD_W ? CA : 1];
+    uint32_t none = 0, flying = 0;
+    auto look = [&](int s) {
+        if constexpr (MODE == LN_GRAD_W) {
+            none = 0;
+#pragma unroll
+            for (int i = 0; i < CA; ++i) {
+                const int k = 64 * s + ln_copy_row<TA, BA, WV>(i, lane, wave);
+                rows[i] = k < K ? ln_row(g, t.p0 + k) : -1;
+                if (rows[i] < 0) none |= 1u << i;
+            }
+        }
+    };
+    auto left = [&](int s) { return K - 64 * (MODE == LN_GRAD_X && s >= nk ? s - nk : s); };
+    auto place = [](int s) { return (NS == 2 ? s & 1 : s % NS) * STAGE; };
+    uint32_t la = 0, lb = 0, lodd[NS - 1] = {};
+    const uint8_t *odd[NS - 1] = {};           /* of a matrix that is not aligned: bases and limits under way */
+    /* before the copies of step s */
+    auto turn = [&](int s) {
+        if (MODE == LN_GRAD_X && s == nk && s < steps) {
+            sa = m3 + 2 * a0;
+            ea = m3 + 2 * (size_t)g.NA * g.K;
+            sb = g.b3 + 2 * (size_t)t.p0 * K;
+            eb = g.b3 + 2 * (size_t)g.P * g.K;
+        }
+        /* a step past the last is copied all the same, one unit over and over, and not read */
+        if (s >= steps) {
+            sa = ea - 16;
+            sb = eb - 16;
+        }
+        la = (uint32_t)min((size_t)(ea - sa) - 16, (size_t)0xFFFFFFF0u);
+        lb = (uint32_t)min((size_t)(eb - sb) - 16, (size_t)0xFFFFFFF0u);
+    };
+    auto at_a = [&](int i) {
+        if (MODE == LN_GRAD_W && gather) return (uint32_t)max(rows[MODE == LN_GRAD_W ? i : 0], 0) * (2u * g.NA) + oa[i];
+        return oa[i];
+    };
+    auto copy_a = [&](int i) { ln_dma(MODE == LN_GRAD_W ? sa : (const uint8_t *)((uintptr_t)sa & ~(uintptr_t)15), min(at_a(i), la)); };
+    auto copy_b = [&](int i) { ln_dma(sb, min(ob[i], lb)); };
+    auto moved = [&]() {
+#pragma unroll
+        for (int i = 0; i < NS - 2; ++i) {
+            odd[i] = odd[i + 1];
+            lodd[i] = lodd[i + 1];
+        }
+        odd[NS - 2] = sa;
+        lodd[NS - 2] = la;
+        if (!gather) sa += TA ? (size_t)128 * g.NA : (size_t)128;
+        sb += TB ? (size_t)128 * g.NB : (size_t)128;
+        flying = none;
+    };
+    auto copy_to = [&](auto c_, uint32_t to) {
+        constexpr int C = decltype(c_)::value;
+        ln_dma_at<(C < CA ? 0 : 128 * BA) + 1024 * WV * (C < CA ? C : C - CA)>(to);
+        if constexpr (C < CA) copy_a(C);
+        else copy_b(C - CA);
+    };
+    auto copies = [&](int s) {
+        const uint32_t to = ldsp + place(s);
+        turn(s);
+        ln_each([&](auto c_) { copy_to(c_, to); }, std::make_integer_sequence<int, CA + CB>{});
+        moved();
+    };
+    /* what this wave's copies of step s brought that does not count, and what DMA could not bring */
+    auto fix = [&](int s) {
+        const int k = left(s);
+        if (s >= steps || (k >= 64 && aligned && !any_bad && !(gather && __any(flying != 0)))) return;
+        uint8_t *to = lds + place(s) + 1024 * wave + 16 * lane;
+#pragma unroll
+        for (int i = 0; i < CA; ++i) {
+            const int r = ln_copy_row<TA, BA, WV>(i, lane, wave), u = ln_copy_unit<TA, BA, WV>(i, lane, wave);
+            gm_v4u *o = (gm_v4u *)(to + 1024 * WV * i);
+            if (gather ? flying >> i & 1 : (TA ? r : 8 * u) >= k) *o = gm_v4u{0, 0, 0, 0};
+            else if (!aligned) *o = *(const LN_G(ln_any16) *)(odd[0] + min(oa[i], lodd[0]));
+        }
+#pragma unroll
+        for (int i = 0; i < CB; ++i) {
+            const int r = ln_copy_row<TB, BB, WV>(i, lane, wave), u = ln_copy_unit<TB, BB, WV>(i, lane, wave);
+            if ((TB ? r : 8 * u) >= k || (bad >> i & 1)) *(gm_v4u *)(to + 128 * BA + 1024 * WV * i) = gm_v4u{0, 0, 0, 0};
+        }
+        /* no load is pending behind this: the compiler would wait for it, and so for all copies, below */
+        gm_wait_vm<0>();
+    };
+
+    k3v4f acc[MA][MB], sums[MB];
+#pragma unroll
+    for (int j = 0; j < MB; ++j) {
+        sums[j] = k3v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < MA; ++i) acc[i][j] = k3v4f{0.f, 0.f, 0.f, 0.f};
+    }
+    const bool bias = MODE == LN_GRAD_W && g.dbias && t.a0 == 0 && wa == 0;
+    const k3v8bf one = __builtin_bit_cast(k3v8bf, gm_v4u{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u});
+    k3v8bf fa[MA], fb[2][MB];
+    auto read_a = [&](int s, int kh, int i) { fa[i] = ln_frag<TA, BA>(lds + place(s), kh, MA * wa + i); };
+    auto read_b = [&](int s, int kh, int j) {
+        fb[kh][j] = ln_frag<TB, BB>(lds + place(s) + 128 * BA, kh, MB * wb + j);
+    };
+    constexpr int PLAN1 = LnPlan<MA, MB, CA + CB>::FIRST;
+    /* the products of half kh of step s and what goes on meanwhile: reads of the next half (of the next
+     * step after the barrier that the second half has), and copies: of step s + NS after that
+     * barrier, the rest in the next step's first half */
+    auto half = [&](auto kh_, int s) {
+        constexpr int KH = decltype(kh_)::value;
+        static constexpr LnPlan<MA, MB, CA + CB> plan(KH == 1);
+        const uint32_t to = ldsp + place(s + KH + NS - 1);
+        if (KH == 1) turn(s + NS);
+        ln_each([&](auto m_) {
+            constexpr int M = decltype(m_)::value, I = M / MB, J = M % MB, C = plan.copy[M];
+            constexpr int R0 = plan.read[M][0], R1 = plan.read[M][1];
+            ln_mfma<BIG>(fa[I], fb[KH][J], acc[I][J]);
+            if constexpr (C >= 0) copy_to(GmInt<C>{}, to);
+            if constexpr (KH == 1 && M == plan.BAR) {
+                ln_wait<(NS - 2) * (CA + CB)>();
+                fix(s + 1);
+                __syncthreads();
+            }
+            if constexpr (R0 >= MA) read_b(s + KH, 1 - KH, R0 - MA);
+            else if constexpr (R0 >= 0) read_a(s + KH, 1 - KH, R0);
+            if constexpr (R1 >= MA) read_b(s + KH, 1 - KH, R1 - MA);
+            else if constexpr (R1 >= 0) read_a(s + KH, 1 - KH, R1);
+            __builtin_amdgcn_sched_barrier(0);
+        }, std::make_integer_sequence<int, MA * MB>{});
+        if (bias) {
+#pragma unroll
+            for (int j = 0; j < MB; ++j) ln_mfma_v<BIG>(one, fb[KH][j], sums[j]);
+        }
+        if (KH == 0) moved();
+    };
+    if (steps) {
+        if (gather) look(0);
+        copies(0);
+        gm_wait_vm<0>();
+        /* arrived (and fixed) before the others are reckoned among those under way */
+        odd[0] = odd[NS - 2];
+        lodd[0] = lodd[NS - 2];
+        fix(0);
+        __syncthreads();
+#pragma unroll
+        for (int s = 1; s < NS - 1; ++s) copies(s);
+        if (gather) look(1);
+        turn(NS - 1);
+        ln_each([&](auto c_) { copy_to(c_, ldsp + place(NS - 1)); }, std::make_integer_sequence<int, PLAN1>{});
+#pragma unroll
+        for (int i = 0; i < MA; ++i) read_a(0, 0, i);
+#pragma unroll
+        for (int j = 0; j < MB; ++j) read_b(0, 0, j);
+        if (BIG) asm volatile("s_nop 7" : : : "memory");       /* the sums' zeros */
+        for (int s = 0; s < steps; ++s) {
+            half(GmInt<0>{}, s);
+            if (gather) look(s + 2);
+            half(GmInt<1>{}, s);
+        }
+        gm_wait_vm<0>();
+#pragma unroll
+        for (int i = 0; i < MA; ++i) ln_settle<BIG>(acc[i]);
+        if (MODE == LN_GRAD_W && BIG) {
+#pragma unroll
+            for (int j = 0; j < MB; ++j) asm volatile("" : "+v"(sums[j]));
+        }
+    }
+    __syncthreads();
+    if (bias && lane < 16) {
+#pragma unroll
+        for (int j = 0; j < MB; ++j) {
+            const int b = t.b0 + 16 * MB * wb + 16 * j + lane;
+            if (b >= g.NB) continue;
+            float *o = g.dbias + (size_t)t.e * g.NB + b;
+            *o = g.accumulate ? *o + sums[j][0] : sums[j][0];
+        }
+    }
+    const int valid = MODE == LN_GRAD_W ? g.NB - t.b0 : t.np;
+    ln_out<MODE, GATED, Y, MA, MB>(g, (float *)lds + wave * 16 * (16 * MA + 4), acc, out, t.e,
+                                   (size_t)(MODE == LN_GRAD_W ? t.b0 : t.p0) + 16 * MB * wb, valid - 16 * MB * wb,
+                                   t.a0 + FA / 2 * wa);
+}
+
+/* bf16 operands whose rows are whole units of 16 bytes, and enough of them: with few tiles a step lasts
+ * as long as its copies take to arrive, and the kernel for any types, many small workgroups with two
+ * steps in registers, is ahead; so it is where an expert's matrix is read for 64 rows or less, or its
+ * gradient made from 96 or less. us, bf16, that kernel and the better tiles:
+ *   1024 x 2048 by 2048 (128 tiles of 128 x 128)       21    33
+ *   512 x 7168 by 3584 (112)                           78    102
+ *   1024 x 7168 by 2 x 2048, gated (256)               126   100
+ *   2048 x 2048 by 2048 (256)                          38    34
+ *   256 experts, 4096 x 2048: 4, 16, 32, 64, 128 rows  631 775 837 1024 1324    693 857 936 1012 1226
+ *   gradient of 64 matrices 1408 x 2048: 16, 64, 96    155 215 219              186 225 222 */
+template <int MODE>
+static bool ln_tile_enough(const LnArgs &g, bool gated)
+{
+    const int mean = g.P / (g.E < g.P ? g.E : max(g.P, 1));
+    if (g.off && MODE == LN_FWD && mean <= 64) return false;
+    if (g.off && MODE == LN_GRAD_W && mean <= 96) return false;
+    return ln_count<MODE>(g, gated ? 64 : 128, 128) > 160;
+}
+
+bool ln_tile_takes(const LnArgs &g, int mode, bool gated, int adt, int bdt)
+{
+    if (adt != K3_WBF16 || bdt != K3_WBF16 || (g.NA % 8 && mode != LN_FWD) || (mode == LN_GRAD_W ? g.NB : g.K) % 8) return false;
+    /* a gathered row's place is a 32-bit offset */
+    if (g.perm && (size_t)g.T * (mode == LN_GRAD_W ? g.NA : g.K) * 2 > UINT32_MAX) return false;
+    if (k3h_misaligned(g.b, 16) || k3h_misaligned(g.b3, 16) || (mode == LN_GRAD_W && k3h_misaligned(g.a, 16))) return false;
+    return mode == LN_FWD ? ln_tile_enough<LN_FWD>(g, gated)
+         : mode == LN_GRAD_X ? ln_tile_enough<LN_GRAD_X>(g, false) : ln_tile_enough<LN_GRAD_W>(g, false);
+}
+
+/* 256 x 256 outputs, one workgroup a CU, or half of that (256 x 128; of matrices 128 x 128, two a CU)? A
+ * call lasts as long as the CU with the most; experts' tiles are uneven enough to make up for a last
+ * round that is not full. us, the two forms:
+ *   4096 x 7168 by 2 x 2048, gated                              174   211
+ *   gradient of the rows, 2 x 2048 -> 7168                      250   329
+ *   gradient of the matrix, 2048 x 7168                         103   165
+ *   4096 x 6 pairs by 64: of rows, 2 x 1408 -> 2048             452   394
+ *   of rows through the activation, 2048 -> 1408                410   367
+ *   of the matrices, 1408 x 2048                                268   298
+ *   4096 x 8 pairs by 384, 2048 -> 7168                         3460  2900 */
+template <int MODE>
+static bool ln_wide(const LnArgs &g, bool gated)
+{
+    const int fa = gated ? 128 : 256;
+    double wide = ln_count<MODE>(g, fa, 256) / 256, half;
+    if (MODE == LN_GRAD_W) half = ln_count<MODE>(g, 128, 128) / 512;
+    else half = ln_count<MODE>(g, fa, 128) / 256;
+    if (!g.off) {
+        wide = ceil(wide);
+        half = ceil(half);
+    }
+    return fmax(wide, 1.0) <= (MODE == LN_GRAD_W ? 0.65 : 0.55) * fmax(half, 1.0);
+}
+
+template <int MODE, bool GATED, typename Y>
+static int ln_tile_y(const char *who, const LnArgs &g, hipStream_t st)
+{
+    constexpr int FA = GATED ? 128 : 256;
+    if (ln_wide<MODE>(g, GATED)) return ln_launch<MODE>(who, k_ln_tile<MODE, GATED, Y, 256, 256, 8, 2>, g, FA, 256, 512, st);
+    if constexpr (MODE == LN_GRAD_W) return ln_launch<MODE>(who, k_ln_tile<MODE, GATED, Y, 128, 128, 4, 2>, g, 128, 128, 256, st);
+    else return ln_launch<MODE>(who, k_ln_tile<MODE, GATED, Y, 256, 128, 8, 3>, g, FA, 128, 512, st);
+}
+
+template <int MODE, bool GATED>
+static int ln_tile_m(const char *who, const LnArgs &g, int ydt, hipStream_t st)
+{
+    return ydt == K3_WBF16 ? ln_tile_y<MODE, GATED, uint16_t>(who, g, st) : ln_tile_y<MODE, GATED, float>(who, g, st);
+}
+
+int ln_run_tile(const char *who, const LnArgs &g, int mode, bool gated, int ydt, hipStream_t st)
+{
+    if (mode == LN_GRAD_X) return ln_tile_m<LN_GRAD_X, false>(who, g, ydt, st);
+    if (mode == LN_GRAD_W) return ln_tile_m<LN_GRAD_W, false>(who, g, ydt, st);
+    return gated ? ln_tile_m<LN_FWD, true>(who, g, ydt, st) : ln_tile_m<LN_FWD, false>(who, g, ydt, st);
+}
