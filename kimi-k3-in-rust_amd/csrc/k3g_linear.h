@@ -79,12 +79,21 @@ __device__ __forceinline__ k3v4f ln_get4(const T *p, int n) { return ln_values(l
  * reads them then 20 us, or 33 where they went past. */
 #define LN_STREAM ((size_t)256 << 20)
 
+/* between two empty statements, or the compiler makes one plain store of this and of the other branch's */
+template <typename V, typename P>
+__device__ __forceinline__ void ln_put_past(const V &v, P *p)
+{
+    asm volatile("" : : : "memory");
+    __builtin_nontemporal_store(v, p);
+    asm volatile("" : : : "memory");
+}
+
 __device__ __forceinline__ void ln_put4(float *p, int n, const k3v4f &v, bool stream)
 {
     LN_G(float) *g = (LN_G(float) *)p;
     if (n >= 4) {
         const gm_v4u u = __builtin_bit_cast(gm_v4u, v);
-        if (stream) __builtin_nontemporal_store(u, (LN_G(ln_any16) *)g);
+        if (stream) ln_put_past(u, (LN_G(ln_any16) *)g);
         else *(LN_G(ln_any16) *)g = u;
         return;
     }
@@ -98,7 +107,7 @@ __device__ __forceinline__ void ln_put4(uint16_t *p, int n, const k3v4f &v, bool
     LN_G(uint16_t) *g = (LN_G(uint16_t) *)p;
     const gm_v2u u = {k3d_bf16x2(v[0], v[1]), k3d_bf16x2(v[2], v[3])};
     if (n >= 4) {
-        if (stream) __builtin_nontemporal_store(u, (LN_G(ln_any8) *)g);
+        if (stream) ln_put_past(u, (LN_G(ln_any8) *)g);
         else *(LN_G(ln_any8) *)g = u;
         return;
     }

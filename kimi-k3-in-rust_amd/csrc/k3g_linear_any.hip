@@ -180,14 +180,24 @@ k_ln_any(const LnArgs g)
                 for (int j = 0; j < M; ++j)
 #pragma unroll
                     for (int i = 0; i < PB; ++i) fb[j][i] = ln_any_frag<RB, B>(lds + (PA + i) * LN_PLANE, h, M * wb + j);
+                k3v8bf fa[M][PA];
 #pragma unroll
-                for (int i = 0; i < M; ++i) {
-                    k3v8bf fa[PA];
+                for (int i = 0; i < M; ++i)
 #pragma unroll
-                    for (int p = 0; p < PA; ++p) fa[p] = ln_any_frag<RA, B>(lds + p * LN_PLANE, h, M * wa + i);
+                    for (int p = 0; p < PA; ++p) fa[i][p] = ln_any_frag<RA, B>(lds + p * LN_PLANE, h, M * wa + i);
+                /* one pair of pieces for every block before the next: a product that adds to the sums of the
+                 * one before waits for it */
 #pragma unroll
-                    for (int j = 0; j < M; ++j) ln_mma<PA, PB>(fa, fb[j], acc[i][j]);
-                }
+                for (int p = PA + PB - 2; p >= 0; --p)
+#pragma unroll
+                    for (int q = 0; q < PB; ++q) {
+                        if (p > 2 || p - q < 0 || p - q >= PA) continue;
+#pragma unroll
+                        for (int i = 0; i < M; ++i)
+#pragma unroll
+                            for (int j = 0; j < M; ++j)
+                                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i][p - q], fb[j][q], acc[i][j], 0, 0, 0);
+                    }
                 if (bias) {
                     k3v8bf one[1];
                     one[0] = __builtin_bit_cast(k3v8bf, gm_v4u{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u});

@@ -333,19 +333,28 @@ k_ln_tile(const LnArgs g)
         if (KH == 0) moved();
     };
     if (steps) {
-        if (gather) look(0);
-        copies(0);
-        gm_wait_vm<0>();
-        /* arrived (and fixed) before the others are reckoned among those under way */
-        odd[0] = odd[NS - 2];
-        lodd[0] = lodd[NS - 2];
-        fix(0);
-        __syncthreads();
+        /* all stages are asked for before the first is waited for; so are the gathered rows of both */
+        int rows1[MODE == LN_GRAD_W ? CA : 1];
+        uint32_t none1 = 0;
+        if (gather) {
+            look(1);
 #pragma unroll
-        for (int s = 1; s < NS - 1; ++s) copies(s);
-        if (gather) look(1);
+            for (int i = 0; i < (MODE == LN_GRAD_W ? CA : 1); ++i) rows1[i] = rows[i];
+            none1 = none;
+            look(0);
+        }
+#pragma unroll
+        for (int s = 0; s < NS - 1; ++s) copies(s);
+        if (gather) {
+#pragma unroll
+            for (int i = 0; i < (MODE == LN_GRAD_W ? CA : 1); ++i) rows[i] = rows1[i];
+            none = none1;
+        }
         turn(NS - 1);
         ln_each([&](auto c_) { copy_to(c_, ldsp + place(NS - 1)); }, std::make_integer_sequence<int, PLAN1>{});
+        ln_wait<(NS - 2) * (CA + CB) + PLAN1>();
+        fix(0);
+        __syncthreads();
 #pragma unroll
         for (int i = 0; i < MA; ++i) read_a(0, 0, i);
 #pragma unroll
