@@ -2,37 +2,37 @@
  * formulas). */
 #include "k3g_linear.h"
 
-/* B x B outputs by four waves, a quarter each: 128 x 128 with 32 k at a time, or, where that makes too
- * few workgroups, 64 x 64 with 64, by G = 2 such groups of waves that take the steps in turn and add
- * up their sums at the end. A thread's two units of each operand come to registers two of its steps
- * ahead, and are split into their pieces on the way to LDS, once a workgroup.
+/* B x B outputs by four waves, a quarter each, 32 k at a time; where that makes too few workgroups, by
+ * G such groups of waves that take the steps in turn and add up their sums at the end. A thread's units
+ * of each operand come to registers two of its steps ahead, and are split into their pieces on the way
+ * to LDS, once a workgroup.
  *
- * LDS: a plane of 8 KB for each piece. 128 x 32: as in k3g_linear.h. 64 x 64: rows of 128 bytes, of
- * contiguous k unit u of row r at slot u ^ (r % 8); rows k with the 32-byte piece c at slot
- * c ^ (k / 2 % 2 + 2 (k / 8 % 2)). Either way a read meets every bank once. */
-#define LN_PLANE 8192
-
+ * What bounds it with two fp32 operands is all of a step, one part after the other: of 34 us for 617
+ * rows' gradient of a matrix 709 x 1411, before it was split over groups, 9 went without the loads, 8
+ * without the split into pieces, 4 without the products, 25 without the steps. With many tiles it is the
+ * products, six for each of fp32 values: 5001 rows, 4999 -> 5003, 169 Tflop/s, or 1.01 P of bf16 products.
+ *
+ * LDS: a plane of 64 B bytes for each piece, as in k3g_linear.h. 64 values: rows k of 128 bytes with the
+ * 32-byte piece c at slot c ^ (k / 2 % 2 + 2 (k / 8 % 2)). Either way a read meets every bank once. */
 /* where unit u of row r (TR: k) lies */
 template <bool TR, int B>
 __device__ __forceinline__ int ln_any_at(int r, int u)
 {
-    if constexpr (B == 128) return TR ? 256 * r + ((16 * u) ^ (32 * ln_swap(r))) : ln_krow(r, u);
-    return 128 * r + (TR ? (16 * u) ^ (32 * (((r >> 1) & 1) | ((r >> 2) & 2))) : 16 * (u ^ (r & 7)));
+    if (!TR) return ln_krow(r, u);
+    return 2 * B * r + ((16 * u) ^ (32 * (B == 128 ? ln_swap(r) : ((r >> 1) & 1) | ((r >> 2) & 2))));
 }
 
-/* block i's operand of k 32 h .. 32 h + 31 */
+/* block i's operand */
 template <bool TR, int B>
-__device__ __forceinline__ k3v8bf ln_any_frag(const uint8_t *plane, int h, int i)
+__device__ __forceinline__ k3v8bf ln_any_frag(const uint8_t *plane, int i)
 {
-    if constexpr (B == 128) return TR ? ln_frag_t(plane, i) : ln_frag_k(plane, i);
-    const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
-    if constexpr (TR) {
-        const int k = 32 * h + 8 * q + (c >> 2), u = 2 * i + ((c & 3) >> 1), in = 8 * (c & 1);
-        const gm_v2u lo = ln_read_tr(plane + ln_any_at<true, B>(k, u) + in);
-        const gm_v2u hi = ln_read_tr(plane + ln_any_at<true, B>(k + 4, u) + in);
-        return __builtin_bit_cast(k3v8bf, gm_v4u{lo.x, lo.y, hi.x, hi.y});
-    }
-    return __builtin_bit_cast(k3v8bf, *(const gm_v4u *)(plane + ln_any_at<false, B>(16 * i + c, 4 * h + q)));
+    if constexpr (!TR) return ln_frag_k(plane, i);
+    if constexpr (B == 128) return ln_frag_t(plane, i);
+    const int lane = threadIdx.x & 63, c = lane & 15;
+    const int k = 8 * (lane >> 4) + (c >> 2), u = 2 * i + ((c & 3) >> 1), in = 8 * (c & 1);
+    const gm_v2u lo = ln_read_tr(plane + ln_any_at<true, B>(k, u) + in);
+    const gm_v2u hi = ln_read_tr(plane + ln_any_at<true, B>(k + 4, u) + in);
+    return __builtin_bit_cast(k3v8bf, gm_v4u{lo.x, lo.y, hi.x, hi.y});
 }
 
 template <int MODE, bool GATED, typename TA, typename TB, typename Y, int B, int G>
@@ -40,8 +40,9 @@ __global__ void __launch_bounds__(256 * G, 2)
 k_ln_any(const LnArgs g)
 {
     constexpr bool RA = MODE != LN_FWD, RB = MODE == LN_GRAD_W;        /* rows k */
-    constexpr int PA = ln_pieces<TA>, PB = ln_pieces<TB>, M = B / 32, BK = 4096 / B, H = BK / 32;
-    constexpr int STAGE = (PA + PB) * LN_PLANE, OUT = 4 * 16 * (16 * M + 4) * 4, JOIN = G > 1 ? 256 * (M * M + M) * 16 : 0;
+    constexpr int PA = ln_pieces<TA>, PB = ln_pieces<TB>, M = B / 32, BK = 32, U = B / 64;
+    constexpr int PLANE = 64 * B, STAGE = (PA + PB) * PLANE;
+    constexpr int OUT = 4 * 16 * (16 * M + 4) * 4, JOIN = (G - 1) * 256 * (M * M + M) * 16;
     constexpr int BYTES = G * STAGE > OUT ? G * STAGE : OUT;
     __shared__ __attribute__((aligned(16))) uint8_t lds_all[BYTES > JOIN ? BYTES : JOIN];
     constexpr int FA = GATED ? B / 2 : B;              /* outputs a of a tile */
@@ -69,12 +70,12 @@ k_ln_any(const LnArgs g)
     /* unit j of this thread: row (or k) and unit of the tile, what it reads next, how many values of it
      * there are whatever k (0: none) */
     constexpr int UA = (RA ? B : BK) / 8, UB = (RB ? B : BK) / 8;      /* units of a row */
-    int ra[2], ua[2], rb[2], ub[2], na[2], nb[2], xr[2];
-    const TA *pa[2];
-    const TB *pb[2];
+    int ra[U], ua[U], rb[U], ub[U], na[U], nb[U], xr[U];
+    const TA *pa[U];
+    const TB *pb[U];
     auto begin = [&](const TA *m1, const TA *m3, const TB *rows) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < U; ++j) {
             const int id = tid + 256 * j;
             ra[j] = id / UA;
             ua[j] = id % UA;
@@ -103,33 +104,33 @@ k_ln_any(const LnArgs g)
     /* the gathered rows of step s, asked for a step ahead of what reads them */
     auto look = [&](int s) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < U; ++j) {
             const int k = BK * s + ra[j];
             xr[j] = k < K ? ln_row(g, t.p0 + k) : -1;
         }
     };
-    LnUnit<TA> va[2][2];
-    LnUnit<TB> vb[2][2];
+    LnUnit<TA> va[2][U];
+    LnUnit<TB> vb[2][U];
     bool inside = false;                       /* every unit of this wave has its 8 values, k apart */
     auto fetch = [&](int s, int d) {
         const bool second = MODE == LN_GRAD_X && s >= nk;
         if (s < G || (second && s < nk + G)) {
             begin(second ? a3 : a1, a3, (const TB *)(second ? g.b3 : g.b));
-            inside = __all(na[0] == 8 && na[1] == 8 && nb[0] == 8 && nb[1] == 8);
+            inside = __all(na[0] == 8 && na[U - 1] == 8 && nb[0] == 8 && nb[U - 1] == 8);
         }
         const int k0 = BK * (second ? s - nk : s), left = s < steps ? K - k0 : 0;
         if (gather && s < G) look(s);
         const size_t ka = (size_t)k0 * (RA ? g.NA : 1), kb = (size_t)k0 * (RB ? g.NB : 1);
         if (inside && left >= BK && !gather) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            for (int j = 0; j < U; ++j) {
                 va[d][j] = ln_whole(pa[j] + ka);
                 vb[d][j] = ln_whole(pb[j] + kb);
             }
             return;
         }
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < U; ++j) {
             const TA *p = pa[j] + (gather ? (size_t)max(xr[j], 0) * g.NA : ka);
             int n = na[j];
             if (!RA) n = min(n, left - 8 * ua[j]);
@@ -150,6 +151,7 @@ k_ln_any(const LnArgs g)
         for (int j = 0; j < M; ++j) acc[i][j] = k3v4f{0.f, 0.f, 0.f, 0.f};
     }
     const bool bias = MODE == LN_GRAD_W && g.dbias && t.a0 == 0 && wa == 0;
+    /* a group's steps are those of its number, G apart; past the last: zeros */
     if (steps) {
         fetch(group, 0);
         fetch(group + G, 1);
@@ -158,75 +160,74 @@ k_ln_any(const LnArgs g)
 #pragma unroll
         for (int d = 0; d < 2; ++d) {
             if (s0 + G * d >= steps) break;
-            const int s = s0 + G * d + group;              /* past the last: zeros */
+            const int s = s0 + G * d + group;
             __syncthreads();
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            for (int j = 0; j < U; ++j) {
                 gm_v4u qa[PA], qb[PB];
                 ln_split(va[d][j], qa);
                 ln_split(vb[d][j], qb);
                 const int oa = ln_any_at<RA, B>(ra[j], ua[j]), ob = ln_any_at<RB, B>(rb[j], ub[j]);
 #pragma unroll
-                for (int i = 0; i < PA; ++i) *(gm_v4u *)(lds + i * LN_PLANE + oa) = qa[i];
+                for (int i = 0; i < PA; ++i) *(gm_v4u *)(lds + i * PLANE + oa) = qa[i];
 #pragma unroll
-                for (int i = 0; i < PB; ++i) *(gm_v4u *)(lds + (PA + i) * LN_PLANE + ob) = qb[i];
+                for (int i = 0; i < PB; ++i) *(gm_v4u *)(lds + (PA + i) * PLANE + ob) = qb[i];
             }
             __syncthreads();
             if (s0 + G * (d + 2) < steps) fetch(s + 2 * G, d);
+            k3v8bf fb[M][PB];
 #pragma unroll
-            for (int h = 0; h < H; ++h) {
-                k3v8bf fb[M][PB];
+            for (int j = 0; j < M; ++j)
 #pragma unroll
-                for (int j = 0; j < M; ++j)
+                for (int i = 0; i < PB; ++i) fb[j][i] = ln_any_frag<RB, B>(lds + (PA + i) * PLANE, M * wb + j);
+            k3v8bf fa[M][PA];
 #pragma unroll
-                    for (int i = 0; i < PB; ++i) fb[j][i] = ln_any_frag<RB, B>(lds + (PA + i) * LN_PLANE, h, M * wb + j);
-                k3v8bf fa[M][PA];
+            for (int i = 0; i < M; ++i)
 #pragma unroll
-                for (int i = 0; i < M; ++i)
+                for (int p = 0; p < PA; ++p) fa[i][p] = ln_any_frag<RA, B>(lds + p * PLANE, M * wa + i);
+            /* one pair of pieces for every block before the next: a product that adds to the sums of the
+             * one before waits for it */
 #pragma unroll
-                    for (int p = 0; p < PA; ++p) fa[i][p] = ln_any_frag<RA, B>(lds + p * LN_PLANE, h, M * wa + i);
-                /* one pair of pieces for every block before the next: a product that adds to the sums of the
-                 * one before waits for it */
+            for (int p = PA + PB - 2; p >= 0; --p)
 #pragma unroll
-                for (int p = PA + PB - 2; p >= 0; --p)
+                for (int q = 0; q < PB; ++q) {
+                    if (p > 2 || p - q < 0 || p - q >= PA) continue;
 #pragma unroll
-                    for (int q = 0; q < PB; ++q) {
-                        if (p > 2 || p - q < 0 || p - q >= PA) continue;
+                    for (int i = 0; i < M; ++i)
 #pragma unroll
-                        for (int i = 0; i < M; ++i)
-#pragma unroll
-                            for (int j = 0; j < M; ++j)
-                                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i][p - q], fb[j][q], acc[i][j], 0, 0, 0);
-                    }
-                if (bias) {
-                    k3v8bf one[1];
-                    one[0] = __builtin_bit_cast(k3v8bf, gm_v4u{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u});
-#pragma unroll
-                    for (int j = 0; j < M; ++j) ln_mma<1, PB>(one, fb[j], sums[j]);
+                        for (int j = 0; j < M; ++j)
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i][p - q], fb[j][q], acc[i][j], 0, 0, 0);
                 }
+            if (bias) {
+                k3v8bf one[1];
+                one[0] = __builtin_bit_cast(k3v8bf, gm_v4u{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u});
+#pragma unroll
+                for (int j = 0; j < M; ++j) ln_mma<1, PB>(one, fb[j], sums[j]);
             }
         }
     __syncthreads();
     if constexpr (G > 1) {
-        /* the second group's sums to the first */
+        /* the other groups' sums to the first, which adds them in their order */
+        constexpr int PART = 256 * (M * M + M);
         k3v4f *join = (k3v4f *)lds_all + tid;
         if (group) {
 #pragma unroll
             for (int i = 0; i < M; ++i) {
-                join[256 * (M * M + i)] = sums[i];
+                join[(group - 1) * PART + 256 * (M * M + i)] = sums[i];
 #pragma unroll
-                for (int j = 0; j < M; ++j) join[256 * (M * i + j)] = acc[i][j];
+                for (int j = 0; j < M; ++j) join[(group - 1) * PART + 256 * (M * i + j)] = acc[i][j];
             }
         }
         __syncthreads();
-        if (!group) {
+        if (!group)
 #pragma unroll
-            for (int i = 0; i < M; ++i) {
-                sums[i] += join[256 * (M * M + i)];
+            for (int k = 0; k < G - 1; ++k)
 #pragma unroll
-                for (int j = 0; j < M; ++j) acc[i][j] += join[256 * (M * i + j)];
-            }
-        }
+                for (int i = 0; i < M; ++i) {
+                    sums[i] += join[k * PART + 256 * (M * M + i)];
+#pragma unroll
+                    for (int j = 0; j < M; ++j) acc[i][j] += join[k * PART + 256 * (M * i + j)];
+                }
         __syncthreads();
         if (group) return;
     }
@@ -246,25 +247,34 @@ k_ln_any(const LnArgs g)
                                  t.a0 + FA / 2 * wa);
 }
 
-/* Which tile: 64 x 64 where 128 x 128 would make less than a workgroup a CU, or experts have too few
- * rows to fill them; two groups of waves where those make no more than that either. us, fp32 rows and
- * (forward, second gradient) fp32 matrices, tiles of 128, of 64 with one group, with two:
- *   617 rows, 709 -> 1411, gradient of the rows      57   30   20
- *   the same, of the matrix                          72   36   35
- *   617 x 6 pairs by 64 experts, 1411 -> 2 x 709     269  221  337 */
+/* Which tile: 128 x 128 where that makes four workgroups a CU, or the last round leaves too many CUs
+ * idle, and experts have the rows to fill them; else 64 x 64, by as many groups of waves as the number
+ * of tiles leaves room for. us, fp32 rows and matrices, tiles of 128, of 64 by one, two and four groups:
+ *   617 rows, 709 -> 1411, gradient of the rows (264 tiles of 64)       66   31   24   19
+ *   the same, of the matrix (276)                                       72   35   26   30
+ *   1500 rows, 1000 -> 2001, gradient of the matrix (512)              149   75   58   62
+ *   2100 rows, 2100 -> 2100 (1089; 289 of 128)                         166  161  161  199
+ *   617 x 6 pairs by 64 experts, 1411 -> 2 x 709 (2880)                275  225  246  321
+ *   5001 rows, 4999 -> 5003 (6241; 1600 of 128)                       1481 1744 1840
+ * In between neither side is the faster one everywhere (3000 rows, 2999 -> 2001, 384 of 128: 239, 269,
+ * 274; its gradient of the rows, 576: 375, 302, 297). */
 template <int MODE, bool GATED, typename TA, typename TB>
 static int ln_any_y(const char *who, const LnArgs &g, int ydt, hipStream_t st)
 {
     const int met = g.off ? (g.E < g.P ? g.E : g.P) : 1;
     const bool short_rows = MODE != LN_GRAD_W && g.off && g.P / met <= 64;
-    if (!short_rows && ln_count<MODE>(g, GATED ? 64 : 128, 128) >= 256)
+    if (!short_rows && ln_count<MODE>(g, GATED ? 64 : 128, 128) >= 1024)
         return ln_launch<MODE>(who, ydt == K3_WBF16 ? k_ln_any<MODE, GATED, TA, TB, uint16_t, 128, 1>
                                                     : k_ln_any<MODE, GATED, TA, TB, float, 128, 1>, g, GATED ? 64 : 128, 128, 256, st);
-    if (ln_count<MODE>(g, GATED ? 32 : 64, 64) > 256)
+    const double tiles = ln_count<MODE>(g, GATED ? 32 : 64, 64);
+    if (tiles > 2048)
         return ln_launch<MODE>(who, ydt == K3_WBF16 ? k_ln_any<MODE, GATED, TA, TB, uint16_t, 64, 1>
                                                     : k_ln_any<MODE, GATED, TA, TB, float, 64, 1>, g, GATED ? 32 : 64, 64, 256, st);
-    return ln_launch<MODE>(who, ydt == K3_WBF16 ? k_ln_any<MODE, GATED, TA, TB, uint16_t, 64, 2>
-                                                : k_ln_any<MODE, GATED, TA, TB, float, 64, 2>, g, GATED ? 32 : 64, 64, 512, st);
+    if (tiles > 256)
+        return ln_launch<MODE>(who, ydt == K3_WBF16 ? k_ln_any<MODE, GATED, TA, TB, uint16_t, 64, 2>
+                                                    : k_ln_any<MODE, GATED, TA, TB, float, 64, 2>, g, GATED ? 32 : 64, 64, 512, st);
+    return ln_launch<MODE>(who, ydt == K3_WBF16 ? k_ln_any<MODE, GATED, TA, TB, uint16_t, 64, 4>
+                                                : k_ln_any<MODE, GATED, TA, TB, float, 64, 4>, g, GATED ? 32 : 64, 64, 1024, st);
 }
 
 template <int MODE, bool GATED>
