@@ -598,9 +598,10 @@ int  k3g_grouped_mxfp4(const void *x, int xdt, int rows, int cols, const int32_t
  * (ydt, dxdt, dwdt), each free. Products of bf16 values are exact in the matrix cores; an fp32
  * operand enters them as three bf16 pieces that together are its 24 bits (values below 2^-110 lose
  * bits, as subnormals do), the products of two fp32 operands without the last three pairs of pieces
- * (below 2^-21 of a product, of either sign, 2^-26 as a rule: less than its rounding to fp32). Sums are fp32, what follows a product is computed on them, and each result is rounded
- * once, to nearest even. An infinity among fp32 values may give NaN where an infinite result would
- * be right; rows without one are not touched by it. */
+ * (below 2^-21 of a product, of either sign, 2^-26 as a rule: less than its rounding to fp32). Sums
+ * are fp32, what follows a product is computed on them, and each result is rounded once, to nearest
+ * even. An infinity among fp32 values may give NaN where an infinite result would be right, and so
+ * may a product past fp32's range; rows without one are not touched by it. */
 enum { K3G_ACT_NONE = 0, K3G_ACT_RELU = 1, K3G_ACT_SILU = 2, K3G_ACT_GELU = 3, K3G_ACT_GELU_TANH = 4,
        K3G_ACT_SITU = 5 };
 
@@ -656,8 +657,10 @@ int  k3g_grouped_grad_x(const void *dy, const void *dy3, int dydt, int rows, int
                         const void *const *w3, int w_step, int wdt, int cols, const K3gBack *back,
                         void *dx, int dxdt, void *stream);
 /* dw: the device address of expert 0's pointer to its gradient [n][cols], expert e's dw_step bytes
- * on; NULL for an expert whose gradients are not wanted (dbias has none for it either). dbias [n_experts][n] or NULL. dy: the sorted
- * rows' [places][n]; x, rows, perm, topk as in k3g_grouped. */
+ * on; NULL for an expert whose gradients are not wanted (dbias has none for it either). No two
+ * experts' gradients may overlap: one that is shared is the sum that the caller makes of both.
+ * dbias [n_experts][n] or NULL. dy: the sorted rows' [places][n]; x, rows, perm, topk as in
+ * k3g_grouped. */
 int  k3g_grouped_grad_w(const void *dy, int dydt, const void *x, int xdt, int rows, int n, int cols,
                         const int32_t *perm, int topk, const int32_t *off, int n_experts,
                         int accumulate, void *const *dw, int dw_step, int dwdt, float *dbias,

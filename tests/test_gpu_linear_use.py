@@ -315,3 +315,86 @@ def test_past_32_bits(gpu):
     for a in range(0, T, 40000):
         want += dy[a:a + 40000].double().t() @ x[a:a + 40000].double()
     assert torch.equal(dw.double(), want)
+
+
+TYPES = [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16")]
+
+
+def whole(gen, dt, *shape):
+    """Whole numbers from -3 to 3: sums of their products are exact in fp32."""
+    import torch
+    v = torch.randint(-3, 4, shape, device="cuda", generator=gen)
+    return v.to(torch.float32 if dt == "f32" else torch.bfloat16)
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("size", [500, 1101, 2999, 4103])
+def test_from_few_tiles_to_many(gpu, size, types):
+    """Squares of odd width, from few outputs to many: all three products, exactly"""
+    import torch
+    print(f"case: {size} x {size} x {size}, {types}", flush=True)
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(size)
+    L, (xdt, wdt) = k3moe.lib(), types
+    x, dy, w = whole(gen, xdt, size, size), whole(gen, xdt, size, size), whole(gen, wdt, size, size)
+    o, bias = torch.empty(size, size, device="cuda"), torch.empty(size, device="cuda")
+    ok(L.k3g_matmul(ptr(x), tag(x), size, size, ptr(w), None, tag(w), size, None, ptr(o), 0, stream()))
+    assert torch.equal(o.double(), x.double() @ w.double().t().contiguous())
+    ok(L.k3g_matmul_grad_x(ptr(dy), None, tag(dy), size, size, ptr(w), None, tag(w), size, None, ptr(o), 0, stream()))
+    assert torch.equal(o.double(), dy.double() @ w.double())
+    ok(L.k3g_matmul_grad_w(ptr(dy), tag(dy), ptr(x), tag(x), size, size, size, 0, ptr(o), 0, ptr(bias), stream()))
+    assert torch.equal(o.double(), dy.double().t().contiguous() @ x.double())
+    assert torch.equal(bias.double(), dy.double().sum(0))
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("pair", [False, True])
+@pytest.mark.parametrize("rows", [1, 2, 15, 16, 17, 31, 33, 48, 63, 64, 65])
+def test_few_rows(gpu, rows, pair, types):
+    """Up to a few rows by matrices of few features to many, with one product or two, exactly"""
+    import torch
+    print(f"case: {rows} rows, {types}, {'two products' if pair else 'one'}", flush=True)
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(rows)
+    L, (xdt, wdt) = k3moe.lib(), types
+    for K in (40, 130, 1100):
+        for n in (5, 333, 7001):
+            x, w, w3 = whole(gen, xdt, rows, K), whole(gen, wdt, n, K), whole(gen, wdt, n, K)
+            y, z, z3 = (torch.full((rows + 1, n), 7.0, device="cuda") for _ in range(3))
+            ep = k3moe.K3gEpilogue()
+            ep.act, ep.b1, ep.b2 = k3moe.K3G_ACT_SITU if pair else k3moe.K3G_ACT_RELU, UNCAPPED, UNCAPPED
+            ep.z, ep.z3 = ptr(z), ptr(z3) if pair else None
+            ok(L.k3g_matmul(ptr(x), tag(x), rows, K, ptr(w), ptr(w3) if pair else None, tag(w), n, C.byref(ep), ptr(y), 0,
+                            stream()))
+            want = x.double() @ w.double().t().contiguous()
+            assert torch.equal(z[:rows].double(), want)
+            if pair:
+                want3 = x.double() @ w3.double().t().contiguous()
+                assert torch.equal(z3[:rows].double(), want3)
+                # SwiGLU of exact factors: the sigmoid and two products, 2^-18 of it
+                s = want * torch.sigmoid(want) * want3
+                assert ((y[:rows].double() - s).abs() <= 2.0 ** -18 * s.abs() + 2.0 ** -100).all()
+            else:
+                assert torch.equal(y[:rows].double(), want.clamp(min=0))
+            for o in (y, z, z3):
+                assert (o[rows:] == 7).all()
+
+
+def test_a_matrix_for_several_experts(gpu):
+    """Experts may share a matrix; their gradients of the rows are each one's own."""
+    import torch
+    print("case: experts that share matrices", flush=True)
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(9)
+    L, P, K, n, E = k3moe.lib(), 190, 72, 104, 5
+    x, dy, w = whole(gen, "bf16", P, K), whole(gen, "bf16", P, n), whole(gen, "bf16", 2, n, K)
+    which = torch.tensor([0, 1, 0, 0, 1], device="cuda")
+    tw = w.data_ptr() + w.stride(0) * 2 * which
+    off = torch.tensor([0, 40, 41, 41, 150, 190], device="cuda", dtype=torch.int32)
+    y, dx = torch.empty(P, n, device="cuda"), torch.empty(P, K, device="cuda")
+    ok(L.k3g_grouped(ptr(x), 1, P, K, None, 1, ptr(off), E, ptr(tw), None, 8, 1, n, None, ptr(y), 0, stream()))
+    ok(L.k3g_grouped_grad_x(ptr(dy), None, 1, P, n, ptr(off), E, ptr(tw), None, 8, 1, K, None, ptr(dx), 0, stream()))
+    for e in range(E):
+        a, b, m = off[e].item(), off[e + 1].item(), w[which[e]].double()
+        assert torch.equal(y[a:b].double(), x[a:b].double() @ m.t().contiguous())
+        assert torch.equal(dx[a:b].double(), dy[a:b].double() @ m)
