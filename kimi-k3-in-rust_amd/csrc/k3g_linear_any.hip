@@ -2,24 +2,25 @@
  * formulas). */
 #include "k3g_linear.h"
 
-/* B x B outputs by four waves, a quarter each, 32 k at a time; where that makes too few workgroups, by
- * G such groups of waves that take the steps in turn and add up their sums at the end. A thread's units
- * of each operand come to registers two of its steps ahead, and are split into their pieces on the way
- * to LDS, once a workgroup.
+/* B x B outputs by four waves, a quarter each (32 x 32: by one), 32 k at a time; where that makes too
+ * few workgroups, by G such groups of waves that take the steps in turn and add up their sums at the
+ * end. A thread's units of each operand come to registers two of its steps ahead, and are split into
+ * their pieces on the way to LDS, once a workgroup.
  *
  * What bounds it with two fp32 operands is all of a step, one part after the other: of 34 us for 617
  * rows' gradient of a matrix 709 x 1411, before it was split over groups, 9 went without the loads, 8
  * without the split into pieces, 4 without the products, 25 without the steps. With many tiles it is the
  * products, six for each of fp32 values: 5001 rows, 4999 -> 5003, 169 Tflop/s, or 1.01 P of bf16 products.
  *
- * LDS: a plane of 64 B bytes for each piece, as in k3g_linear.h. 64 values: rows k of 128 bytes with the
- * 32-byte piece c at slot c ^ (k / 2 % 2 + 2 (k / 8 % 2)). Either way a read meets every bank once. */
+ * LDS: a plane of 64 B bytes for each piece, as in k3g_linear.h. 64 and 32 values: rows k of 128 and
+ * 64 bytes with the 32-byte piece c at slot c ^ (k / 2 % 2 + 2 (k / 8 % 2)) and c ^ (k / 8 % 2). Either
+ * way a read meets every bank once. */
 /* where unit u of row r (TR: k) lies */
 template <bool TR, int B>
 __device__ __forceinline__ int ln_any_at(int r, int u)
 {
     if (!TR) return ln_krow(r, u);
-    return 2 * B * r + ((16 * u) ^ (32 * (B == 128 ? ln_swap(r) : ((r >> 1) & 1) | ((r >> 2) & 2))));
+    return 2 * B * r + ((16 * u) ^ (32 * (B == 128 ? ln_swap(r) : B == 64 ? ((r >> 1) & 1) | ((r >> 2) & 2) : (r >> 3) & 1)));
 }
 
 /* block i's operand */
@@ -35,21 +36,25 @@ __device__ __forceinline__ k3v8bf ln_any_frag(const uint8_t *plane, int i)
     return __builtin_bit_cast(k3v8bf, gm_v4u{lo.x, lo.y, hi.x, hi.y});
 }
 
+/* threads of a group */
+template <int B> constexpr int ln_any_threads = B == 32 ? 64 : 256;
+
 template <int MODE, bool GATED, typename TA, typename TB, typename Y, int B, int G>
-__global__ void __launch_bounds__(256 * G, 2)
+__global__ void __launch_bounds__(ln_any_threads<B> * G, 2)
 k_ln_any(const LnArgs g)
 {
     constexpr bool RA = MODE != LN_FWD, RB = MODE == LN_GRAD_W;        /* rows k */
-    constexpr int PA = ln_pieces<TA>, PB = ln_pieces<TB>, M = B / 32, BK = 32, U = B / 64;
+    constexpr int PA = ln_pieces<TA>, PB = ln_pieces<TB>, N = ln_any_threads<B>, W = B == 32 ? 1 : 2;
+    constexpr int M = B / (16 * W), BK = 32, U = 4 * B / N;
     constexpr int PLANE = 64 * B, STAGE = (PA + PB) * PLANE;
-    constexpr int OUT = 4 * 16 * (16 * M + 4) * 4, JOIN = (G - 1) * 256 * (M * M + M) * 16;
+    constexpr int OUT = W * W * 16 * (16 * M + 4) * 4, JOIN = (G - 1) * N * (M * M + M) * 16;
     constexpr int BYTES = G * STAGE > OUT ? G * STAGE : OUT;
     __shared__ __attribute__((aligned(16))) uint8_t lds_all[BYTES > JOIN ? BYTES : JOIN];
     constexpr int FA = GATED ? B / 2 : B;              /* outputs a of a tile */
     LnTile t;
     if (!ln_tile<MODE, FA, B>(g, t)) return;
-    const int tid = threadIdx.x & 255, group = G > 1 ? gm_uniform(threadIdx.x >> 8) : 0;
-    const int lane = tid & 63, wave = gm_uniform(tid >> 6), wa = wave & 1, wb = wave >> 1;
+    const int tid = threadIdx.x % N, group = G > 1 ? gm_uniform(threadIdx.x / N) : 0;
+    const int lane = tid & 63, wave = gm_uniform(tid >> 6), wa = wave % W, wb = wave / W;
     uint8_t *lds = lds_all + group * STAGE;
     const TA *a1 = (const TA *)g.a, *a3 = (const TA *)g.a3;
     Y *out = (Y *)g.y;
@@ -60,7 +65,7 @@ k_ln_any(const LnArgs g)
         a1 = (const TA *)ln_matrix(g, g.a, t.e);
         if (g.a3) a3 = (const TA *)ln_matrix(g, g.a3, t.e);
         if (!a1 || (g.a3 && !a3)) {
-            ln_zeros<MODE, GATED, Y, 256 * G>(g, out, t.p0, t.np, t.a0, FA);
+            ln_zeros<MODE, GATED, Y, N * G>(g, out, t.p0, t.np, t.a0, FA);
             return;
         }
     }
@@ -76,7 +81,7 @@ k_ln_any(const LnArgs g)
     auto begin = [&](const TA *m1, const TA *m3, const TB *rows) {
 #pragma unroll
         for (int j = 0; j < U; ++j) {
-            const int id = tid + 256 * j;
+            const int id = tid + N * j;
             ra[j] = id / UA;
             ua[j] = id % UA;
             rb[j] = id / UB;
@@ -208,14 +213,14 @@ k_ln_any(const LnArgs g)
     __syncthreads();
     if constexpr (G > 1) {
         /* the other groups' sums to the first, which adds them in their order */
-        constexpr int PART = 256 * (M * M + M);
+        constexpr int PART = N * (M * M + M);
         k3v4f *join = (k3v4f *)lds_all + tid;
         if (group) {
 #pragma unroll
             for (int i = 0; i < M; ++i) {
-                join[(group - 1) * PART + 256 * (M * M + i)] = sums[i];
+                join[(group - 1) * PART + N * (M * M + i)] = sums[i];
 #pragma unroll
-                for (int j = 0; j < M; ++j) join[(group - 1) * PART + 256 * (M * i + j)] = acc[i][j];
+                for (int j = 0; j < M; ++j) join[(group - 1) * PART + N * (M * i + j)] = acc[i][j];
             }
         }
         __syncthreads();
@@ -224,9 +229,9 @@ k_ln_any(const LnArgs g)
             for (int k = 0; k < G - 1; ++k)
 #pragma unroll
                 for (int i = 0; i < M; ++i) {
-                    sums[i] += join[k * PART + 256 * (M * M + i)];
+                    sums[i] += join[k * PART + N * (M * M + i)];
 #pragma unroll
-                    for (int j = 0; j < M; ++j) acc[i][j] += join[k * PART + 256 * (M * i + j)];
+                    for (int j = 0; j < M; ++j) acc[i][j] += join[k * PART + N * (M * i + j)];
                 }
         __syncthreads();
         if (group) return;
@@ -235,7 +240,7 @@ k_ln_any(const LnArgs g)
         /* every row of the product with ones is the sums; lane c holds those of index c */
 #pragma unroll
         for (int j = 0; j < M; ++j) {
-            const int b = t.b0 + B / 2 * wb + 16 * j + lane;
+            const int b = t.b0 + 16 * M * wb + 16 * j + lane;
             if (b >= g.NB) continue;
             float *o = g.dbias + (size_t)t.e * g.NB + b;
             *o = g.accumulate ? *o + sums[j][0] : sums[j][0];
@@ -243,15 +248,19 @@ k_ln_any(const LnArgs g)
     }
     const int valid = MODE == LN_GRAD_W ? g.NB - t.b0 : t.np;
     ln_out<MODE, GATED, Y, M, M>(g, (float *)lds_all + wave * 16 * (16 * M + 4), acc, out, t.e,
-                                 (size_t)(MODE == LN_GRAD_W ? t.b0 : t.p0) + B / 2 * wb, valid - B / 2 * wb,
-                                 t.a0 + FA / 2 * wa);
+                                 (size_t)(MODE == LN_GRAD_W ? t.b0 : t.p0) + 16 * M * wb, valid - 16 * M * wb,
+                                 t.a0 + FA / W * wa);
 }
 
 /* Which tile: 128 x 128 where that makes four workgroups a CU, or the last round leaves too many CUs
  * idle, and experts have the rows to fill them; else 64 x 64, by as many groups of waves as the number
- * of tiles leaves room for. us, fp32 rows and matrices, tiles of 128, of 64 by one, two and four groups:
- *   617 rows, 709 -> 1411, gradient of the rows (264 tiles of 64)       66   31   24   19
- *   the same, of the matrix (276)                                       72   35   26   30
+ * of tiles leaves room for; 32 x 32 by eight waves where they are so few that these are at most a
+ * workgroup a CU. us, fp32 rows and matrices, tiles of 128, of 64 by one, two and four groups, of 32:
+ *   759 rows, 1632 -> 207 (48 tiles of 64)                                         29   18
+ *   500 rows, 500 -> 500, gradient of the matrix (64)                              15   10
+ *   640 rows, 700 -> 640 (100)                                                     17   23
+ *   617 rows, 709 -> 1411, gradient of the rows (230)                   66   31   24   19   42
+ *   the same, of the matrix (276)                                       72   35   26   30   51
  *   1500 rows, 1000 -> 2001, gradient of the matrix (512)              149   75   58   62
  *   2100 rows, 2100 -> 2100 (1089; 289 of 128)                         166  161  161  199
  *   617 x 6 pairs by 64 experts, 1411 -> 2 x 709 (2880)                275  225  246  321
@@ -267,6 +276,9 @@ static int ln_any_y(const char *who, const LnArgs &g, int ydt, hipStream_t st)
         return ln_launch<MODE>(who, ydt == K3_WBF16 ? k_ln_any<MODE, GATED, TA, TB, uint16_t, 128, 1>
                                                     : k_ln_any<MODE, GATED, TA, TB, float, 128, 1>, g, GATED ? 64 : 128, 128, 256, st);
     const double tiles = ln_count<MODE>(g, GATED ? 32 : 64, 64);
+    if (tiles <= 64)
+        return ln_launch<MODE>(who, ydt == K3_WBF16 ? k_ln_any<MODE, GATED, TA, TB, uint16_t, 32, 8>
+                                                    : k_ln_any<MODE, GATED, TA, TB, float, 32, 8>, g, GATED ? 16 : 32, 32, 512, st);
     if (tiles > 2048)
         return ln_launch<MODE>(who, ydt == K3_WBF16 ? k_ln_any<MODE, GATED, TA, TB, uint16_t, 64, 1>
                                                     : k_ln_any<MODE, GATED, TA, TB, float, 64, 1>, g, GATED ? 32 : 64, 64, 256, st);
