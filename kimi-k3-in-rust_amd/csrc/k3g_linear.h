@@ -270,8 +270,8 @@ __device__ __forceinline__ void ln_finish(const LnArgs &g, Y *out, size_t at, in
 /* A wave's sums (MA x MB blocks of 16 a x 16 b) out by way of LDS (16 x (16 MA + 4) floats of its
  * own), so that it reads and writes whole pieces of rows: rows row0 + 0 .. rows - 1, columns col0 on.
  * GATED: the blocks are the two matrices' in turn. Everything that 16 rows read from memory is asked
- * for in one or two goes, the first before their sums go to LDS (one piece of a row at a time, a residual of 4096 x 7168
- * took 50 of 248 us). */
+ * for in one or two goes, the first before their sums go to LDS (one piece of a row at a time, a
+ * residual of 4096 x 7168 took 50 of 248 us). */
 template <int MODE, bool GATED, typename Y, int MA, int MB>
 __device__ __forceinline__ void ln_out(const LnArgs &g, float *lds, const k3v4f (&acc)[MA][MB], Y *out, int e,
                                        size_t row0, int rows, int col0)
@@ -367,9 +367,9 @@ __device__ __forceinline__ bool ln_tile(const LnArgs &g, LnTile &t)
 
 /* ------------------------------------------------------------------- LDS tiles ----
  *
- * An operand's tile of 32 k, bf16: contiguous k: rows of 64 bytes, 16-byte unit u of row r at slot
- * u ^ (r / 2 % 4); contiguous a (or b): 32 rows k of 128 values, 256 bytes, the 32-byte piece c at
- * slot c ^ (k % 4 + 4 (k / 8 % 2)), which the transposing read takes four rows k of at once. */
+ * An operand's tile of 32 contiguous k, bf16: rows of 64 bytes, 16-byte unit u of row r at slot
+ * u ^ (r / 2 % 4). Of rows k, 128 values each: the 32-byte piece c at slot c ^ ln_swap(k), so that the
+ * four rows k that a transposing read takes at once lie in other banks. */
 __device__ __forceinline__ int ln_krow(int row, int u) { return 64 * row + 16 * (u ^ ((row >> 1) & 3)); }
 __device__ __forceinline__ int ln_swap(int k) { return (k & 3) | ((k >> 1) & 4); }
 
@@ -383,21 +383,6 @@ __device__ __forceinline__ gm_v2u ln_read_tr(const uint8_t *p)
 #else
     return gm_v2u{};
 #endif
-}
-
-/* block i's operand from a tile whose rows are k: lane (c, q) gets k = 8 q .. 8 q + 7 of index 16 i + c */
-__device__ __forceinline__ k3v8bf ln_frag_t(const uint8_t *tile, int i)
-{
-    const int lane = threadIdx.x & 63, k = 8 * (lane >> 4) + ((lane & 15) >> 2), at = 32 * i + 8 * (lane & 3);
-    const gm_v2u lo = ln_read_tr(tile + 256 * k + (at ^ (32 * ln_swap(k))));
-    const gm_v2u hi = ln_read_tr(tile + 256 * (k + 4) + (at ^ (32 * ln_swap(k + 4))));
-    return __builtin_bit_cast(k3v8bf, gm_v4u{lo.x, lo.y, hi.x, hi.y});
-}
-
-__device__ __forceinline__ k3v8bf ln_frag_k(const uint8_t *tile, int i)
-{
-    const int lane = threadIdx.x & 63;
-    return __builtin_bit_cast(k3v8bf, *(const gm_v4u *)(tile + ln_krow(16 * i + (lane & 15), lane >> 4)));
 }
 
 /* ------------------------------------------------------------------- launches ---- */

@@ -2,39 +2,47 @@
  * formulas). */
 #include "k3g_linear.h"
 
-/* B x B outputs by four waves, a quarter each (32 x 32: by one), 32 k at a time; where that makes too
- * few workgroups, by G such groups of waves that take the steps in turn and add up their sums at the
- * end. A thread's units of each operand come to registers two of its steps ahead, and are split into
- * their pieces on the way to LDS, once a workgroup.
+/* B x B outputs by four waves, a quarter each (32 x 32: by one), 32 or 64 k at a time; where that
+ * makes too few workgroups, by G such groups of waves that take the steps in turn and add up their
+ * sums at the end. A thread's units of each operand come to registers two of its steps ahead, and are
+ * split into their pieces on the way to LDS, once a workgroup.
  *
  * What bounds it with two fp32 operands is all of a step, one part after the other: of 34 us for 617
  * rows' gradient of a matrix 709 x 1411, before it was split over groups, 9 went without the loads, 8
- * without the split into pieces, 4 without the products, 25 without the steps. With many tiles it is the
- * products, six for each of fp32 values: 5001 rows, 4999 -> 5003, 169 Tflop/s, or 1.01 P of bf16 products.
+ * without the split into pieces, 4 without the products, 25 without the steps. With many tiles it is
+ * the products, six for each of fp32 values: 5001 rows, 4999 -> 5003, 1.48 ms, 169 Tflop/s, or 1.01 P
+ * of bf16 products. Where few rows meet many matrices it is the matrices' way in: 64 experts' 2 x 2048
+ * x 7168 in bf16, 3.0 GB, 511 us, 6.0 TB/s.
  *
- * LDS: a plane of 64 B bytes for each piece, as in k3g_linear.h. 64 and 32 values: rows k of 128 and
- * 64 bytes with the 32-byte piece c at slot c ^ (k / 2 % 2 + 2 (k / 8 % 2)) and c ^ (k / 8 % 2). Either
- * way a read meets every bank once. */
+ * LDS: a plane for each piece, of contiguous k as in k3g_linear.h (of 64 k: rows of 128 bytes, unit u
+ * of row r at slot u ^ (r % 8)), of rows k with the 32-byte piece c at slot c ^ (k % 4 + 4 (k / 8 % 2)),
+ * c ^ (k / 2 % 2 + 2 (k / 8 % 2)) or c ^ (k / 8 % 2) for 128, 64 and 32 values. Either way a read meets
+ * every bank once. */
 /* where unit u of row r (TR: k) lies */
-template <bool TR, int B>
+template <bool TR, int B, int BK>
 __device__ __forceinline__ int ln_any_at(int r, int u)
 {
-    if (!TR) return ln_krow(r, u);
+    if (!TR) return BK == 64 ? 128 * r + 16 * (u ^ (r & 7)) : ln_krow(r, u);
     return 2 * B * r + ((16 * u) ^ (32 * (B == 128 ? ln_swap(r) : B == 64 ? ((r >> 1) & 1) | ((r >> 2) & 2) : (r >> 3) & 1)));
 }
 
-/* block i's operand */
-template <bool TR, int B>
-__device__ __forceinline__ k3v8bf ln_any_frag(const uint8_t *plane, int i)
+/* block i's operand of k 32 h .. 32 h + 31 */
+template <bool TR, int B, int BK>
+__device__ __forceinline__ k3v8bf ln_any_frag(const uint8_t *plane, int h, int i)
 {
-    if constexpr (!TR) return ln_frag_k(plane, i);
-    if constexpr (B == 128) return ln_frag_t(plane, i);
-    const int lane = threadIdx.x & 63, c = lane & 15;
-    const int k = 8 * (lane >> 4) + (c >> 2), u = 2 * i + ((c & 3) >> 1), in = 8 * (c & 1);
-    const gm_v2u lo = ln_read_tr(plane + ln_any_at<true, B>(k, u) + in);
-    const gm_v2u hi = ln_read_tr(plane + ln_any_at<true, B>(k + 4, u) + in);
+    const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+    if constexpr (!TR)
+        return __builtin_bit_cast(k3v8bf, *(const gm_v4u *)(plane + ln_any_at<false, B, BK>(16 * i + c, 4 * h + q)));
+    const int k = 32 * h + 8 * q + (c >> 2), u = 2 * i + ((c & 3) >> 1), in = 8 * (c & 1);
+    const gm_v2u lo = ln_read_tr(plane + ln_any_at<true, B, BK>(k, u) + in);
+    const gm_v2u hi = ln_read_tr(plane + ln_any_at<true, B, BK>(k + 4, u) + in);
     return __builtin_bit_cast(k3v8bf, gm_v4u{lo.x, lo.y, hi.x, hi.y});
 }
+
+/* k of a step: where there are tiles enough for many workgroups a CU, whole lines of bf16 values (64
+ * experts of a row each by 2 x 2048 x 7168: 511 us, and 555 by 32; fp32, 617 x 6 pairs: 226, 232) */
+template <int B, int G>
+constexpr int ln_any_k = B == 64 && G == 1 ? 64 : 32;
 
 /* threads of a group */
 template <int B> constexpr int ln_any_threads = B == 32 ? 64 : 256;
@@ -45,8 +53,8 @@ k_ln_any(const LnArgs g)
 {
     constexpr bool RA = MODE != LN_FWD, RB = MODE == LN_GRAD_W;        /* rows k */
     constexpr int PA = ln_pieces<TA>, PB = ln_pieces<TB>, N = ln_any_threads<B>, W = B == 32 ? 1 : 2;
-    constexpr int M = B / (16 * W), BK = 32, U = 4 * B / N;
-    constexpr int PLANE = 64 * B, STAGE = (PA + PB) * PLANE;
+    constexpr int M = B / (16 * W), BK = ln_any_k<B, G>, U = B * BK / (8 * N);
+    constexpr int PLANE = 2 * B * BK, STAGE = (PA + PB) * PLANE;
     constexpr int OUT = W * W * 16 * (16 * M + 4) * 4, JOIN = (G - 1) * N * (M * M + M) * 16;
     constexpr int BYTES = G * STAGE > OUT ? G * STAGE : OUT;
     __shared__ __attribute__((aligned(16))) uint8_t lds_all[BYTES > JOIN ? BYTES : JOIN];
@@ -172,7 +180,7 @@ k_ln_any(const LnArgs g)
                 gm_v4u qa[PA], qb[PB];
                 ln_split(va[d][j], qa);
                 ln_split(vb[d][j], qb);
-                const int oa = ln_any_at<RA, B>(ra[j], ua[j]), ob = ln_any_at<RB, B>(rb[j], ub[j]);
+                const int oa = ln_any_at<RA, B, BK>(ra[j], ua[j]), ob = ln_any_at<RB, B, BK>(rb[j], ub[j]);
 #pragma unroll
                 for (int i = 0; i < PA; ++i) *(gm_v4u *)(lds + i * PLANE + oa) = qa[i];
 #pragma unroll
@@ -180,34 +188,37 @@ k_ln_any(const LnArgs g)
             }
             __syncthreads();
             if (s0 + G * (d + 2) < steps) fetch(s + 2 * G, d);
-            k3v8bf fb[M][PB];
 #pragma unroll
-            for (int j = 0; j < M; ++j)
+            for (int h = 0; h < BK / 32; ++h) {
+                k3v8bf fb[M][PB];
 #pragma unroll
-                for (int i = 0; i < PB; ++i) fb[j][i] = ln_any_frag<RB, B>(lds + (PA + i) * PLANE, M * wb + j);
-            k3v8bf fa[M][PA];
+                for (int j = 0; j < M; ++j)
 #pragma unroll
-            for (int i = 0; i < M; ++i)
+                    for (int i = 0; i < PB; ++i) fb[j][i] = ln_any_frag<RB, B, BK>(lds + (PA + i) * PLANE, h, M * wb + j);
+                k3v8bf fa[M][PA];
 #pragma unroll
-                for (int p = 0; p < PA; ++p) fa[i][p] = ln_any_frag<RA, B>(lds + p * PLANE, M * wa + i);
-            /* one pair of pieces for every block before the next: a product that adds to the sums of the
-             * one before waits for it */
+                for (int i = 0; i < M; ++i)
 #pragma unroll
-            for (int p = PA + PB - 2; p >= 0; --p)
+                    for (int p = 0; p < PA; ++p) fa[i][p] = ln_any_frag<RA, B, BK>(lds + p * PLANE, h, M * wa + i);
+                /* one pair of pieces for every block before the next: a product that adds to the sums of the
+                 * one before waits for it */
 #pragma unroll
-                for (int q = 0; q < PB; ++q) {
-                    if (p > 2 || p - q < 0 || p - q >= PA) continue;
+                for (int p = PA + PB - 2; p >= 0; --p)
 #pragma unroll
-                    for (int i = 0; i < M; ++i)
+                    for (int q = 0; q < PB; ++q) {
+                        if (p > 2 || p - q < 0 || p - q >= PA) continue;
 #pragma unroll
-                        for (int j = 0; j < M; ++j)
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i][p - q], fb[j][q], acc[i][j], 0, 0, 0);
+                        for (int i = 0; i < M; ++i)
+#pragma unroll
+                            for (int j = 0; j < M; ++j)
+                                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i][p - q], fb[j][q], acc[i][j], 0, 0, 0);
+                    }
+                if (bias) {
+                    k3v8bf one[1];
+                    one[0] = __builtin_bit_cast(k3v8bf, gm_v4u{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u});
+#pragma unroll
+                    for (int j = 0; j < M; ++j) ln_mma<1, PB>(one, fb[j], sums[j]);
                 }
-            if (bias) {
-                k3v8bf one[1];
-                one[0] = __builtin_bit_cast(k3v8bf, gm_v4u{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u});
-#pragma unroll
-                for (int j = 0; j < M; ++j) ln_mma<1, PB>(one, fb[j], sums[j]);
             }
         }
     __syncthreads();

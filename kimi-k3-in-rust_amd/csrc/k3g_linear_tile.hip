@@ -6,16 +6,24 @@
 
 #include "k3g_linear.h"
 
-/* ---- bf16 rows and matrices whose widths are multiples of 8: BA x BB outputs by four waves, a
- * quarter each, 64 k at a time. The tiles come to LDS by DMA, NS stages; an operand's fragments of
- * the next 32 k are read while the products of these 32 run, across the stages too, so a step has one
- * barrier, in its middle: before it every wave has read the last of this stage (into which the
- * copies for step NS after this one then go) and its own copies of the next stage have arrived.
+/* BA x BB outputs by eight waves (of matrices' gradients also 128 x 128 by four), MA x MB blocks of 16 x
+ * 16 each, 64 k at a time. The tiles come to LDS by DMA, NS stages; an operand's fragments of the next
+ * 32 k are read while the products of these 32 run, across the stages too, so a step has one barrier,
+ * in its middle: before it every wave has read the last of this stage (into which the copies for step
+ * NS after this one then go) and its own copies of the next stage have arrived.
  *
- * Rows of contiguous k are 128 bytes of LDS, unit u of row r at slot u ^ (r % 8); rows k of
- * contiguous a or b as in the tiles of 32 k above, 64 of them. */
-/* The 1 KB copies of an operand's stage by WV waves, WV i + wave the one of this wave: which row (TR: k) of the
- * tile this lane copies 16 bytes of, and which unit of it */
+ * Rows of contiguous k are 128 bytes of LDS, unit u of row r at slot u ^ (r % 8): a DMA of whole lines
+ * takes 19 cycles a KB and CU, one of rows of 64 bytes 29. Rows k of contiguous a or b lie with the
+ * 32-byte piece c at slot c ^ ln_swap(k).
+ *
+ * What bounds it: dense, the matrix cores, busy 64 % of all cycles and waited for most of the rest
+ * (4096 x 7168 by 2 x 2048, gated, values kept: 178 us, 1.35 Pflop/s; the library's plain products reach
+ * 1.3 to 1.47). Of experts' gradients, what there is to write and what a tile costs before its first
+ * and after its last product (about 5 and 4 us, with 6 steps in between on average: 64 matrices of 1408
+ * x 2048 from 24576 pairs, 344 us, 738 MB written, 0.41 Pflop/s). */
+
+/* The 1 KB copies of an operand's stage by WV waves, WV i + wave the one of this wave: which row (TR:
+ * k) of the tile this lane copies 16 bytes of, and which unit of it */
 template <bool TR, int B, int WV>
 __device__ __forceinline__ int ln_copy_row(int i, int lane, int wave)
 {
