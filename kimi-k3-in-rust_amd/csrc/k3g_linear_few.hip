@@ -155,13 +155,10 @@ static int ln_few_run(const char *who, const LnArgs &g, int ydt, hipStream_t st)
 }
 
 /* Row blocks, waves and blocks of places of a workgroup. us, bf16, weights not in the caches:
- *   U, WV, NB                       1, 8, 1   4, 4, 1   1, 8, 2   1, 8, 4   2, 4, 4   tiles of 128
- *   1 x 7168 by 2 x 2048, gated     14.5      37.5      15.9      20.4      24.3      105
- *   1 x 2048 by 7168                8.7       12.4      9.6       13.9      10.5      34
- *   24 x 7168 by 3584               27.9      38.2      22.0      24.5      31.1      107
- *   48 x 7168 by 3584               42.0      39.2      40.0      33.3      41.5      109
- *   64 x 7168 by 2 x 2048, gated    55        40        45        40        50        109
- *   64 x 2048 by 7168               28        23        25        23        16.6      39
+ *   U, WV, NB                       1, 8, 1   4, 4, 1   1, 8, 2   1, 8, 4
+ *   1 x 7168 by 2 x 2048, gated     14.5      37.5      15.9      20.4
+ *   1 x 2048 by 7168                8.7       12.4      9.6       13.9
+ *   24 x 7168 by 3584               27.9      38.2      22.0      24.5
  * Experts of about a row each and not too many columns (64 x 2 x 1408 by 2048, 16 tokens x 6) take
  * four row blocks and four waves, 82 us against 151 with one and eight and 89 with tiles (8 tokens x 8 by 2 x
  * 2048 x 7168: 564, 569 and 515, so the columns count). */
@@ -171,15 +168,26 @@ static int ln_few_t(const char *who, const LnArgs &g, int ydt, hipStream_t st)
     if (g.off) return ln_few_run<GATED, TA, TB, 4, 4, 1>(who, g, ydt, st);
     if (g.P <= 16) return ln_few_run<GATED, TA, TB, 1, 8, 1>(who, g, ydt, st);
     if (g.P <= 32) return ln_few_run<GATED, TA, TB, 1, 8, 2>(who, g, ydt, st);
-    /* two row blocks where that leaves most CUs a workgroup */
-    if ((g.NA + (GATED ? 15 : 31)) / (GATED ? 16 : 32) >= 192) return ln_few_run<GATED, TA, TB, 2, 4, 4>(who, g, ydt, st);
     return ln_few_run<GATED, TA, TB, 1, 8, 4>(who, g, ydt, st);
 }
 
+/* Up to 16 rows, up to 32 by not too many features, up to 64 where the columns are few too: the rows are
+ * read again for every 16 features. us, this kernel and the tiles of any types, bf16 and fp32:
+ *   1, 16 rows, 7168 -> 7168       19.7 37.6, 28.0 37.5     49 110, 62 113
+ *   1, 16 rows, 7168 -> 28672      72 96, 108 102           163 213, 213 219
+ *   32 rows, 7168 -> 3584          22.0 23.0                45 71
+ *   32 rows, 7168 -> 7168          39.8 39.5                86 115
+ *   32 rows, 7168 -> 10240         65 48                    125 118
+ *   32 rows, 4096 -> 32000         88 57                    200 141
+ *   64 rows, 500 -> 500            5.9 7.6                  7.6 9.3
+ *   64 rows, 1024 -> 4096          8.1 7.9                  13.9 13.7
+ *   64 rows, 7168 -> 3584          34 22                    71 70 */
 bool ln_few_takes(const LnArgs &g, int mode)
 {
     if (mode != LN_FWD) return false;
-    return g.off ? g.P <= 2 * (g.E < g.P ? g.E : g.P) && g.K <= 4096 : g.P <= 64;
+    if (g.off) return g.P <= 2 * (g.E < g.P ? g.E : g.P) && g.K <= 4096;
+    const int features = g.a3 ? 2 * g.NA : g.NA;
+    return g.P <= 16 || (g.P <= 32 && features <= 8192) || (g.P <= 64 && features <= 4096 && g.K <= 1024);
 }
 
 template <bool GATED>
