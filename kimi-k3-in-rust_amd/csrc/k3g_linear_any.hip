@@ -265,11 +265,13 @@ k_ln_any(const LnArgs g)
 
 /* Which tile: 128 x 128 where that makes four workgroups a CU, or the last round leaves too many CUs
  * idle, and experts have the rows to fill them; else 64 x 64, by as many groups of waves as the number
- * of tiles leaves room for; 32 x 32 by eight waves where they are so few that these are at most a
- * workgroup a CU. us, fp32 rows and matrices, tiles of 128, of 64 by one, two and four groups, of 32:
+ * of tiles leaves room for; 32 x 32 by eight waves where all of these run at once, one or, with four
+ * pieces' planes, two a CU. us, fp32 rows and matrices, tiles of 128, of 64 by one, two and four groups, of 32:
  *   759 rows, 1632 -> 207 (48 tiles of 64)                                         29   18
  *   500 rows, 500 -> 500, gradient of the matrix (64)                              15   10
- *   640 rows, 700 -> 640 (100)                                                     17   23
+ *   1767 rows, 160 -> 1440, gradient of the matrix (69; 225 of 32)                 32   18
+ *   640 rows, 700 -> 640 (100; 400 of 32)                                          17   23
+ *   the same with bf16 matrices                                                    13   12
  *   617 rows, 709 -> 1411, gradient of the rows (230)                   66   31   24   19   42
  *   the same, of the matrix (276)                                       72   35   26   30   51
  *   1500 rows, 1000 -> 2001, gradient of the matrix (512)              149   75   58   62
@@ -287,7 +289,8 @@ static int ln_any_y(const char *who, const LnArgs &g, int ydt, hipStream_t st)
         return ln_launch<MODE>(who, ydt == K3_WBF16 ? k_ln_any<MODE, GATED, TA, TB, uint16_t, 128, 1>
                                                     : k_ln_any<MODE, GATED, TA, TB, float, 128, 1>, g, GATED ? 64 : 128, 128, 256, st);
     const double tiles = ln_count<MODE>(g, GATED ? 32 : 64, 64);
-    if (tiles <= 64)
+    constexpr int ROOM = ln_pieces<TA> + ln_pieces<TB> <= 4 ? 512 : 256;
+    if (ln_count<MODE>(g, GATED ? 16 : 32, 32) <= ROOM)
         return ln_launch<MODE>(who, ydt == K3_WBF16 ? k_ln_any<MODE, GATED, TA, TB, uint16_t, 32, 8>
                                                     : k_ln_any<MODE, GATED, TA, TB, float, 32, 8>, g, GATED ? 16 : 32, 32, 512, st);
     if (tiles > 2048)
